@@ -319,7 +319,7 @@ int mn_mst_candidate_graph_f32(const float *means, const float *vars, int64_t c,
 /* ---------------------------------------------------------------------- */
 /* K2 — Laplacian assembly from kNN rows (CSR)                            */
 /* ---------------------------------------------------------------------- */
-enum mn_value_type { MN_F32 = 0, MN_F64 = 1 };
+enum mn_value_type { MN_F32 = 0, MN_F64 = 1, MN_BF16 = 2 /* item scores, softmax loss */ };
 enum mn_weight_kernel {
     MN_W_GIVEN = 0,    /* nbr_val already holds edge weights                    */
     MN_W_RATIONAL = 1  /* w = 1/(1+(dist/sigma)^p), dist <= eps, w > 1e-12
@@ -630,6 +630,73 @@ int mn_knn_cos_bf16_qc(const uint16_t *Q, int64_t nq, const uint16_t *C, int64_t
                        int64_t q_offset, int64_t c_offset, const mn_cos_opts *opts,
                        int32_t *out_idx, double *out_dist, double *out_w);
 int mn_bf16_last_stats(mn_knn_stats *out);
+
+/* ---------------------------------------------------------------------- */
+/* Item scores in 8 bits; softmax loss over an item table                 */
+/* ---------------------------------------------------------------------- */
+/* These calls have no counterpart in the reference.  They are made for a
+ * training or serving loop and differ from the rest of this header in one
+ * thing: they only ENQUEUE on `stream` and return (a kernel's own error shows
+ * at the caller's next synchronisation), take their workspace from the caller
+ * and may be captured into a graph.  A workspace must not be used by two calls
+ * that can run at the same time, two captured graphs that replay side by side
+ * among them; its contents mean nothing between calls.  Pointers to X, Q, C,
+ * codes and the workspace are 16-byte aligned (MN_EINVAL / MN_ECAP).  Matrices
+ * are row-major and dense but for codes, whose rows are `ld` bytes apart (a
+ * multiple of 16, >= d). */
+
+/* Per row a = max |x|: scale = a / 127, code = rint(x (127 / a)) (f32, ties to
+ * even), codes d .. ld - 1 of a row 0.  X [n][d] MN_F32 or MN_BF16.  A row of
+ * zeros: scale 0, codes 0.  A row with an infinity or a NaN: scale NaN (so
+ * every score with it is NaN), codes 0. */
+int mn_quantize_rows_i8(const void *X, int32_t x_type, int64_t n, int32_t d, int8_t *codes,
+                        int64_t ld, float *scale, void *stream);
+/* X [n][d] = code * scale, MN_F32, or rounded to MN_BF16. */
+int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const float *scale, int64_t n,
+                          int32_t d, void *X, int32_t x_type, void *stream);
+/* Y [m][n] (MN_F32, or rounded to MN_BF16) = (sum_k q_ik c_jk) q_scale[i]
+ * c_scale[j]: the sum exact, then rounded to f32 and multiplied in that order.
+ * d <= 131071.  What lies behind column d of a row of codes has no effect. */
+int mn_scores_i8_workspace(int64_t m, int32_t d, size_t *bytes);
+int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, const int8_t *C,
+                 int64_t ldc, const float *c_scale, int64_t n, int32_t d, void *Y, int32_t y_type,
+                 void *ws, size_t ws_bytes, void *stream);
+
+/* Softmax cross entropy of the queries Q [t][d] over the rows of C [v][d]
+ * (both MN_F32 or MN_BF16) with logits z = scale q.c, scale > 0; no [t][v]
+ * matrix is kept.  targets [t] (int64) hold global row ids, C's rows are the
+ * ids c_offset .. c_offset + v - 1 (c_offset 0: the whole table).  A row with a
+ * negative target has no part: loss 0, gradient 0, and what it holds (a NaN)
+ * reaches no other row.
+ * mn_softmax_stats writes per row rest = log sum exp z over the items but the
+ * target, zt = the target's logit (-inf where it is not among the rows here),
+ * loss = log(1 + exp(rest - zt)) (may be NULL; +inf where zt is -inf) and mean
+ * (2 floats, may be NULL) = the mean of loss over the rows that take part and 1
+ * / their number ((0, 1) when there is none).
+ * mn_softmax_merge joins the (rest, zt) [parts][t] of row ranges of a table to
+ * those of the whole.
+ * mn_softmax_backward takes the whole table's rest and zt, and grad: one value
+ * (grad_n 1) or one per row (grad_n t), times *grad_scale where that is not
+ * NULL (device).  It writes dC [v][d], this range's rows' gradient, and dQ
+ * [t][d], this range's part of the queries' (add up the ranges'); either may be
+ * NULL.  Types as Q and C.
+ * bf16: the entries (p - [target]) of the logits' gradient are rounded to bf16
+ * for the two products with C and Q (dQ gets the target's rounding back); sums
+ * are f32.  f32: products of three-way split bf16 values, to f32 accuracy.
+ * Results do not depend on the run: no atomics. */
+int mn_softmax_workspace(int64_t t, int64_t v, int32_t d, int32_t x_type, int32_t backward,
+                         size_t *bytes);
+int mn_softmax_stats(const void *Q, const void *C, int32_t x_type, int64_t t, int64_t v, int32_t d,
+                     const int64_t *targets, int64_t c_offset, float scale, float *rest, float *zt,
+                     float *loss, float *mean, void *ws, size_t ws_bytes, void *stream);
+int mn_softmax_merge(const float *rests, const float *zts, int64_t parts, int64_t t,
+                     const int64_t *targets, float *rest, float *zt, float *loss, float *mean,
+                     void *stream);
+int mn_softmax_backward(const void *Q, const void *C, int32_t x_type, int64_t t, int64_t v,
+                        int32_t d, const int64_t *targets, int64_t c_offset, float scale,
+                        const float *rest, const float *zt, const float *grad, int64_t grad_n,
+                        const float *grad_scale, void *dQ, void *dC, void *ws, size_t ws_bytes,
+                        void *stream);
 
 #ifdef __cplusplus
 }

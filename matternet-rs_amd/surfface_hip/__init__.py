@@ -5,12 +5,14 @@ Every op runs on the GPU through the C ABI; there is no CPU fallback.
 """
 from . import _lib
 from ._lib import MnError, lib
-from . import clustering, energy, graph, l2f64, laplacian, search, sorted_index, sparsification
+from . import clustering, energy, graph, l2f64, laplacian, scores, search, softmax, sorted_index, sparsification
 from .clustering import ClusteringOutput, ClusteringStage, nearest_centroid
 from .graph import (BuilderParams, EigenMaps, GraphFactory, GraphLaplacian, SparsityError,
                     build_laplacian_matrix, standardize_columns)
 from .l2f64 import (estimate_intrinsic_dimension, knn_l2_f64, nearest_subcentroid,
                     prepare_query_items_energy, topk_by_l2, topk_by_l2_rows)
+from .scores import Int8Rows, dequantize_rows, quantize_rows, scores_i8
+from .softmax import softmax_backward, softmax_loss, softmax_merge, softmax_stats
 from .search import (normalise_query_lambda, prepare_query_lambdas, search_lambda_aware,
                      search_lambda_aware_hybrid)
 from .sparsification import SfGrassSparsifier, sparsify_rows, sparsify_sfgrass_csr
@@ -39,4 +41,6 @@ __all__ = ["MnError", "lib", "clustering", "ClusteringOutput", "ClusteringStage"
            "SfGrassSparsifier", "sparsify_rows", "sparsify_sfgrass_csr", "search", "search_lambda_aware",
            "normalise_query_lambda", "prepare_query_lambdas",
            "search_lambda_aware_hybrid", "l2f64", "knn_l2_f64", "topk_by_l2", "topk_by_l2_rows",
-           "nearest_subcentroid", "prepare_query_items_energy", "estimate_intrinsic_dimension"]
+           "nearest_subcentroid", "prepare_query_items_energy", "estimate_intrinsic_dimension",
+           "scores", "Int8Rows", "quantize_rows", "dequantize_rows", "scores_i8", "softmax",
+           "softmax_loss", "softmax_stats", "softmax_merge", "softmax_backward"]

@@ -54,7 +54,7 @@ class KnnStats(C.Structure):
         return {f: getattr(self, f) for f, _ in self._fields_}
 
 
-MN_F32, MN_F64 = 0, 1
+MN_F32, MN_F64, MN_BF16 = 0, 1, 2
 MN_W_GIVEN, MN_W_RATIONAL = 0, 1
 MN_SYM_UNION, MN_SYM_MAX = 0, 1
 
@@ -164,6 +164,16 @@ SIGNATURES = {
                                          P, P]),
     "mn_search_lambda_aware_hybrid": (C.c_int, [P, I32, I64, I32, P, P, P, I64, I32,
                                                 C.c_double, P, P, P]),
+    "mn_quantize_rows_i8": (C.c_int, [P, I32, I64, I32, P, I64, P, P]),
+    "mn_dequantize_rows_i8": (C.c_int, [P, I64, P, I64, I32, P, I32, P]),
+    "mn_scores_i8_workspace": (C.c_int, [I64, I32, C.POINTER(C.c_size_t)]),
+    "mn_scores_i8": (C.c_int, [P, I64, P, I64, P, I64, P, I64, I32, P, I32, P, C.c_size_t, P]),
+    "mn_softmax_workspace": (C.c_int, [I64, I64, I32, I32, I32, C.POINTER(C.c_size_t)]),
+    "mn_softmax_stats": (C.c_int, [P, P, I32, I64, I64, I32, P, I64, C.c_float, P, P, P, P, P,
+                                   C.c_size_t, P]),
+    "mn_softmax_merge": (C.c_int, [P, P, I64, I64, P, P, P, P, P, P]),
+    "mn_softmax_backward": (C.c_int, [P, P, I32, I64, I64, I32, P, I64, C.c_float, P, P, P, I64, P,
+                                      P, P, P, C.c_size_t, P]),
 }
 MN_SPARSIFY_SFGRASS, MN_SPARSIFY_INLINE = 0, 1
 

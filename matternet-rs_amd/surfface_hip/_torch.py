@@ -1,6 +1,7 @@
 """Device-memory plumbing via PyTorch-ROCm (allocation and streams only)."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -15,6 +16,30 @@ def require_cuda(t: torch.Tensor, dtype, name: str, ndim: int | None = None) -> 
     if ndim is not None and t.dim() != ndim:
         raise ValueError(f"{name} must be {ndim}-D")
     return t.contiguous()
+
+
+def require_aligned(t: torch.Tensor, dtype, name: str, ndim: int | None = None) -> torch.Tensor:
+    """require_cuda, and a copy where the rows start off a 16-byte border (a
+    slice of a larger tensor) or another device than the current one holds them."""
+    t = require_cuda(t, dtype, name, ndim)
+    if t.device.index is not None and t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, another tensor of the call on cuda:{torch.cuda.current_device()}")
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+@contextlib.contextmanager
+def enqueue(stream, *tensors):
+    """For calls that return before their work is done: inside, `stream` is the
+    current one, so that what is allocated belongs to it, and the inputs' memory
+    is kept until its work on them is done."""
+    if stream is None:
+        yield
+        return
+    with torch.cuda.stream(stream):
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and t.device.type == "cuda":
+                t.record_stream(stream)
+        yield
 
 
 def ptr(t: torch.Tensor) -> C.c_void_p:
@@ -36,7 +61,7 @@ def _first_cuda(args, kwargs):
     for a in list(args) + list(kwargs.values()):
         if isinstance(a, torch.Tensor) and a.device.type == "cuda":
             return a.device
-        for v in (getattr(a, "indptr", None), getattr(a, "keys", None)):
+        for v in (getattr(a, "indptr", None), getattr(a, "keys", None), getattr(a, "codes", None)):
             if isinstance(v, torch.Tensor) and v.device.type == "cuda":
                 return v.device
     return None
