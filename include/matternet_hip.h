@@ -645,7 +645,7 @@ int mn_bf16_last_stats(mn_knn_stats *out);
  * are row-major and dense but for codes, whose rows are `ld` bytes apart (a
  * multiple of 16, >= d). */
 
-/* Per row a = max |x|: scale = a / 127, code = rint(x (127 / a)) (f32, ties to
+/* Per row a = max |x|: scale = a / 127, code = rint(x (127 (1 / a))) (f32, ties to
  * even), codes d .. ld - 1 of a row 0.  X [n][d] MN_F32 or MN_BF16.  A row of
  * zeros: scale 0, codes 0.  A row with an infinity or a NaN: scale NaN (so
  * every score with it is NaN), codes 0. */

@@ -1,16 +1,38 @@
 // mm_tiles.hpp — matrix products of the item scores (scores.hip) and of the
 // softmax loss (softmax.hip) on the matrix cores.
 //
-// Two forms, both with f32 (bf16 operands) or int32 (int8 operands) sums:
-//   k_nt   Y[i][j] = sum_k A[i][k] B[j][k]     (rows against rows)
-//   k_kn   Y[m][n] = sum_k A(m,k) B[k][n]      (A [m][k] or [k][m])
-// An epilogue object takes each wave's accumulators.
+//   k_nt   Y[i][j] = sum_k A[i][k] B[j][k]   (rows against rows): a block keeps
+//          256 rows of A and goes through a run of 256-row tiles of B
+//   k_kn   Y[m][n] = sum_k A(m,k) B[k][n]    (A [m][k] or [k][m]): one 256 x 256
+//          tile a block, the sum over k split over blockIdx.z
+// with f32 (bf16 operands) or int32 (int8 operands) sums; an epilogue object
+// takes each wave's accumulators.
 //
 // f32 operands come as three bf16 planes x = h + m + l (8 + 8 + 8 significant
 // bits: exact but for subnormal tails).  Their product is the sum of six bf16
 // products (hh, hm, mh, hl, lh, mm); what is left out (ml, lm, ll) is below
 // 2^-25 of |x||y|, the rounding of one f32 product.  The small ones are added
-// first.
+// first.  Six products at the bf16 rate are 2.7 times the f32 matrix rate.
+//
+// Schedule (both kernels).  Eight waves, each 64 (i, m) x 128 (j, n) = 4 x 8
+// tiles of 16 x 16: 128 accumulator registers.  A k-step is 64 bytes of k (32
+// bf16, 64 int8) of both operands, 32 KB, in a ring of four slots, filled three
+// steps ahead by loads that go to LDS directly.  Waves w and w + 4 share a SIMD
+// and run one barrier window apart: while one issues its 32 matrix
+// instructions, the other reads the next step's fragments and issues its four
+// loads, so the matrix pipe does not wait for LDS.  A slot is refilled in the
+// window after the one in which its last reads ended (lgkmcnt(0) before the
+// barrier); vmcnt(8) before a barrier leaves the newest two steps in flight, so
+// the step read after the next barrier has landed.  Past the last step the
+// loads repeat it into the slot that nobody reads any more: the count stays.
+//
+// LDS layouts, free of bank conflicts.  Rows of k: a row's k-step is 64 bytes,
+// piece c (16 bytes) of row r at c ^ 2 ((r >> s) & 1), s = 3 where a fragment's
+// 16 rows are consecutive, 4 where its quads of rows are 8 apart.  Rows of k by
+// columns ([k][256]): 512 bytes a row, read transposed (ds_read_b64_tr_b16:
+// lane l of 16 gives the address of four columns of row l >> 2 and gets column
+// l of the four rows); the 32-byte slot of 16 columns s of row k is at s ^
+// ((k & 3) | ((k >> 3) & 1) << 2).
 #pragma once
 #include "common.hpp"
 
@@ -19,10 +41,16 @@ namespace mm {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr int KBY = 64;  // bytes of a row in one k-step: 32 bf16 or 64 int8
+constexpr int TILE = 256;              // rows / columns of a tile
+constexpr int KBY = 64;                // bytes of k in a step
+constexpr int NSLOT = 4;
+constexpr int HALF = TILE * KBY;       // one operand's step, 16 KB
+constexpr int NT = 512;
 
 // planes of A and B in the six products, smallest first
 __device__ __forceinline__ int seg_a(int s) { return (0x001021 >> (4 * s)) & 3; }
@@ -30,127 +58,343 @@ __device__ __forceinline__ int seg_b(int s) { return (0x010201 >> (4 * s)) & 3; 
 
 struct Bf16 {
     typedef f32x4 acc_t;
-    static __device__ __forceinline__ acc_t mma(uint4 a, uint4 b, acc_t c) {
+    static __device__ __forceinline__ acc_t mma(u32x4 a, u32x4 b, acc_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                        __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
 };
 struct Int8 {
     typedef i32x4 acc_t;
-    static __device__ __forceinline__ acc_t mma(uint4 a, uint4 b, acc_t c) {
+    static __device__ __forceinline__ acc_t mma(u32x4 a, u32x4 b, acc_t c) {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
                                                      __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
     }
 };
 
-struct NtArgs {
-    const char *A;      // [nplane][m][lda], rows zero from their end to nk * KBY
-    const char *B;      // [nplane][n][ldb]; bytes past bmax + 16 are never read
-    int64_t lda, ldb;   // bytes
-    int64_t planeA, planeB;
-    int64_t m, n;
-    int nk;             // k-steps of KBY bytes
-    int nseg;           // 1, or 6 (f32 planes)
-    int bmax;           // last 16-byte piece of a row of B
+struct alignas(1024) Ring {
+    char b[NSLOT][2][HALF];  // [.][0]: i / m, [.][1]: j / n
 };
 
-// 128 x 128 tile, four waves of 64 x 64.
+__device__ __forceinline__ uint32_t lds_addr(const void *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
+}
+
+// 16 bytes a lane from base + voff to LDS at lds + 16 lane
+__device__ __forceinline__ void dma16(const char *base, int voff, uint32_t lds) {
+    const uint64_t a = (uint64_t)(uintptr_t)base;
+    u32x4 r;
+    r.x = __builtin_amdgcn_readfirstlane((uint32_t)a);
+    r.y = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
+    r.z = 0xffffffffu;
+    r.w = 0x00020000u;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r)
+                 : "memory", "m0");
+}
+// 4 bytes a lane
+__device__ __forceinline__ void dma4(const char *base, int voff, uint32_t lds) {
+    const uint64_t a = (uint64_t)(uintptr_t)base;
+    u32x4 r;
+    r.x = __builtin_amdgcn_readfirstlane((uint32_t)a);
+    r.y = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
+    r.z = 0xffffffffu;
+    r.w = 0x00020000u;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r)
+                 : "memory", "m0");
+}
+
+// the end of a barrier window
+__device__ __forceinline__ void window_end() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void read_window_end() {
+    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    window_end();
+}
+
+// block b of n so that each of the 8 XCDs (blocks go to them in turn) gets a
+// contiguous range: neighbours share operands in one L2
+__device__ __forceinline__ int xcd_range(int b, int n) {
+    const int q = n / 8, r = n % 8, x = b % 8;
+    return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + b / 8;
+}
+
+struct NtArgs {
+    const char *A;      // [planes][m][lda] bytes, rows zero from their end to nk * KBY
+    const char *B;      // [planes][n][ldb]; bytes past bmax + 16 of a row are never read
+    int64_t lda, ldb, planeA, planeB;
+    int64_t m, n;
+    int nk;             // k-steps of a row
+    int nseg;           // 1, or 6 (f32 planes)
+    int bmax;           // last 16-byte piece of a row of B
+    int panels, slices; // 256-row panels of A; runs of tiles of B
+    int tiles, run;     // tiles of B, tiles of a run
+};
+
+// How many runs the tiles of B are cut into for `panels` panels: the cut with
+// the least rounds of 256 blocks, a run costing its tiles and 0.3 for filling
+// the ring.
+inline void plan_runs(NtArgs &a) {
+    a.panels = (int)((a.m + TILE - 1) / TILE);
+    a.tiles = (int)((a.n + TILE - 1) / TILE);
+    double best = 1e300;
+    for (int run = 1; run <= a.tiles; run = run < 32 ? run + 1 : run + run / 16) {
+        const int64_t s = (a.tiles + run - 1) / run, blocks = s * a.panels;
+        const double cost = (double)((blocks + 255) / 256) * (run + 0.3);
+        if (blocks < (1 << 30) && cost < best * 0.999) {
+            best = cost;
+            a.run = run;
+        }
+    }
+    a.slices = (a.tiles + a.run - 1) / a.run;
+}
+
+// accumulator r of tile (f, g): row i = 16 f + (lane & 15) of the wave's 64,
+// column j = 32 (g >> 1) + 8 (lane >> 4) + 4 (g & 1) + r of its 128, so that a
+// lane holds 8 neighbours of a row in each pair of tiles
 template <class OP, class EPI>
-__global__ __launch_bounds__(256) void k_nt(NtArgs a, EPI epi, int64_t tiles_j) {
-    __shared__ uint4 sA[128][5], sB[128][5];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int64_t bi = blockIdx.x / tiles_j, bj = blockIdx.x % tiles_j;
-    const int64_t i0 = bi * 128, j0 = bj * 128;
-    typename OP::acc_t acc[4][4];
-#pragma unroll
-    for (int f = 0; f < 4; ++f)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) acc[f][g] = (typename OP::acc_t)(0);
-    for (int sg = 0; sg < a.nseg; ++sg) {
-        const char *A = a.A + (a.nseg == 1 ? 0 : seg_a(sg) * a.planeA);
-        const char *B = a.B + (a.nseg == 1 ? 0 : seg_b(sg) * a.planeB);
-        for (int k = 0; k < a.nk; ++k) {
-#pragma unroll
-            for (int e = tid; e < 512; e += 256) {
-                const int r = e >> 2, c = e & 3;
-                const int64_t ra = min(i0 + r, a.m - 1), rb = min(j0 + r, a.n - 1);
-                sA[r][c] = *reinterpret_cast<const uint4 *>(A + ra * a.lda + k * KBY + 16 * c);
-                sB[r][c] = *reinterpret_cast<const uint4 *>(B + rb * a.ldb + min(k * KBY + 16 * c, a.bmax));
+__global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
+    __shared__ Ring rg;
+    __shared__ typename EPI::Shared sh;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wi = w & 3, wj = w >> 2;
+    const int fr = lane & 15, fk = lane >> 4;
+    // four panels by eight runs on an XCD at a time
+    int v = xcd_range((int)blockIdx.x, (int)gridDim.x);
+    const int grp = v / (4 * a.slices);
+    v -= grp * 4 * a.slices;
+    const int gp = min(4, a.panels - 4 * grp);
+    const int slice = v / gp, panel = 4 * grp + v % gp;
+    const int64_t i0 = (int64_t)panel * TILE;
+    const int t0 = slice * a.run, t1 = min(a.tiles, t0 + a.run);
+    const int nstep = a.nk * a.nseg * (t1 - t0);
+
+    // ---- loads: wave w stages rows 32 w .. 32 w + 31 of both operands
+    const int r0 = 32 * w + (lane >> 2), r1 = r0 + 16;
+    const int ilast = (int)min<int64_t>(TILE - 1, a.m - 1 - i0);
+    const int pci = 16 * ((lane & 3) ^ (((r0 >> 3) & 1) << 1));  // r1: the same bit
+    const int pcj0 = 16 * ((lane & 3) ^ (((r0 >> 4) & 1) << 1)), pcj1 = 16 * ((lane & 3) ^ (((r1 >> 4) & 1) << 1));
+    const int vi0 = min(r0, ilast) * (int)a.lda + pci, vi1 = min(r1, ilast) * (int)a.lda + pci;
+    int vj0 = 0, vj1 = 0;
+    int st = t0, ss = 0, sk = 0;   // the staged step: tile, product, k
+    uint32_t slot = 0;
+    const char *pa, *pb;
+    auto bases = [&]() __attribute__((always_inline)) {
+        pa = a.A + i0 * a.lda + (a.nseg == 1 ? 0 : seg_a(ss) * a.planeA);
+        pb = a.B + (int64_t)st * TILE * a.ldb + (a.nseg == 1 ? 0 : seg_b(ss) * a.planeB);
+    };
+    auto rows_j = [&]() __attribute__((always_inline)) {
+        const int jlast = (int)min<int64_t>(TILE - 1, a.n - 1 - (int64_t)st * TILE);
+        vj0 = min(r0, jlast) * (int)a.ldb;
+        vj1 = min(r1, jlast) * (int)a.ldb;
+    };
+    bases();
+    rows_j();
+    const uint32_t li = lds_addr(&rg.b[0][0][32 * w * KBY]), lj = lds_addr(&rg.b[0][1][32 * w * KBY]);
+    auto issue = [&]() __attribute__((always_inline)) {
+        const int ko = sk * KBY;
+        const int left = a.bmax - ko;  // pieces past a row's last one repeat it
+        dma16(pa + ko, vi0, li + slot);
+        dma16(pa + ko, vi1, li + slot + 1024);
+        dma16(pb + ko, vj0 + min(pcj0, left), lj + slot);
+        dma16(pb + ko, vj1 + min(pcj1, left), lj + slot + 1024);
+        slot = (slot + 2 * HALF) & (NSLOT * 2 * HALF - 1);
+        if (++sk == a.nk) {
+            sk = 0;
+            if (++ss == a.nseg) {
+                ss = 0;
+                if (st + 1 < t1) {
+                    ++st;
+                    rows_j();
+                } else {  // past the end: the last step again
+                    ss = a.nseg - 1;
+                    sk = a.nk - 1;
+                }
             }
-            __syncthreads();
-            uint4 fa[4], fb[4];
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-                fa[f] = sA[64 * (w & 1) + 16 * f + (lane & 15)][lane >> 4];
-                fb[f] = sB[64 * (w >> 1) + 16 * f + (lane & 15)][lane >> 4];
-            }
+            bases();
+        }
+    };
+
+    typename OP::acc_t acc[4][8];
+    u32x4 fi[4], fj[8];
+    const char *ri = &rg.b[0][0][(64 * wi + fr) * KBY + 16 * (fk ^ (((fr >> 3) & 1) << 1))];
+    // row of fragment g: 32 (g >> 1) + 4 (g & 1) + 8 (fr >> 2) + (fr & 3)
+    const char *rj = &rg.b[0][1][(128 * wj + 8 * (fr >> 2) + (fr & 3)) * KBY + 16 * (fk ^ (((fr >> 3) & 1) << 1))];
+    epi.init(sh, i0 + 64 * wi, lane);
+    issue();
+    issue();
+    issue();
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    window_end();
+    if (wj) window_end();
+    int k = 0, t = t0;
+    const int per = a.nk * a.nseg;
+    for (int n = 0; n < nstep; ++n) {
+        if (k == 0) {
+            if (n) epi.tile(sh, acc, (int64_t)(t - 1) * TILE + 128 * wj, lane, (t - 1) & 1);
+            epi.fetch(sh, (int64_t)t * TILE, tid, t & 1);
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) acc[f][g] = OP::mma(fb[g], fa[f], acc[f][g]);
-            __syncthreads();
+                for (int g = 0; g < 8; ++g) acc[f][g] = (typename OP::acc_t)(0);
+        }
+        const int so = (n & (NSLOT - 1)) * 2 * HALF;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) fi[f] = *reinterpret_cast<const u32x4 *>(ri + so + 16 * f * KBY);
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+            fj[g] = *reinterpret_cast<const u32x4 *>(rj + so + (32 * (g >> 1) + 4 * (g & 1)) * KBY);
+        issue();
+        if (EPI::FETCH && per < 4) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        read_window_end();
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int g = 0; g < 8; ++g) acc[f][g] = OP::mma(fj[g], fi[f], acc[f][g]);
+        window_end();
+        if (++k == per) {
+            k = 0;
+            ++t;
         }
     }
-    // acc[f][g][r] = Y[i0w + 16 f + (lane & 15)][j0w + 16 g + 4 (lane >> 4) + r]
-    epi(acc, i0 + 64 * (w & 1), j0 + 64 * (w >> 1), lane);
+    if (!wj) window_end();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    epi.tile(sh, acc, (int64_t)(t1 - 1) * TILE + 128 * wj, lane, (t1 - 1) & 1);
+    epi.finish(sh, i0 + 64 * wi, slice * 2 + wj, lane);
 }
 
 struct KnArgs {
-    const uint16_t *A;  // [nplane][m][lda] (A_T false) or [nplane][k][lda] (A_T true)
-    const uint16_t *B;  // [nplane][k][ldb]
-    int64_t lda, ldb, planeA, planeB;
-    int64_t m, n, k;    // rows / columns past m, n, k are not used
-    int64_t kpart;      // k's per grid z
+    const char *A;      // [planes][m][lda] (A_T false) or [planes][k][lda] (A_T true); whole tiles exist
+    const char *B;      // [planes][k][ldb]; columns past ldb and rows past k are never read
+    int64_t lda, ldb, planeA, planeB;  // bytes; ldb a multiple of 16
+    int64_t k;          // rows of B; A's entries past k are zero
+    int steps;          // k-steps of 32 of a block (blockIdx.z takes the z-th run of them)
+    int steps_all;
     int nseg;
 };
 
-// 128 x 128 tile, four waves of 64 x 64; blockIdx.z takes k's [z kpart, +kpart).
+// accumulator r of tile (f, g): row m = 16 f + (lane & 15) of the wave's 64,
+// column n = 16 g + 4 (lane >> 4) + r of its 128
 template <bool A_T, class EPI>
-__global__ __launch_bounds__(256) void k_kn(KnArgs a, EPI epi) {
-    __shared__ uint16_t sA[128][40], sB[128][40];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int64_t m0 = (int64_t)blockIdx.x * 128, n0 = (int64_t)blockIdx.y * 128;
-    const int64_t kb = blockIdx.z * a.kpart, ke = min(a.k, kb + a.kpart);
-    f32x4 acc[4][4];
+__global__ __launch_bounds__(NT, 2) void k_kn(KnArgs a, EPI epi) {
+    __shared__ Ring rg;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wi = w & 3, wj = w >> 2;
+    const int fr = lane & 15, fk = lane >> 4;
+    const int64_t m0 = (int64_t)blockIdx.y * TILE, n0 = (int64_t)blockIdx.x * TILE;
+    const int s0 = (int)blockIdx.z * a.steps, s1 = min(a.steps_all, s0 + a.steps);
+    const int per = s1 - s0, nstep = max(0, per) * a.nseg;
+
+    // ---- loads.  [k][256]: wave w stages rows 4 w .. 4 w + 3 in two pieces of
+    // two rows; [256][k]: rows 32 w .. as k_nt
+    const int kr0 = 4 * w + (lane >> 5);  // the second piece: kr0 + 2
+    auto col = [&](int kr) __attribute__((always_inline)) {
+        const int f = (kr & 3) | (((kr >> 3) & 1) << 2);
+        return 16 * ((((lane & 31) >> 1) ^ f) * 2 + (lane & 1));
+    };
+    const int cj0 = (int)min<int64_t>(col(kr0), a.ldb - 16 - 2 * n0), cj1 = (int)min<int64_t>(col(kr0 + 2), a.ldb - 16 - 2 * n0);
+    const int64_t kstep = 32 * a.ldb;
+    int vi0, vi1;
+    int64_t astep;
+    if constexpr (A_T) {
+        vi0 = kr0 * (int)a.lda + col(kr0);
+        vi1 = (kr0 + 2) * (int)a.lda + col(kr0 + 2);
+        astep = 32 * a.lda;
+    } else {
+        const int r0 = 32 * w + (lane >> 2);
+        const int pc = 16 * ((lane & 3) ^ (((r0 >> 3) & 1) << 1));
+        vi0 = r0 * (int)a.lda + pc;
+        vi1 = (r0 + 16) * (int)a.lda + pc;
+        astep = KBY;
+    }
+    int ss = 0, sk = s0;
+    uint32_t slot = 0;
+    const char *pa, *pb;
+    auto bases = [&]() __attribute__((always_inline)) {
+        pa = a.A + (a.nseg == 1 ? 0 : seg_a(ss) * a.planeA) + (A_T ? 2 * m0 : m0 * a.lda) + sk * astep;
+        pb = a.B + (a.nseg == 1 ? 0 : seg_b(ss) * a.planeB) + 2 * n0 + sk * kstep;
+    };
+    bases();
+    const uint32_t li = lds_addr(&rg.b[0][0][2048 * w]), lj = lds_addr(&rg.b[0][1][2048 * w]);
+    auto issue = [&]() __attribute__((always_inline)) {
+        const int last = (int)min<int64_t>(31, a.k - 1 - (int64_t)sk * 32);
+        dma16(pa, vi0, li + slot);
+        dma16(pa, vi1, li + slot + 1024);
+        dma16(pb, min(kr0, last) * (int)a.ldb + cj0, lj + slot);
+        dma16(pb, min(kr0 + 2, last) * (int)a.ldb + cj1, lj + slot + 1024);
+        slot = (slot + 2 * HALF) & (NSLOT * 2 * HALF - 1);
+        pa += astep;
+        pb += kstep;
+        if (++sk == s1) {
+            if (ss + 1 < a.nseg) {
+                ++ss;
+                sk = s0;
+            } else {  // past the end: the last step again
+                sk = s1 - 1;
+            }
+            bases();
+        }
+    };
+
+    f32x4 acc[4][8];
 #pragma unroll
     for (int f = 0; f < 4; ++f)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) acc[f][g] = (f32x4)(0.f);
-    for (int sg = 0; sg < a.nseg; ++sg) {
-        const uint16_t *A = a.A + (a.nseg == 1 ? 0 : seg_a(sg) * a.planeA);
-        const uint16_t *B = a.B + (a.nseg == 1 ? 0 : seg_b(sg) * a.planeB);
-        for (int64_t k0 = kb; k0 < ke; k0 += 32) {
-            for (int e = tid; e < 128 * 32; e += 256) {
-                const int kk = e >> 7, c = e & 127;
-                const int64_t k = k0 + kk;
-                sB[c][kk] = k < ke && n0 + c < a.n ? B[k * a.ldb + n0 + c] : (uint16_t)0;
-                if (A_T) {
-                    sA[c][kk] = k < ke && m0 + c < a.m ? A[k * a.lda + m0 + c] : (uint16_t)0;
-                } else {
-                    const int r = e >> 5, q = e & 31;
-                    sA[r][q] = k0 + q < ke && m0 + r < a.m ? A[(m0 + r) * a.lda + k0 + q] : (uint16_t)0;
-                }
-            }
-            __syncthreads();
-            uint4 fa[4], fb[4];
+        for (int g = 0; g < 8; ++g) acc[f][g] = (f32x4)(0.f);
+    u32x4 fi[4], fj[8];
+    // transposed reads: row 8 fk + (fr >> 2) (and 4 below), 16-column slot s
+    const int fx = (fr >> 2) | ((fk & 1) << 2);
+    const int trow = (8 * fk + (fr >> 2)) * 512 + 8 * (fr & 3);
+    const char *ri = &rg.b[0][0][(64 * wi + fr) * KBY + 16 * (fk ^ (((fr >> 3) & 1) << 1))];
+    auto tr = [&](const char *half, int s) __attribute__((always_inline)) {
+        const char *p = half + trow + 32 * (s ^ fx);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * 512));
+        const uint2 a2 = __builtin_bit_cast(uint2, x), b2 = __builtin_bit_cast(uint2, y);
+        return (u32x4){a2.x, a2.y, b2.x, b2.y};
+    };
+    if (nstep > 0) {
+        issue();
+        issue();
+        issue();
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        window_end();
+        if (wj) window_end();
+        for (int n = 0; n < nstep; ++n) {
+            const int so = (n & (NSLOT - 1)) * 2 * HALF;
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
-                fa[f] = *reinterpret_cast<const uint4 *>(&sA[64 * (w & 1) + 16 * f + (lane & 15)][8 * (lane >> 4)]);
-                fb[f] = *reinterpret_cast<const uint4 *>(&sB[64 * (w >> 1) + 16 * f + (lane & 15)][8 * (lane >> 4)]);
+                if constexpr (A_T) fi[f] = tr(&rg.b[0][0][0] + so, 4 * wi + f);
+                else fi[f] = *reinterpret_cast<const u32x4 *>(ri + so + 16 * f * KBY);
             }
+#pragma unroll
+            for (int g = 0; g < 8; ++g) fj[g] = tr(&rg.b[0][1][0] + so, 8 * wj + g);
+            issue();
+            read_window_end();
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) acc[f][g] = Bf16::mma(fb[g], fa[f], acc[f][g]);
-            __syncthreads();
+                for (int g = 0; g < 8; ++g) acc[f][g] = Bf16::mma(fj[g], fi[f], acc[f][g]);
+            window_end();
         }
+        if (!wj) window_end();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    // acc[f][g][r] = Y[m0w + 16 f + (lane & 15)][n0w + 16 g + 4 (lane >> 4) + r]
-    epi(acc, m0 + 64 * (w & 1), n0 + 64 * (w >> 1), lane, (int)blockIdx.z);
+    epi(acc, m0 + 64 * wi, n0 + 128 * wj, lane, (int)blockIdx.z);
 }
 
 __device__ __forceinline__ uint16_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
 __device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
+    return (uint32_t)bf16_bits(x) | ((uint32_t)bf16_bits(y) << 16);
+}
 
 // x = h + m + l.  A finite x whose nearest bf16 is infinite takes the one
 // below; m and l of a non-finite x are 0.

@@ -1,7 +1,7 @@
 // scores.hip — rows in 8 bits with a scale per row, and the scores of
 // quantised queries against a quantised item table:
 //
-//     a_i = max_k |x_ik|,  scale_i = a_i / 127,  code_ik = rint(x_ik (127 / a_i))
+//     a_i = max_k |x_ik|,  scale_i = a_i / 127,  code_ik = rint(x_ik (127 (1 / a_i)))
 //     y_ij = (sum_k qcode_ik ccode_jk) qscale_i cscale_j
 //
 // The sums are exact (int32: 128 * 128 * d < 2^31 for d <= 131071); y is the
@@ -24,8 +24,8 @@ __device__ __forceinline__ float load_x<float>(const float *X, int64_t e) { retu
 template <>
 __device__ __forceinline__ float load_x<uint16_t>(const uint16_t *X, int64_t e) { return mm::bf16_value(X[e]); }
 
-// Below 2^-100 the reciprocal 127 / a would overflow: such a row is multiplied
-// by 2^64 first (exact).  A row of zeros has scale 0 and codes 0; a row that
+// Below 2^-100 the reciprocal 1 / a could overflow, above 2^100 be subnormal:
+// such a row is multiplied by 2^64 or 2^-64 first (exact where it matters).  A row of zeros has scale 0 and codes 0; a row that
 // holds an infinity or a NaN has scale NaN, which every score with it shows.
 template <typename T>
 __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64_t n, int d,
@@ -39,8 +39,8 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64
         for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
         float a = __uint_as_float(top);
         const bool finite = top < 0x7f800000u;
-        const float up = a < 0x1p-100f ? 0x1p64f : 1.f;
-        const float inv = finite && top != 0 ? 127.f / (a * up) : 0.f;
+        const float up = a < 0x1p-100f ? 0x1p64f : a > 0x1p100f ? 0x1p-64f : 1.f;
+        const float inv = finite && top != 0 ? 1.f / (a * up) * 127.f : 0.f;
         for (int k = lane; k < ld; k += 64) {
             float v = 0.f;
             if (k < d && finite) v = __builtin_rintf(load_x(X, i * d + k) * up * inv);
@@ -78,27 +78,64 @@ __global__ __launch_bounds__(256) void k_pad_codes(const int8_t *__restrict__ Q,
 
 template <typename T>
 struct ScoreEpi {
+    struct Shared {
+        float cs[2][mm::TILE];  // the items' scales of a tile, two tiles in turn
+    };
+    static constexpr bool FETCH = true;
     const float *qs, *cs;
     T *Y;
     int64_t m, n;
-    __device__ __forceinline__ void operator()(mm::i32x4 (&acc)[4][4], int64_t i0, int64_t j0, int lane) const {
+    float q[4];
+    int64_t i0_;
+    __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
+        i0_ = i0;
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-            const int64_t i = i0 + 16 * f + (lane & 15);
-            if (i >= m) continue;
-            const float s = qs[i];
+        for (int f = 0; f < 4; ++f) q[f] = qs[min(i0 + 16 * f + (lane & 15), m - 1)];
+    }
+    __device__ __forceinline__ void fetch(Shared &sh, int64_t j0, int tid, int par) {
+        const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+        if (w < 4)
+            mm::dma4((const char *)(cs + j0), 4 * (int)min<int64_t>(tid, n - 1 - j0), mm::lds_addr(&sh.cs[par][64 * w]));
+    }
+    __device__ __forceinline__ void tile(Shared &sh, mm::i32x4 (&acc)[4][8], int64_t j0, int lane, int par) {
+        const int jl = 8 * (lane >> 4);
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < 8; g += 2) {
+            const int64_t j = j0 + jl + 16 * g;
+            float c[8];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int64_t j = j0 + 16 * g + 4 * (lane >> 4) + r;
-                    if (j >= n) continue;
-                    const float v = (float)acc[f][g][r] * s * cs[j];
-                    if constexpr (sizeof(T) == 4) Y[i * n + j] = v;
-                    else Y[i * n + j] = mm::bf16_bits(v);
+            for (int q8 = 0; q8 < 8; ++q8) c[q8] = sh.cs[par][(int)(j0 & (mm::TILE - 1)) + jl + 16 * g + q8];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const int64_t i = i0_ + 16 * f + (lane & 15);
+                float x[8];
+#pragma unroll
+                for (int q8 = 0; q8 < 8; ++q8) x[q8] = (float)acc[f][g + (q8 >> 2)][q8 & 3] * q[f] * c[q8];
+                if (i >= m) continue;
+                T *p = Y + i * n + j;
+                if constexpr (sizeof(T) == 4) {
+                    if (j + 8 <= n) {
+                        __builtin_memcpy(p, x, 32);
+                    } else {
+#pragma unroll
+                        for (int q8 = 0; q8 < 8; ++q8)
+                            if (j + q8 < n) p[q8] = x[q8];
+                    }
+                } else {
+                    if (j + 8 <= n) {
+                        const uint4 y = make_uint4(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]),
+                                                   mm::bf16_pair(x[4], x[5]), mm::bf16_pair(x[6], x[7]));
+                        __builtin_memcpy(p, &y, 16);
+                    } else {
+#pragma unroll
+                        for (int q8 = 0; q8 < 8; ++q8)
+                            if (j + q8 < n) p[q8] = mm::bf16_bits(x[q8]);
+                    }
                 }
+            }
         }
     }
+    __device__ __forceinline__ void finish(Shared &, int64_t, int, int) {}
 };
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -161,6 +198,8 @@ extern "C" int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, 
     using namespace mn::i8;
     clear_error();
     MN_REQUIRE(m >= 0 && n >= 0 && d >= 1, MN_EINVAL, "mn_scores_i8: m >= 0, n >= 0, d >= 1 needed");
+    MN_REQUIRE(m <= INT_MAX - 1024 && n <= INT_MAX - 1024 && (m + 255) / 256 * ((n + 255) / 256) < (1 << 30), MN_ENOTSUP,
+               "mn_scores_i8: too many scores for one call");
     MN_REQUIRE(d <= 131071, MN_ENOTSUP, "mn_scores_i8: d > 131071 (an int32 sum could overflow)");
     MN_REQUIRE(ldq >= d && ldc >= d && ldq % 16 == 0 && ldc % 16 == 0, MN_EINVAL,
                "mn_scores_i8: row strides need to be >= d and multiples of 16");
@@ -192,14 +231,24 @@ extern "C" int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, 
     a.nk = ldp / mm::KBY;
     a.nseg = 1;
     a.bmax = (d + 15) / 16 * 16 - 16;
-    const int64_t ti = (m + 127) / 128, tj = (n + 127) / 128;
-    MN_REQUIRE(ti * tj < INT_MAX, MN_ENOTSUP, "mn_scores_i8: too many scores for one call");
+    mm::plan_runs(a);
+    const dim3 grid((unsigned)(a.panels * a.slices));
     if (y_type == MN_F32) {
-        ScoreEpi<float> epi = {q_scale, c_scale, (float *)Y, m, n};
-        hipLaunchKernelGGL((mm::k_nt<mm::Int8, ScoreEpi<float>>), dim3((unsigned)(ti * tj)), dim3(256), 0, s, a, epi, tj);
+        ScoreEpi<float> epi = {};
+        epi.qs = q_scale;
+        epi.cs = c_scale;
+        epi.Y = (float *)Y;
+        epi.m = m;
+        epi.n = n;
+        hipLaunchKernelGGL((mm::k_nt<mm::Int8, ScoreEpi<float>>), grid, dim3(mm::NT), 0, s, a, epi);
     } else {
-        ScoreEpi<uint16_t> epi = {q_scale, c_scale, (uint16_t *)Y, m, n};
-        hipLaunchKernelGGL((mm::k_nt<mm::Int8, ScoreEpi<uint16_t>>), dim3((unsigned)(ti * tj)), dim3(256), 0, s, a, epi, tj);
+        ScoreEpi<uint16_t> epi = {};
+        epi.qs = q_scale;
+        epi.cs = c_scale;
+        epi.Y = (uint16_t *)Y;
+        epi.m = m;
+        epi.n = n;
+        hipLaunchKernelGGL((mm::k_nt<mm::Int8, ScoreEpi<uint16_t>>), grid, dim3(mm::NT), 0, s, a, epi);
     }
     MN_KCHECK(s, "k_nt");
     return MN_OK;

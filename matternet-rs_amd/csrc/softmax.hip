@@ -53,43 +53,89 @@ __global__ __launch_bounds__(256) void k_pack(const void *__restrict__ X, int64_
     }
 }
 
-// A wave's 64 columns of logits: their largest and the sum of exp of the rest,
-// the target's left out, to part[column group][row]; the target's logit to zt.
+// Per lane and row the largest logit so far (m2, base 2, rounded: the number
+// that every exponent is taken from) and the sum of exp of the rest, the
+// target's left out; joined over the lanes and written per run of tiles and
+// half of the columns.  An element costs a max, an fma, an exp and an add: for
+// 768 columns of operands about a seventh of its time on the matrix pipe.
 struct StatsEpi {
+    struct Shared {};
+    static constexpr bool FETCH = false;
     float2 *part;
     float *zt;
     const int64_t *targets;
-    int64_t c_offset, t, v;
+    int64_t c_offset, t;
+    int v;
     float scale, scale2;  // scale2 = scale log2(e)
-    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][4], int64_t i0, int64_t j0, int lane) const {
-        if (j0 >= v) return;
+    int at[4];
+    float m2[4], sum[4];
+    int64_t row0;
+    __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
+        row0 = i0 + (lane & 15);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            const int64_t i = i0 + 16 * f + (lane & 15);
-            int64_t at = -1;
-            if (i < t && targets[i] >= 0) at = targets[i] - c_offset;
-            float top = -__builtin_inff();
+            const int64_t i = row0 + 16 * f, x = i < t ? targets[i] : -1;
+            at[f] = x >= c_offset && x - c_offset < v ? (int)(x - c_offset) : -1;
+            m2[f] = -__builtin_inff();
+            sum[f] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
+    __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][8], int64_t j0, int lane, int) {
+        const int jw = (int)j0, jl = jw + 8 * (lane >> 4);
+        bool hit = jw + 128 > v;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+        for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 128u;
+        if (__ballot(hit)) {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                float z = 0.f;
+                bool mine = false;
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = jl + 32 * (g >> 1) + 4 * (g & 1) + r;
+                        z = j == at[f] ? acc[f][g][r] : z;
+                        mine = mine || j == at[f];
+                        acc[f][g][r] = j >= v || j == at[f] ? -__builtin_inff() : acc[f][g][r];
+                    }
+                if (mine) zt[row0 + 16 * f] = z * scale;
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            float top = acc[f][0][0];
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[f][g][r]);
+            const float m = fmaxf(m2[f], top * scale2);
+            const float mz = m == -__builtin_inff() ? 0.f : m;
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int g = 0; g < 8; g += 2)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int64_t j = j0 + 16 * g + 4 * (lane >> 4) + r;
-                    if (j == at && j < v && at >= 0) zt[i] = acc[f][g][r] * scale;
-                    if (j >= v || j == at) acc[f][g][r] = -__builtin_inff();
-                    top = fmaxf(top, acc[f][g][r]);
+                    s0 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g][r], scale2, -mz));
+                    s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g + 1][r], scale2, -mz));
                 }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float m2 = top == -__builtin_inff() ? 0.f : top * scale2;
-            float sum = 0.f;
+            sum[f] = sum[f] * __builtin_amdgcn_exp2f(m2[f] - mz) + (s0 + s1);
+            m2[f] = m;
+        }
+    }
+    __device__ __forceinline__ void finish(Shared &, int64_t, int piece, int lane) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+        for (int f = 0; f < 4; ++f) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g][r], scale2, -m2));
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (lane < 16 && i < t)
-                part[(j0 / 64) * t + i] = make_float2(top == -__builtin_inff() ? top : m2, sum);
+            for (int o = 16; o <= 32; o <<= 1) {
+                const float mo = __shfl_xor(m2[f], o), so = __shfl_xor(sum[f], o);
+                const float m = fmaxf(m2[f], mo), mz = m == -__builtin_inff() ? 0.f : m;
+                sum[f] = sum[f] * __builtin_amdgcn_exp2f(m2[f] - mz) + so * __builtin_amdgcn_exp2f(mo - mz);
+                m2[f] = m;
+            }
+            const int64_t i = row0 + 16 * f;
+            if (lane < 16 && i < t) part[piece * t + i] = make_float2(m2[f], sum[f]);
         }
     }
 };
@@ -232,63 +278,106 @@ __global__ __launch_bounds__(256) void k_rows(const float *__restrict__ rest, co
     at[i] = a;
 }
 
-// D of a piece of the table, [tp][ldd] (three planes for f32 operands)
+// D of a piece of the table, [tp][ldd] (three planes for f32 operands); zeros
+// in the rows and columns that only fill tiles.
 template <int PLANES>
 struct DlogitsEpi {
+    struct Shared {};
+    static constexpr bool FETCH = false;
     uint16_t *D;
-    int64_t ldd, plane, tp, v;  // v: columns of this piece that exist
+    int64_t ldd, plane;
+    int v;  // columns of this piece that exist
     const Row *row;
-    const int32_t *at;
+    const int32_t *at_;
     int64_t j_first;
     float scale2;
-    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][4], int64_t i0, int64_t j0, int lane) const {
+    int at[4];
+    float rel[4], lse2[4], dt[4];
+    bool any;
+    int64_t i0_;
+    __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
+        any = false;
+        i0_ = i0;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             const int64_t i = i0 + 16 * f + (lane & 15);
-            if (i >= tp) continue;
             const Row r = row[i];
-            const int64_t a = at[i] < 0 ? -1 : at[i] - j_first;
+            rel[f] = r.rel;
+            lse2[f] = r.lse2;
+            dt[f] = r.dt;
+            const int64_t a = at_[i] - j_first;
+            at[f] = at_[i] >= 0 && a >= 0 && a < v ? (int)a : -1;
+            any = any || r.rel != 0.f;
+        }
+        any = __ballot(any) != 0;
+    }
+    __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
+    __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][8], int64_t j0, int lane, int) {
+        const int jw = (int)j0, jl = 8 * (lane >> 4);
+        bool hit = jw + 128 > v || !any;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+        for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 128u;
+        const bool slow = __ballot(hit) != 0;
+        uint16_t *base = D + i0_ * ldd + j0;
+        const int lrow = (lane & 15) * (int)ldd + jl;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t j = j0 + 16 * g + 4 * (lane >> 4) + q;
-                    if (j >= ldd) continue;
-                    float x = r.rel * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g][q], scale2, -r.lse2));
-                    if (j == a) x = r.dt;
-                    if (j >= v || r.rel == 0.f) x = 0.f;
-                    if constexpr (PLANES == 1) {
-                        D[i * ldd + j] = mm::bf16_bits(x);
-                    } else {
-                        uint16_t p[3];
-                        mm::split3(x, p);
+        for (int f = 0; f < 4; ++f) {
 #pragma unroll
-                        for (int s = 0; s < 3; ++s) D[s * plane + i * ldd + j] = p[s];
+            for (int g = 0; g < 8; g += 2) {
+                float x[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    x[q] = rel[f] * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g + (q >> 2)][q & 3], scale2, -lse2[f]));
+                if (slow) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const int j = jw + jl + 16 * g + q;
+                        if (j == at[f]) x[q] = dt[f];
+                        if (j >= v || !any) x[q] = 0.f;
                     }
                 }
+                uint16_t *p = base + (int64_t)16 * f * ldd + (lrow + 16 * g);
+                if constexpr (PLANES == 1) {
+                    *reinterpret_cast<uint4 *>(p) = make_uint4(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]),
+                                                               mm::bf16_pair(x[4], x[5]), mm::bf16_pair(x[6], x[7]));
+                } else {
+                    uint32_t o[3][4];
+#pragma unroll
+                    for (int q = 0; q < 8; q += 2) {
+                        uint16_t a[3], b[3];
+                        mm::split3(x[q], a);
+                        mm::split3(x[q + 1], b);
+#pragma unroll
+                        for (int s = 0; s < 3; ++s) o[s][q / 2] = (uint32_t)a[s] | ((uint32_t)b[s] << 16);
+                    }
+#pragma unroll
+                    for (int s = 0; s < 3; ++s)
+                        *reinterpret_cast<uint4 *>(p + s * plane) = make_uint4(o[s][0], o[s][1], o[s][2], o[s][3]);
+                }
+            }
         }
     }
+    __device__ __forceinline__ void finish(Shared &, int64_t, int, int) {}
 };
 
-// partial sums of dQ: [splits][t][d] f32, added up over the pieces of the table
+// partial sums of dQ: [splits][m][ld] f32 (ld a multiple of 4), added up over
+// the pieces of the table
 struct PartEpi {
     float *part;
-    int64_t m, n;
+    int64_t m, ld;
     bool first;
-    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][4], int64_t m0, int64_t n0, int lane, int z) const {
+    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][8], int64_t m0, int64_t n0, int lane, int z) const {
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             const int64_t i = m0 + 16 * f + (lane & 15);
             if (i >= m) continue;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t c = n0 + 16 * g + 4 * (lane >> 4) + q;
-                    if (c >= n) continue;
-                    float *p = part + ((int64_t)z * m + i) * n + c;
-                    *p = first ? acc[f][g][q] : *p + acc[f][g][q];
-                }
+            for (int g = 0; g < 8; ++g) {
+                const int64_t c = n0 + 16 * g + 4 * (lane >> 4);
+                if (c >= ld) continue;
+                mm::f32x4 *p = reinterpret_cast<mm::f32x4 *>(part + ((int64_t)z * m + i) * ld + c);
+                *p = first ? acc[f][g] : *p + acc[f][g];
+            }
         }
     }
 };
@@ -298,28 +387,44 @@ struct GradEpi {
     void *out;
     int64_t m, n;
     const float *gs;
-    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][4], int64_t m0, int64_t n0, int lane, int) const {
+    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][8], int64_t m0, int64_t n0, int lane, int) const {
         const float s = gs[0];
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             const int64_t i = m0 + 16 * f + (lane & 15);
             if (i >= m) continue;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+            for (int g = 0; g < 8; ++g) {
+                const int64_t c = n0 + 16 * g + 4 * (lane >> 4);
+                const mm::f32x4 x = acc[f][g] * s;
+                if constexpr (F32) {
+                    float *p = (float *)out + i * n + c;
+                    if (c + 4 <= n) {
+                        __builtin_memcpy(p, &x, 16);
+                    } else {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t c = n0 + 16 * g + 4 * (lane >> 4) + q;
-                    if (c >= n) continue;
-                    if constexpr (F32) ((float *)out)[i * n + c] = acc[f][g][q] * s;
-                    else ((uint16_t *)out)[i * n + c] = mm::bf16_bits(acc[f][g][q] * s);
+                        for (int q = 0; q < 4; ++q)
+                            if (c + q < n) p[q] = x[q];
+                    }
+                } else {
+                    uint16_t *p = (uint16_t *)out + i * n + c;
+                    if (c + 4 <= n) {
+                        const uint2 y = make_uint2(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]));
+                        __builtin_memcpy(p, &y, 8);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            if (c + q < n) p[q] = mm::bf16_bits(x[q]);
+                    }
                 }
+            }
         }
     }
 };
 
 // dQ = factor (sum of the partials + resid c_target)
 template <bool F32>
-__global__ __launch_bounds__(256) void k_reduce_dq(const float *__restrict__ part, int splits, int64_t t, int d,
+__global__ __launch_bounds__(256) void k_reduce_dq(const float *__restrict__ part, int splits, int ldp, int64_t t, int d,
                                                    const uint16_t *__restrict__ C, const Row *__restrict__ row,
                                                    const int32_t *__restrict__ at,
                                                    const int64_t *__restrict__ targets,
@@ -330,7 +435,7 @@ __global__ __launch_bounds__(256) void k_reduce_dq(const float *__restrict__ par
         const int64_t i = e / d;
         float x = 0.f;
         if (targets[i] >= 0) {
-            for (int p = 0; p < splits; ++p) x += part[p * total + e];
+            for (int p = 0; p < splits; ++p) x += part[(p * t + i) * ldp + (e - i * d)];
             if (!F32 && at[i] >= 0)
                 x += row[i].resid * mm::bf16_value(C[(int64_t)at[i] * d + (e - i * d)]);
             x *= s;
@@ -348,11 +453,12 @@ inline unsigned grid1(int64_t n, int per, int64_t most = 1 << 20) {
 
 // Sizes of one call and where its workspace holds what.
 struct Plan {
-    int64_t t, v, tp;
-    int d, kp, planes;
+    int64_t t, v, tp;   // tp: t in whole tiles
+    int d, kp, ldp, planes;
     bool pack_c;
-    int64_t vc;      // items per piece (backward)
-    int splits;      // of dQ's sum over a piece
+    mm::NtArgs nt;      // the whole table's logits: how its tiles are cut
+    int64_t vc;         // items per piece (backward), in whole tiles
+    int splits;         // of dQ's sum over a piece
     size_t q, c, part, row, at, gs, D, dq, bytes;
 };
 
@@ -362,26 +468,39 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
     p.v = v;
     p.d = d;
     p.kp = (d + 31) / 32 * 32;
+    p.ldp = (d + 3) / 4 * 4;
     p.planes = f32 ? 3 : 1;
     p.pack_c = f32 || p.kp != d;
-    p.tp = (t + 127) / 128 * 128;
+    p.tp = (t + mm::TILE - 1) / mm::TILE * mm::TILE;
+    p.nt.lda = p.nt.ldb = p.kp * 2;
+    p.nt.planeA = t * p.kp * 2;
+    p.nt.planeB = v * p.kp * 2;
+    p.nt.m = t;
+    p.nt.n = v;
+    p.nt.nk = p.kp / 32;
+    p.nt.nseg = f32 ? 6 : 1;
+    p.nt.bmax = p.kp * 2 - 16;
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += up(b); return at; };
     p.q = take((size_t)p.planes * t * p.kp * 2);
     p.c = take(p.pack_c ? (size_t)p.planes * v * p.kp * 2 : 0);
     if (!backward) {
-        p.part = take((size_t)((v + 63) / 64) * t * 8);
+        mm::plan_runs(p.nt);
+        p.part = take((size_t)p.nt.slices * 2 * t * 8);
     } else {
-        const int64_t budget = (int64_t)128 << 20;
-        p.vc = std::max<int64_t>(128, budget / (p.tp * 2 * p.planes) / 128 * 128);
-        p.vc = std::min<int64_t>(p.vc, (v + 127) / 128 * 128);
-        const int64_t tiles = (t + 127) / 128 * ((d + 127) / 128);
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, p.vc / 128));
+        // pieces of equal size whose D (read twice after it is written) stays
+        // below 192 MB, most of the last-level cache
+        const int64_t all = (v + mm::TILE - 1) / mm::TILE;
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(4096, ((int64_t)192 << 20) / (p.tp * mm::TILE * 2 * p.planes)));
+        const int64_t pieces = (all + most - 1) / most;
+        p.vc = (all + pieces - 1) / pieces * mm::TILE;
+        const int64_t tiles = p.tp / mm::TILE * ((d + mm::TILE - 1) / mm::TILE);
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, p.vc / mm::TILE));
         p.row = take(sizeof(Row) * p.tp);
         p.at = take(4 * p.tp);
         p.gs = take(8);
         p.D = take((size_t)p.planes * p.tp * p.vc * 2);
-        p.dq = take((size_t)p.splits * t * d * 4);
+        p.dq = take((size_t)p.splits * t * p.ldp * 4);
     }
     p.bytes = o;
     return p;
@@ -406,17 +525,9 @@ static int operands(const Plan &p, const void *Q, const void *C, bool f32, const
 }
 
 static mm::NtArgs nt_args(const Plan &p, const void *C, char *ws) {
-    mm::NtArgs a = {};
+    mm::NtArgs a = p.nt;
     a.A = ws + p.q;
     a.B = p.pack_c ? ws + p.c : (const char *)C;
-    a.lda = a.ldb = p.kp * 2;
-    a.planeA = p.t * p.kp * 2;
-    a.planeB = p.v * p.kp * 2;
-    a.m = p.t;
-    a.n = p.v;
-    a.nk = p.kp / 32;
-    a.nseg = p.planes == 3 ? 6 : 1;
-    a.bmax = p.kp * 2 - 16;
     return a;
 }
 
@@ -431,12 +542,19 @@ static int stats_impl(const void *Q, const void *C, int32_t x_type, int64_t t, i
     hipLaunchKernelGGL(k_fill, dim3(grid1(t, 256)), dim3(256), 0, s, zt, t, -__builtin_inff());
     MN_KCHECK(s, "k_fill");
     const mm::NtArgs a = nt_args(p, C, w);
-    StatsEpi epi = {(float2 *)(w + p.part), zt, targets, c_offset, t, v, scale, scale * kLog2e};
-    const int64_t ti = (t + 127) / 128, tj = (v + 127) / 128;
-    hipLaunchKernelGGL((mm::k_nt<mm::Bf16, StatsEpi>), dim3((unsigned)(ti * tj)), dim3(256), 0, s, a, epi, tj);
+    StatsEpi epi = {};
+    epi.part = (float2 *)(w + p.part);
+    epi.zt = zt;
+    epi.targets = targets;
+    epi.c_offset = c_offset;
+    epi.t = t;
+    epi.v = (int)v;
+    epi.scale = scale;
+    epi.scale2 = scale * kLog2e;
+    hipLaunchKernelGGL((mm::k_nt<mm::Bf16, StatsEpi>), dim3((unsigned)(a.panels * a.slices)), dim3(mm::NT), 0, s, a, epi);
     MN_KCHECK(s, "k_nt");
     hipLaunchKernelGGL(k_join, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, epi.part, (const float *)nullptr,
-                       (const float *)nullptr, (v + 63) / 64, t, targets, rest, zt, loss);
+                       (const float *)nullptr, (int64_t)a.slices * 2, t, targets, rest, zt, loss);
     MN_KCHECK(s, "k_join");
     if (mean) {
         hipLaunchKernelGGL(k_mean, dim3(1), dim3(1024), 0, s, loss, targets, t, mean);
@@ -462,50 +580,56 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
                        grad_n, gs, F32, row, at);
     MN_KCHECK(s, "k_rows");
     constexpr int PL = F32 ? 3 : 1;
-    const uint16_t *Cp = (const uint16_t *)(p.pack_c ? w + p.c : (const char *)C);
+    const char *Cp = p.pack_c ? w + p.c : (const char *)C;
+    const int row_tiles = (int)(p.tp / mm::TILE), col_tiles = (d + mm::TILE - 1) / mm::TILE;
     for (int64_t j0 = 0; j0 < v; j0 += p.vc) {
         const int64_t vn = std::min(p.vc, v - j0);           // items of this piece
-        const int64_t vp = (vn + 127) / 128 * 128;           // columns of D that get written
         mm::NtArgs a = nt_args(p, C, w);
         a.B += j0 * a.ldb;
         a.n = vn;
-        DlogitsEpi<PL> epi = {(uint16_t *)(w + p.D), p.vc, p.tp * p.vc, p.tp, vn, row, at, j0, scale * kLog2e};
-        hipLaunchKernelGGL((mm::k_nt<mm::Bf16, DlogitsEpi<PL>>), dim3((unsigned)(p.tp / 128 * (vp / 128))), dim3(256), 0,
-                           s, a, epi, vp / 128);
+        mm::plan_runs(a);
+        DlogitsEpi<PL> epi = {};
+        epi.D = (uint16_t *)(w + p.D);
+        epi.ldd = p.vc;
+        epi.plane = p.tp * p.vc;
+        epi.v = (int)vn;
+        epi.row = row;
+        epi.at_ = at;
+        epi.j_first = j0;
+        epi.scale2 = scale * kLog2e;
+        hipLaunchKernelGGL((mm::k_nt<mm::Bf16, DlogitsEpi<PL>>), dim3((unsigned)(a.panels * a.slices)), dim3(mm::NT), 0, s,
+                           a, epi);
         MN_KCHECK(s, "k_nt");
         mm::KnArgs g = {};
-        g.lda = p.vc;
-        g.ldb = p.kp;
-        g.planeA = p.tp * p.vc;
-        g.n = d;
+        g.A = w + p.D;
+        g.lda = 2 * p.vc;
+        g.ldb = 2 * p.kp;
+        g.planeA = 2 * p.tp * p.vc;
         g.nseg = F32 ? 6 : 1;
-        g.A = (const uint16_t *)(w + p.D);
         if (dQ) {
-            g.B = Cp + j0 * p.kp;
-            g.planeB = v * p.kp;
-            g.m = t;
+            g.B = Cp + j0 * g.ldb;
+            g.planeB = v * g.ldb;
             g.k = vn;
-            g.kpart = ((vp + p.splits - 1) / p.splits + 31) / 32 * 32;
-            PartEpi pe = {(float *)(w + p.dq), t, d, j0 == 0};
-            hipLaunchKernelGGL((mm::k_kn<false, PartEpi>), dim3(grid1(t, 128), grid1(d, 128), p.splits), dim3(256), 0, s,
-                               g, pe);
+            g.steps_all = (int)((vn + 31) / 32);
+            g.steps = (g.steps_all + p.splits - 1) / p.splits;
+            PartEpi pe = {(float *)(w + p.dq), t, p.ldp, j0 == 0};
+            hipLaunchKernelGGL((mm::k_kn<false, PartEpi>), dim3(col_tiles, row_tiles, p.splits), dim3(mm::NT), 0, s, g, pe);
             MN_KCHECK(s, "k_kn");
         }
         if (dC) {
-            g.B = (const uint16_t *)(w + p.q);
-            g.planeB = t * p.kp;
-            g.m = vn;
+            g.B = w + p.q;
+            g.planeB = t * g.ldb;
             g.k = t;
-            g.kpart = (t + 31) / 32 * 32;
+            g.steps_all = g.steps = (int)((t + 31) / 32);
             GradEpi<F32> ge = {(char *)dC + j0 * d * (F32 ? 4 : 2), vn, d, gs};
-            hipLaunchKernelGGL((mm::k_kn<true, GradEpi<F32>>), dim3(grid1(vn, 128), grid1(d, 128), 1), dim3(256), 0, s, g,
-                               ge);
+            hipLaunchKernelGGL((mm::k_kn<true, GradEpi<F32>>), dim3(col_tiles, (unsigned)((vn + mm::TILE - 1) / mm::TILE), 1),
+                               dim3(mm::NT), 0, s, g, ge);
             MN_KCHECK(s, "k_kn");
         }
     }
     if (dQ) {
         hipLaunchKernelGGL(k_reduce_dq<F32>, dim3(grid1(t * d, 256, 65536)), dim3(256), 0, s, (const float *)(w + p.dq),
-                           p.splits, t, d, (const uint16_t *)C, row, at, targets, gs, dQ);
+                           p.splits, p.ldp, t, d, (const uint16_t *)C, row, at, targets, gs, dQ);
         MN_KCHECK(s, "k_reduce_dq");
     }
     return MN_OK;
@@ -518,7 +642,7 @@ static int check_args(const char *who, int32_t x_type, int64_t t, int64_t v, int
     MN_REQUIRE(std::isfinite(scale) && scale > 0.f, MN_EINVAL, "%s: scale has to be positive and finite", who);
     MN_REQUIRE(t <= (1 << 24) && v < INT_MAX - 1024 && d <= 65536, MN_ENOTSUP,
                "%s: t <= 2^24, v < 2^31 - 1025, d <= 65536", who);
-    MN_REQUIRE((t + 127) / 128 * ((v + 127) / 128) < INT_MAX, MN_ENOTSUP, "%s: t v too large for one call", who);
+    MN_REQUIRE((t + 255) / 256 * ((v + 255) / 256) < (1 << 30), MN_ENOTSUP, "%s: t v too large for one call", who);
     return MN_OK;
 }
 

@@ -56,7 +56,7 @@ def _rows(r: Int8Rows, name: str):
 @on_device
 def quantize_rows(X: torch.Tensor, stream=None) -> Int8Rows:
     """Rows of X [n, d] (f32 or bf16) in 8 bits: scale = max|x| / 127, code =
-    rint(x (127 / max|x|)).  A row of zeros gets scale 0; a row that holds an
+    rint(x (127 (1 / max|x|))).  A row of zeros gets scale 0; a row that holds an
     infinity or a NaN gets scale NaN, which every score with it shows."""
     if not isinstance(X, torch.Tensor) or X.dtype not in VALUE_TYPES:
         raise TypeError("X must be a float32 or bfloat16 tensor")

@@ -12,13 +12,14 @@ U32, UBF = 2.0 ** -24, 2.0 ** -8  # half a step of f32 and bf16, relative
 
 
 def quantize_ref(x):
-    """The formula in f32, as numpy rounds it; rows below 2^-100 times 2^64 first."""
+    """The formula in f32, as numpy rounds it; rows below 2^-100 (above 2^100) times 2^64 (2^-64) first."""
     x = np.asarray(x, np.float32)
     a = np.abs(x).max(1, initial=0.0).astype(np.float32)
     finite = np.isfinite(x).all(1)
     up = np.where(a < np.float32(2.0 ** -100), np.float32(2.0 ** 64), np.float32(1.0))
+    up = np.where(a > np.float32(2.0 ** 100), np.float32(2.0 ** -64), up)
     with np.errstate(all="ignore"):
-        inv = np.where(finite & (a != 0), np.float32(127.0) / (a * up), np.float32(0.0))
+        inv = np.where(finite & (a != 0), (np.float32(1.0) / (a * up)) * np.float32(127.0), np.float32(0.0))
         v = np.rint((x * up[:, None]) * inv[:, None])
         v = np.where(finite[:, None], np.clip(v, -127, 127), 0.0)
         scale = np.where(finite, a / np.float32(127.0), np.float32(np.nan))
