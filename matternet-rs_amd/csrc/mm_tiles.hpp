@@ -3,8 +3,8 @@
 //
 //   k_nt   Y[i][j] = sum_k A[i][k] B[j][k]   (rows against rows): a block keeps
 //          256 rows of A and goes through a run of 256-row tiles of B
-//   k_kn   Y[m][n] = sum_k A(m,k) B[k][n]    (A [m][k] or [k][m]): one 256 x 256
-//          tile a block, the sum over k split over blockIdx.z
+//   k_kn2  Y[m][n] = sum_k A(m,k) B[k][n]    (A [m][k] or [k][m]): one 256 x 256
+//          tile and run of k a block, two such products in a launch
 // with f32 (bf16 operands) or int32 (int8 operands) sums; an epilogue object
 // takes each wave's accumulators.
 //
@@ -274,22 +274,20 @@ struct KnArgs {
     const char *B;      // [planes][k][ldb]; columns past ldb and rows past k are never read
     int64_t lda, ldb, planeA, planeB;  // bytes; ldb a multiple of 16
     int64_t k;          // rows of B; A's entries past k are zero
-    int steps;          // k-steps of 32 of a block (blockIdx.z takes the z-th run of them)
+    int steps;          // k-steps of 32 of a run (a block takes one)
     int steps_all;
     int nseg;
 };
 
-// accumulator r of tile (f, g): row m = 16 f + (lane & 15) of the wave's 64,
-// column n = 16 g + 4 (lane >> 4) + r of its 128
+// One tile: accumulator r of (f, g) is row m = 16 f + (lane & 15) of the wave's
+// 64, column n = 16 g + 4 (lane >> 4) + r of its 128; z: which run of k-steps.
 template <bool A_T, class EPI>
-__global__ __launch_bounds__(NT, 2) void k_kn(KnArgs a, EPI epi) {
-    __shared__ Ring rg;
+__device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &epi, int64_t m0, int64_t n0, int z) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = w & 3, wj = w >> 2;
     const int fr = lane & 15, fk = lane >> 4;
-    const int64_t m0 = (int64_t)blockIdx.y * TILE, n0 = (int64_t)blockIdx.x * TILE;
-    const int s0 = (int)blockIdx.z * a.steps, s1 = min(a.steps_all, s0 + a.steps);
+    const int s0 = z * a.steps, s1 = min(a.steps_all, s0 + a.steps);
     const int per = s1 - s0, nstep = max(0, per) * a.nseg;
 
     // ---- loads.  [k][256]: wave w stages rows 4 w .. 4 w + 3 in two pieces of
@@ -387,13 +385,57 @@ __global__ __launch_bounds__(NT, 2) void k_kn(KnArgs a, EPI epi) {
         if (!wj) window_end();
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    epi(acc, m0 + 64 * wi, n0 + 128 * wj, lane, (int)blockIdx.z);
+    epi(acc, m0 + 64 * wi, n0 + 128 * wj, lane, z);
+}
+
+// What a launch of k_kn2 has of one product: blocks = splits x rows x cols of
+// tiles, columns fastest (they share A), then rows (they share B).
+struct KnGrid {
+    int cols, rows, splits;
+    __host__ __device__ int blocks() const { return cols * rows * splits; }
+};
+
+// Two products in one launch, so that the tiles of the second fill the
+// processors that the last round of the first leaves idle: A [m][k] first, then
+// A [k][m].
+template <class E1, class E2>
+__global__ __launch_bounds__(NT, 2) void k_kn2(KnArgs a1, E1 e1, KnGrid g1, KnArgs a2, E2 e2, KnGrid g2) {
+    __shared__ Ring rg;
+    const int b = (int)blockIdx.x, n1 = g1.blocks();
+    if (b < n1) {
+        const int v = xcd_range(b, n1), r = v / g1.cols;
+        kn_tile<false>(rg, a1, e1, (int64_t)(r % g1.rows) * TILE, (int64_t)(v % g1.cols) * TILE, r / g1.rows);
+    } else {
+        const int v = xcd_range(b - n1, g2.blocks()), r = v / g2.cols;
+        kn_tile<true>(rg, a2, e2, (int64_t)(r % g2.rows) * TILE, (int64_t)(v % g2.cols) * TILE, r / g2.rows);
+    }
 }
 
 __device__ __forceinline__ uint16_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
 __device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 __device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
     return (uint32_t)bf16_bits(x) | ((uint32_t)bf16_bits(y) << 16);
+}
+
+// the first n (<= 4) of x to element e of an f32 or bf16 array, any alignment
+template <bool F32>
+__device__ __forceinline__ void store4(void *out, int64_t e, int n, f32x4 x) {
+    if constexpr (F32) {
+        float *p = (float *)out + e;
+        if (n == 4) {
+            __builtin_memcpy(p, &x, 16);
+        } else {
+            for (int q = 0; q < n; ++q) p[q] = q == 0 ? x[0] : q == 1 ? x[1] : x[2];
+        }
+    } else {
+        uint16_t *p = (uint16_t *)out + e;
+        const uint2 y = make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]));
+        if (n == 4) {
+            __builtin_memcpy(p, &y, 8);
+        } else {
+            for (int q = 0; q < n; ++q) p[q] = (uint16_t)((q < 2 ? y.x : y.y) >> (16 * (q & 1)));
+        }
+    }
 }
 
 // x = h + m + l.  A finite x whose nearest bf16 is infinite takes the one

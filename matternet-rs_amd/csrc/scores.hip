@@ -8,6 +8,7 @@
 // sum rounded to f32, times the query's scale, times the item's.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "common.hpp"
 #include "mm_tiles.hpp"
@@ -15,52 +16,130 @@
 namespace mn {
 namespace i8 {
 
-// A row's largest |x| as bits: NaN > inf > every finite value, so one integer
-// maximum also tells whether the row holds something that is not finite.
+// 8 values of a row from column k (a multiple of 8), zeros past column d.
+// vec: rows start on 16-byte borders.
 template <typename T>
-__device__ __forceinline__ float load_x(const T *X, int64_t e);
-template <>
-__device__ __forceinline__ float load_x<float>(const float *X, int64_t e) { return X[e]; }
-template <>
-__device__ __forceinline__ float load_x<uint16_t>(const uint16_t *X, int64_t e) { return mm::bf16_value(X[e]); }
-
-// Below 2^-100 the reciprocal 1 / a could overflow, above 2^100 be subnormal:
-// such a row is multiplied by 2^64 or 2^-64 first (exact where it matters).  A row of zeros has scale 0 and codes 0; a row that
-// holds an infinity or a NaN has scale NaN, which every score with it shows.
-template <typename T>
-__global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64_t n, int d,
-                                                  int8_t *__restrict__ codes, int64_t ld,
-                                                  float *__restrict__ scale) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
-        uint32_t top = 0;
-        for (int k = lane; k < d; k += 64) top = max(top, __float_as_uint(load_x(X, i * d + k)) & 0x7fffffffu);
+__device__ __forceinline__ void load8(const T *row, int k, int d, bool vec, float (&v)[8]) {
+    if (vec && k + 8 <= d) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = reinterpret_cast<const float4 *>(row + k)[0], b = reinterpret_cast<const float4 *>(row + k)[1];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 a = *reinterpret_cast<const uint4 *>(row + k);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-        float a = __uint_as_float(top);
-        const bool finite = top < 0x7f800000u;
-        const float up = a < 0x1p-100f ? 0x1p64f : a > 0x1p100f ? 0x1p-64f : 1.f;
-        const float inv = finite && top != 0 ? 1.f / (a * up) * 127.f : 0.f;
-        for (int k = lane; k < ld; k += 64) {
-            float v = 0.f;
-            if (k < d && finite) v = __builtin_rintf(load_x(X, i * d + k) * up * inv);
-            codes[i * ld + k] = (int8_t)(int)fminf(fmaxf(v, -127.f), 127.f);
+            for (int e = 0; e < 8; ++e) v[e] = mm::bf16_value((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
         }
-        if (lane == 0) scale[i] = finite ? a / 127.f : __builtin_nanf("");
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool in = k + e < d;
+            if constexpr (sizeof(T) == 4) v[e] = in ? row[k + e] : 0.f;
+            else v[e] = in ? mm::bf16_value(row[k + e]) : 0.f;
+        }
     }
 }
 
+// L lanes take a row, 8 values a lane at a time; up to 16 values a lane stay in
+// registers between the two passes (longer rows are read again, from L2).  A
+// row's largest |x| is folded as bits: NaN > inf > every finite value, so one
+// integer maximum also tells whether the row holds something that is not
+// finite.
+// Below 2^-100 the reciprocal 1 / a could overflow, above 2^100 be subnormal:
+// such a row is multiplied by 2^64 or 2^-64 first (exact where it matters).  A
+// row of zeros has scale 0 and codes 0; a row that holds an infinity or a NaN
+// has scale NaN, which every score with it shows.
+template <typename T, int L>
+__global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64_t n, int d, bool vec,
+                                                  int8_t *__restrict__ codes, int64_t ld,
+                                                  float *__restrict__ scale) {
+    const int l = threadIdx.x % L;
+    const int64_t i = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (i >= n) return;  // whole groups of L lanes
+    const T *row = X + i * d;
+    float v[2][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int k = 8 * (L * u + l);
+        if (u == 0 || k < d) load8(row, k, d, vec, v[u]);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[u][e]) & 0x7fffffffu);
+    }
+    for (int k = 8 * (2 * L + l); k < d; k += 8 * L) {
+        float x[8];
+        load8(row, k, d, vec, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    const float a = __uint_as_float(top);
+    const bool finite = top < 0x7f800000u;
+    const float up = a < 0x1p-100f ? 0x1p64f : a > 0x1p100f ? 0x1p-64f : 1.f;
+    const float inv = finite && top != 0 ? 1.f / (a * up) * 127.f : 0.f;
+    int8_t *out = codes + i * ld;
+    for (int u = 0; 8 * (L * u + l) < ld; ++u) {
+        const int k = 8 * (L * u + l);
+        float x[8];
+        if (u < 2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = u == 0 ? v[0][e] : v[1][e];
+        } else {
+            load8(row, k, d, vec, x);
+        }
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float c = finite ? __builtin_rintf(x[e] * up * inv) : 0.f;
+            w[e >> 2] |= ((uint32_t)(int)fminf(fmaxf(c, -127.f), 127.f) & 255u) << (8 * (e & 3));
+        }
+        *reinterpret_cast<uint2 *>(out + k) = make_uint2(w[0], w[1]);
+    }
+    if (l == 0) scale[i] = finite ? a / 127.f : __builtin_nanf("");
+}
+
+// 8 codes a thread at a time; a block takes 2048 pieces of 8 in a row
 template <typename T>
 __global__ __launch_bounds__(256) void k_dequantize(const int8_t *__restrict__ codes, int64_t ld,
-                                                    const float *__restrict__ scale, int64_t n, int d,
+                                                    const float *__restrict__ scale, int64_t n, int d, bool vec,
                                                     T *__restrict__ X) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
+    const uint32_t n8 = (uint32_t)(d + 7) / 8;
+    const int64_t base = (int64_t)blockIdx.x * 2048, total = n * n8;
+    const int64_t row0 = base / n8;
+    const uint32_t rem = (uint32_t)(base - row0 * n8);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const uint32_t l = 256 * u + threadIdx.x;
+        if (base + l >= total) return;
+        const uint32_t x = rem + l, q = x / n8;
+        const int k = 8 * (int)(x - q * n8);
+        const int64_t i = row0 + q;
         const float s = scale[i];
-        for (int k = lane; k < d; k += 64) {
-            const float v = (float)codes[i * ld + k] * s;
-            if constexpr (sizeof(T) == 4) X[i * d + k] = v;
-            else X[i * d + k] = mm::bf16_bits(v);
+        const uint2 c = *reinterpret_cast<const uint2 *>(codes + i * ld + k);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3))) * s;
+        T *out = X + i * d + k;
+        if (vec && k + 8 <= d) {
+            if constexpr (sizeof(T) == 4) {
+                reinterpret_cast<float4 *>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<float4 *>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                *reinterpret_cast<uint4 *>(out) = make_uint4(mm::bf16_pair(v[0], v[1]), mm::bf16_pair(v[2], v[3]),
+                                                             mm::bf16_pair(v[4], v[5]), mm::bf16_pair(v[6], v[7]));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < d) {
+                    if constexpr (sizeof(T) == 4) out[e] = v[e];
+                    else out[e] = mm::bf16_bits(v[e]);
+                }
         }
     }
 }
@@ -139,6 +218,24 @@ struct ScoreEpi {
 };
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// lanes a row: the power of two that takes ld in one turn, 2 to 64
+template <typename T>
+void quantize(const T *X, int64_t n, int d, int8_t *codes, int64_t ld, float *scale, hipStream_t s) {
+    const bool vec = (d * sizeof(T)) % 16 == 0 && aligned16(X);
+    auto go = [&](auto L) {
+        constexpr int l = decltype(L)::value, per = 256 / l;
+        hipLaunchKernelGGL((k_quantize<T, l>), dim3((unsigned)((n + per - 1) / per)), dim3(256), 0, s, X, n, d, vec, codes,
+                           ld, scale);
+    };
+    if (ld <= 16) go(std::integral_constant<int, 2>());
+    else if (ld <= 32) go(std::integral_constant<int, 4>());
+    else if (ld <= 64) go(std::integral_constant<int, 8>());
+    else if (ld <= 128) go(std::integral_constant<int, 16>());
+    else if (ld <= 256) go(std::integral_constant<int, 32>());
+    else go(std::integral_constant<int, 64>());
+}
+
 inline int padded(int d) { return (d + mm::KBY - 1) / mm::KBY * mm::KBY; }
 
 }  // namespace i8
@@ -150,16 +247,15 @@ extern "C" int mn_quantize_rows_i8(const void *X, int32_t x_type, int64_t n, int
     mn::clear_error();
     MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX, MN_EINVAL,
                "mn_quantize_rows_i8: n >= 0, d >= 1, ld >= d and a multiple of 16 needed");
+    MN_REQUIRE(n < INT_MAX && n * ((d + 7) / 8) / 2048 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
+               "mn_quantize_rows_i8: n < 2^31 - 1 rows and n d < 2^44 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_quantize_rows_i8: MN_F32 or MN_BF16");
     if (n == 0) return MN_OK;
     MN_REQUIRE(X && codes && scale, MN_EINVAL, "mn_quantize_rows_i8: NULL pointer");
     MN_REQUIRE(aligned16(codes), MN_EINVAL, "mn_quantize_rows_i8: codes not 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const unsigned grid = (unsigned)std::min<int64_t>((n + 3) / 4, 1 << 20);
-    if (x_type == MN_F32)
-        hipLaunchKernelGGL(k_quantize<float>, dim3(grid), dim3(256), 0, s, (const float *)X, n, d, codes, ld, scale);
-    else
-        hipLaunchKernelGGL(k_quantize<uint16_t>, dim3(grid), dim3(256), 0, s, (const uint16_t *)X, n, d, codes, ld, scale);
+    if (x_type == MN_F32) quantize((const float *)X, n, d, codes, ld, scale, s);
+    else quantize((const uint16_t *)X, n, d, codes, ld, scale, s);
     MN_KCHECK(s, "k_quantize");
     return MN_OK;
 }
@@ -170,16 +266,20 @@ extern "C" int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const floa
     mn::clear_error();
     MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX, MN_EINVAL,
                "mn_dequantize_rows_i8: n >= 0, d >= 1, ld >= d and a multiple of 16 needed");
+    MN_REQUIRE(n < INT_MAX && n * ((d + 7) / 8) / 2048 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
+               "mn_dequantize_rows_i8: n < 2^31 - 1 rows and n d < 2^44 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_dequantize_rows_i8: MN_F32 or MN_BF16");
     if (n == 0) return MN_OK;
     MN_REQUIRE(X && codes && scale, MN_EINVAL, "mn_dequantize_rows_i8: NULL pointer");
     MN_REQUIRE(aligned16(codes), MN_EINVAL, "mn_dequantize_rows_i8: codes not 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const unsigned grid = (unsigned)std::min<int64_t>((n + 3) / 4, 1 << 20);
+    const dim3 grid((unsigned)((n * ((d + 7) / 8) + 2047) / 2048));
     if (x_type == MN_F32)
-        hipLaunchKernelGGL(k_dequantize<float>, dim3(grid), dim3(256), 0, s, codes, ld, scale, n, d, (float *)X);
+        hipLaunchKernelGGL(k_dequantize<float>, grid, dim3(256), 0, s, codes, ld, scale, n, d,
+                           d % 4 == 0 && aligned16(X), (float *)X);
     else
-        hipLaunchKernelGGL(k_dequantize<uint16_t>, dim3(grid), dim3(256), 0, s, codes, ld, scale, n, d, (uint16_t *)X);
+        hipLaunchKernelGGL(k_dequantize<uint16_t>, grid, dim3(256), 0, s, codes, ld, scale, n, d,
+                           d % 8 == 0 && aligned16(X), (uint16_t *)X);
     MN_KCHECK(s, "k_dequantize");
     return MN_OK;
 }

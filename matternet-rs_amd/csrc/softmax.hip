@@ -31,26 +31,152 @@ struct Row {
     float rel, lse2, dt, resid;
 };
 
-// [rows][d] to `P` planes of [rows][kp] bf16, zero past d; rows whose target
-// is < 0 become zeros, so that what they hold (a NaN, say) reaches no sum.
+// A matrix [rows][d] on its way into planes [rows][kp] of bf16, zero past d.
+// Rows whose target is < 0 become zeros, so that what they hold (a NaN, say)
+// reaches no sum.  A thread takes 8 values at a time.
+struct Pack {
+    const void *X;
+    uint16_t *out;
+    const int64_t *targets;  // or NULL
+    int64_t rows;
+    int d, kp, blocks;
+    bool vec;                // rows start on 16-byte borders
+};
+constexpr int kPackPer = 8;  // pieces of 8 values a thread
+
 template <bool F32>
-__global__ __launch_bounds__(256) void k_pack(const void *__restrict__ X, int64_t rows, int d, int kp,
-                                              const int64_t *__restrict__ targets,
-                                              uint16_t *__restrict__ out) {
-    const int64_t total = rows * kp, stride = (int64_t)gridDim.x * 256;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += stride) {
-        const int64_t i = e / kp;
-        const int k = (int)(e - i * kp);
-        const bool has = k < d && (!targets || targets[i] >= 0);
-        if constexpr (F32) {
-            uint16_t p[3];
-            mm::split3(has ? ((const float *)X)[i * d + k] : 0.f, p);
+__device__ __forceinline__ void pack(const Pack &p, int block) {
+    const int n8 = p.kp / 8;
+    const int64_t base = (int64_t)block * (256 * kPackPer), total = p.rows * n8;
+    const int64_t row0 = base / n8;
+    const uint32_t rem = (uint32_t)(base - row0 * n8);
 #pragma unroll
-            for (int q = 0; q < 3; ++q) out[q * total + e] = p[q];
+    for (int u = 0; u < kPackPer; ++u) {
+        const uint32_t l = 256 * u + threadIdx.x;
+        if (base + l >= total) return;
+        const uint32_t x = rem + l, q = x / (uint32_t)n8, k = 8 * (x - q * n8);
+        const int64_t i = row0 + q;
+        const bool has = !p.targets || p.targets[i] >= 0;
+        uint16_t *o = p.out + 8 * (base + l);
+        if constexpr (F32) {
+            const float *src = (const float *)p.X + i * p.d + k;
+            float v[8];
+            if (p.vec && k + 8 <= (uint32_t)p.d) {
+                const float4 v0 = reinterpret_cast<const float4 *>(src)[0], v1 = reinterpret_cast<const float4 *>(src)[1];
+                v[0] = v0.x, v[1] = v0.y, v[2] = v0.z, v[3] = v0.w;
+                v[4] = v1.x, v[5] = v1.y, v[6] = v1.z, v[7] = v1.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = k + e < (uint32_t)p.d ? src[e] : 0.f;
+            }
+            uint32_t w[3][4];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                uint16_t a[3], b[3];
+                mm::split3(has ? v[e] : 0.f, a);
+                mm::split3(has ? v[e + 1] : 0.f, b);
+#pragma unroll
+                for (int s = 0; s < 3; ++s) w[s][e / 2] = (uint32_t)a[s] | ((uint32_t)b[s] << 16);
+            }
+#pragma unroll
+            for (int s = 0; s < 3; ++s)
+                *reinterpret_cast<uint4 *>(o + s * (8 * total)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
         } else {
-            out[e] = has ? ((const uint16_t *)X)[i * d + k] : (uint16_t)0;
+            const uint16_t *src = (const uint16_t *)p.X + i * p.d + k;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (has) {
+                if (p.vec && k + 8 <= (uint32_t)p.d) {
+                    v = *reinterpret_cast<const uint4 *>(src);
+                } else {
+                    uint32_t e[8];
+#pragma unroll
+                    for (int q8 = 0; q8 < 8; ++q8) e[q8] = k + q8 < (uint32_t)p.d ? src[q8] : 0u;
+                    v = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
+                }
+            }
+            *reinterpret_cast<uint4 *>(o) = v;
         }
     }
+}
+
+__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
+
+// What the rows need before the products: forward the targets' logits (a wave
+// a row: f32 sums of the d products) and the count of blocks of k_join that are
+// done; backward Row and the target within the rows of C here.
+struct Rows {
+    int64_t t, tp, v, c_offset;
+    const int64_t *targets;
+    const void *Q, *C;
+    int d;
+    float *zt_out;         // forward
+    int32_t *done;
+    const float *rest, *zt;  // backward (rest not NULL)
+    const float *grad, *grad_scale;
+    int64_t grad_n;
+    float scale;
+    float *gs;             // [0] the factor of every gradient, [1] max |g| (grad_n > 1: of k_grad_max)
+    Row *row;
+    int32_t *at;
+};
+
+template <bool F32>
+__device__ __forceinline__ void rows(const Rows &p, int block) {
+    if (!p.rest) {
+        const int lane = threadIdx.x & 63;
+        const int64_t i = (int64_t)block * 4 + (threadIdx.x >> 6);
+        if (block == 0 && threadIdx.x == 0) *p.done = 0;
+        if (i >= p.t) return;
+        const int64_t at = p.targets[i] - p.c_offset;
+        if (p.targets[i] < 0 || at < 0 || at >= p.v) {
+            if (lane == 0) p.zt_out[i] = -__builtin_inff();
+            return;
+        }
+        float z = 0.f;
+        for (int k = lane; k < p.d; k += 64) {
+            if constexpr (F32)
+                z = __builtin_fmaf(((const float *)p.Q)[i * p.d + k], ((const float *)p.C)[at * p.d + k], z);
+            else
+                z = __builtin_fmaf(mm::bf16_value(((const uint16_t *)p.Q)[i * p.d + k]),
+                                   mm::bf16_value(((const uint16_t *)p.C)[at * p.d + k]), z);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o);
+        if (lane == 0) p.zt_out[i] = z * p.scale;
+        return;
+    }
+    const int64_t i = (int64_t)block * 256 + threadIdx.x;
+    if (i >= p.tp) return;
+    const float top = p.grad_n == 1 ? fabsf(p.grad[0]) : p.gs[1];
+    if (i == 0) p.gs[0] = (p.grad_scale ? top * p.grad_scale[0] : top) * p.scale;
+    Row r = {0.f, 0.f, 0.f, 0.f};
+    int32_t a = -1;
+    if (i < p.t && p.targets[i] >= 0) {
+        const int64_t tl = p.targets[i] - p.c_offset;
+        const float g = p.grad_n == 1 ? p.grad[0] : p.grad[i];
+        const float inf = __builtin_inff();
+        const float re = p.rest[i], z = p.zt[i];
+        r.rel = top == 0.f ? 0.f : g / top;
+        const float lse = re == -inf ? z : z == -inf ? re : z + softplus(re - z);
+        r.lse2 = lse * kLog2e;
+        r.dt = re == -inf ? 0.f : -r.rel / (1.f + expf(z - re));
+        if (tl >= 0 && tl < p.v) {
+            a = (int32_t)tl;
+            if (!F32) r.resid = r.dt - mm::bf16_value(mm::bf16_bits(r.dt));
+        }
+    }
+    p.row[i] = r;
+    p.at[i] = a;
+}
+
+// One launch for all that comes before the products.
+template <bool F32>
+__global__ __launch_bounds__(256) void k_prep(Pack q, Pack c, Rows r) {
+    int b = (int)blockIdx.x;
+    if (b < q.blocks) return pack<F32>(q, b);
+    b -= q.blocks;
+    if (b < c.blocks) return pack<F32>(c, b);
+    rows<F32>(r, b - c.blocks);
 }
 
 // Per lane and row the largest logit so far (m2, base 2, rounded: the number
@@ -62,11 +188,10 @@ struct StatsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;
     float2 *part;
-    float *zt;
     const int64_t *targets;
     int64_t c_offset, t;
     int v;
-    float scale, scale2;  // scale2 = scale log2(e)
+    float scale2;  // scale log2(e)
     int at[4];
     float m2[4], sum[4];
     int64_t row0;
@@ -88,20 +213,14 @@ struct StatsEpi {
         for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 128u;
         if (__ballot(hit)) {
 #pragma unroll
-            for (int f = 0; f < 4; ++f) {
-                float z = 0.f;
-                bool mine = false;
+            for (int g = 0; g < 8; ++g)
 #pragma unroll
-                for (int g = 0; g < 8; ++g)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
+                    for (int f = 0; f < 4; ++f) {
                         const int j = jl + 32 * (g >> 1) + 4 * (g & 1) + r;
-                        z = j == at[f] ? acc[f][g][r] : z;
-                        mine = mine || j == at[f];
                         acc[f][g][r] = j >= v || j == at[f] ? -__builtin_inff() : acc[f][g][r];
                     }
-                if (mine) zt[row0 + 16 * f] = z * scale;
-            }
         }
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
@@ -140,25 +259,58 @@ struct StatsEpi {
     }
 };
 
-__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
-
 // loss of a row from (rest, zt); -inf for zt: no target in any range (loss +inf)
 __device__ __forceinline__ float row_loss(float rest, float zt) {
     if (rest == -__builtin_inff()) return zt == rest ? __builtin_inff() : 0.f;
     return zt == -__builtin_inff() ? __builtin_inff() : softplus(rest - zt);
 }
 
-// one wave a row: joins n (maximum, sum) pairs (base 2), or with `rests` n
-// values of rest and zt (the ranges of a table)
+template <class F>
+__device__ __forceinline__ float block_fold(float x, float *sh, F f) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = f(x, __shfl_xor(x, o));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = sh[0];
+    for (int w = 1; w < (int)blockDim.x / 64; ++w) x = f(x, sh[w]);
+    __syncthreads();
+    return x;
+}
+
+// out = (mean of the losses of the rows that take part, 1 / their number); no
+// such row: (0, 1).  One block and a fixed order.
+__device__ __forceinline__ void mean_of(const float *loss, const int64_t *targets, int64_t t, float *out) {
+    __shared__ float sh[16];
+    float sum = 0.f, num = 0.f;
+    for (int64_t i = threadIdx.x; i < t; i += blockDim.x) {
+        const bool has = targets[i] >= 0;
+        sum += has ? loss[i] : 0.f;
+        num += has ? 1.f : 0.f;
+    }
+    auto add = [](float a, float b) { return a + b; };
+    sum = block_fold(sum, sh, add);
+    num = fmaxf(block_fold(num, sh, add), 1.f);
+    if (threadIdx.x == 0) {
+        out[0] = sum / num;
+        out[1] = 1.f / num;
+    }
+}
+__global__ __launch_bounds__(1024) void k_mean(const float *loss, const int64_t *targets, int64_t t, float *out) {
+    mean_of(loss, targets, t, out);
+}
+
+// One wave a row: joins n (maximum, sum) pairs (base 2), or with `rests` n
+// values of rest and zt (the ranges of a table).  With `done` the block that
+// ends last takes the mean (it sees the others' losses: each counts itself
+// after a fence, it reads them after one).
 __global__ __launch_bounds__(256) void k_join(const float2 *__restrict__ part, const float *__restrict__ rests,
                                               const float *__restrict__ zts, int64_t n, int64_t t,
-                                              const int64_t *__restrict__ targets, float *__restrict__ rest,
-                                              float *__restrict__ zt, float *__restrict__ loss) {
+                                              const int64_t *__restrict__ targets, float *rest, float *zt,
+                                              float *loss, float *mean, int32_t *done) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= t) return;
     float top = -__builtin_inff(), sum = 0.f, z = -__builtin_inff();
-    for (int64_t k = lane; k < n; k += 64) {
+    for (int64_t k = lane; k < n && i < t; k += 64) {
         float2 p;
         if (part) {
             p = part[k * t + i];
@@ -185,97 +337,33 @@ __global__ __launch_bounds__(256) void k_join(const float2 *__restrict__ part, c
         top = m;
         z = fmaxf(z, __shfl_xor(z, o));
     }
-    if (lane == 0) {
+    if (lane == 0 && i < t) {
         const float r = sum == 0.f ? -__builtin_inff() : (top == -__builtin_inff() ? sum : (top + log2f(sum)) * kLn2);
         if (!zts) z = zt[i];
         else zt[i] = z;
         rest[i] = r;
         if (loss) loss[i] = targets[i] < 0 ? 0.f : row_loss(r, z);
     }
-}
-
-__global__ __launch_bounds__(256) void k_fill(float *__restrict__ p, int64_t n, float v) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = v;
-}
-
-template <class F>
-__device__ __forceinline__ float block_fold(float x, float *sh, F f) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = f(x, __shfl_xor(x, o));
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
+    if (!done) return;
+    __shared__ int last;
+    __threadfence();
     __syncthreads();
-    x = sh[0];
-    for (int w = 1; w < (int)blockDim.x / 64; ++w) x = f(x, sh[w]);
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
     __syncthreads();
-    return x;
+    if (!last) return;
+    __threadfence();
+    mean_of(loss, targets, t, mean);
 }
 
-// out = (mean of the losses of the rows that take part, 1 / their number);
-// no such row: (0, 1).  One block: the order of the sum is fixed.
-__global__ __launch_bounds__(1024) void k_mean(const float *__restrict__ loss, const int64_t *__restrict__ targets,
-                                               int64_t t, float *__restrict__ out) {
-    __shared__ float sh[16];
-    float sum = 0.f, num = 0.f;
-    for (int64_t i = threadIdx.x; i < t; i += 1024) {
-        const bool has = targets[i] >= 0;
-        sum += has ? loss[i] : 0.f;
-        num += has ? 1.f : 0.f;
-    }
-    auto add = [](float a, float b) { return a + b; };
-    sum = block_fold(sum, sh, add);
-    num = fmaxf(block_fold(num, sh, add), 1.f);
-    if (threadIdx.x == 0) {
-        out[0] = sum / num;
-        out[1] = 1.f / num;
-    }
-}
-
-// gs[0] = the factor of every gradient (scale, max |g|, *grad_scale), gs[1] = max |g|
-__global__ __launch_bounds__(1024) void k_grad_scale(const float *__restrict__ grad, int64_t grad_n,
-                                                     const float *__restrict__ grad_scale,
-                                                     const int64_t *__restrict__ targets, float scale,
-                                                     float *__restrict__ gs) {
+// gs[1] = the largest |g| of the rows that take part
+__global__ __launch_bounds__(1024) void k_grad_max(const float *__restrict__ grad, int64_t t,
+                                                   const int64_t *__restrict__ targets, float *__restrict__ gs) {
     __shared__ float sh[16];
     float top = 0.f;
-    if (grad_n == 1) {
-        top = fabsf(grad[0]);
-    } else {
-        for (int64_t i = threadIdx.x; i < grad_n; i += 1024)
-            top = fmaxf(top, targets[i] >= 0 ? fabsf(grad[i]) : 0.f);
-        top = block_fold(top, sh, [](float a, float b) { return fmaxf(a, b); });
-    }
-    if (threadIdx.x == 0) {
-        gs[0] = (grad_scale ? top * grad_scale[0] : top) * scale;
-        gs[1] = top;
-    }
-}
-
-__global__ __launch_bounds__(256) void k_rows(const float *__restrict__ rest, const float *__restrict__ zt,
-                                              const int64_t *__restrict__ targets, int64_t c_offset, int64_t t,
-                                              int64_t tp, int64_t v, const float *__restrict__ grad, int64_t grad_n,
-                                              const float *__restrict__ gs, bool f32, Row *__restrict__ row,
-                                              int32_t *__restrict__ at) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= tp) return;
-    Row r = {0.f, 0.f, 0.f, 0.f};
-    int32_t a = -1;
-    if (i < t && targets[i] >= 0) {
-        const int64_t tl = targets[i] - c_offset;
-        const float top = gs[1], g = grad_n == 1 ? grad[0] : grad[i];
-        const float inf = __builtin_inff();
-        const float re = rest[i], z = zt[i];
-        r.rel = top == 0.f ? 0.f : g / top;
-        const float lse = re == -inf ? z : z == -inf ? re : z + softplus(re - z);
-        r.lse2 = lse * kLog2e;
-        r.dt = re == -inf ? 0.f : -r.rel / (1.f + expf(z - re));
-        if (tl >= 0 && tl < v) {
-            a = (int32_t)tl;
-            if (!f32) r.resid = r.dt - mm::bf16_value(mm::bf16_bits(r.dt));
-        }
-    }
-    row[i] = r;
-    at[i] = a;
+    for (int64_t i = threadIdx.x; i < t; i += 1024) top = fmaxf(top, targets[i] >= 0 ? fabsf(grad[i]) : 0.f);
+    top = block_fold(top, sh, [](float a, float b) { return fmaxf(a, b); });
+    if (threadIdx.x == 0) gs[1] = top;
 }
 
 // D of a piece of the table, [tp][ldd] (three planes for f32 operands); zeros
@@ -396,53 +484,39 @@ struct GradEpi {
 #pragma unroll
             for (int g = 0; g < 8; ++g) {
                 const int64_t c = n0 + 16 * g + 4 * (lane >> 4);
-                const mm::f32x4 x = acc[f][g] * s;
-                if constexpr (F32) {
-                    float *p = (float *)out + i * n + c;
-                    if (c + 4 <= n) {
-                        __builtin_memcpy(p, &x, 16);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            if (c + q < n) p[q] = x[q];
-                    }
-                } else {
-                    uint16_t *p = (uint16_t *)out + i * n + c;
-                    if (c + 4 <= n) {
-                        const uint2 y = make_uint2(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]));
-                        __builtin_memcpy(p, &y, 8);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            if (c + q < n) p[q] = mm::bf16_bits(x[q]);
-                    }
-                }
+                if (c < n) mm::store4<F32>(out, i * n + c, (int)min<int64_t>(4, n - c), acc[f][g] * s);
             }
         }
     }
 };
 
-// dQ = factor (sum of the partials + resid c_target)
+// dQ = factor (sum of the partials + resid c_target); a thread takes 4 columns
 template <bool F32>
 __global__ __launch_bounds__(256) void k_reduce_dq(const float *__restrict__ part, int splits, int ldp, int64_t t, int d,
                                                    const uint16_t *__restrict__ C, const Row *__restrict__ row,
                                                    const int32_t *__restrict__ at,
                                                    const int64_t *__restrict__ targets,
                                                    const float *__restrict__ gs, void *__restrict__ dQ) {
-    const int64_t total = t * d, stride = (int64_t)gridDim.x * 256;
-    const float s = gs[0];
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += stride) {
-        const int64_t i = e / d;
-        float x = 0.f;
-        if (targets[i] >= 0) {
-            for (int p = 0; p < splits; ++p) x += part[(p * t + i) * ldp + (e - i * d)];
-            if (!F32 && at[i] >= 0)
-                x += row[i].resid * mm::bf16_value(C[(int64_t)at[i] * d + (e - i * d)]);
-            x *= s;
+    const uint32_t n4 = ldp / 4;
+    const int64_t total = t * n4, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= total) return;
+    const int64_t i = total <= 0xffffffffll ? (int64_t)((uint32_t)e / n4) : e / n4;
+    const int c = 4 * (int)(e - i * n4);
+    mm::f32x4 x = (mm::f32x4)(0.f);
+    if (targets[i] >= 0) {
+        const mm::f32x4 *p = reinterpret_cast<const mm::f32x4 *>(part) + e;
+#pragma unroll 8
+        for (int s = 0; s < splits; ++s) x += p[s * total];
+        if (!F32 && at[i] >= 0) {
+            const float r = row[i].resid;
+            const uint16_t *src = C + (int64_t)at[i] * d + c;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < d) x[q] += r * mm::bf16_value(src[q]);
         }
-        if constexpr (F32) ((float *)dQ)[e] = x;
-        else ((uint16_t *)dQ)[e] = mm::bf16_bits(x);
+        x *= gs[0];
     }
+    mm::store4<F32>(dQ, i * d + c, min(4, d - c), x);
 }
 
 inline size_t up(size_t x) { return (x + 255) / 256 * 256; }
@@ -456,10 +530,10 @@ struct Plan {
     int64_t t, v, tp;   // tp: t in whole tiles
     int d, kp, ldp, planes;
     bool pack_c;
-    mm::NtArgs nt;      // the whole table's logits: how its tiles are cut
-    int64_t vc;         // items per piece (backward), in whole tiles
+    mm::NtArgs nt;      // the whole table's logits
+    int64_t vc, vmax;   // items per piece (backward), of the longest piece, in whole tiles
     int splits;         // of dQ's sum over a piece
-    size_t q, c, part, row, at, gs, D, dq, bytes;
+    size_t q, c, part, done, row, at, gs, D, dq, bytes;
 };
 
 inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
@@ -487,19 +561,29 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
     if (!backward) {
         mm::plan_runs(p.nt);
         p.part = take((size_t)p.nt.slices * 2 * t * 8);
+        p.done = take(4);
     } else {
-        // pieces of equal size whose D (read twice after it is written) stays
-        // below 192 MB, most of the last-level cache
-        const int64_t all = (v + mm::TILE - 1) / mm::TILE;
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(4096, ((int64_t)192 << 20) / (p.tp * mm::TILE * 2 * p.planes)));
-        const int64_t pieces = (all + most - 1) / most;
-        p.vc = (all + pieces - 1) / pieces * mm::TILE;
-        const int64_t tiles = p.tp / mm::TILE * ((d + mm::TILE - 1) / mm::TILE);
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, p.vc / mm::TILE));
+        // Pieces whose D stays below 256 MB and whose tiles fill whole rounds
+        // of 256 blocks; a short rest joins the last piece where it fits.
+        const int64_t all = (v + mm::TILE - 1) / mm::TILE, panels = p.tp / mm::TILE;
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(4096, ((int64_t)256 << 20) / (p.tp * mm::TILE * 2 * p.planes)));
+        const int64_t unit = std::max<int64_t>(1, 256 / panels);
+        const int64_t piece = most >= unit ? most / unit * unit : most;
+        const int64_t rest = all % piece;
+        int64_t longest = std::min(piece, all);
+        if (all > piece && rest > 0 && piece + rest <= most) longest = piece + rest;
+        p.vc = std::min(piece, all) * mm::TILE;
+        p.vmax = longest * mm::TILE;
+        // dQ's runs about as long as dC's sums (t), so that the last round of
+        // blocks ends together; more than a round of blocks only where the
+        // partial sums stay small next to the products
+        const int64_t tiles = panels * ((d + mm::TILE - 1) / mm::TILE);
+        const int64_t want = (p.vc / 32 + t / 32) / std::max<int64_t>(1, t / 32);
+        p.splits = (int)std::max<int64_t>(1, std::min({want, (tiles >= 32 ? 768 : 256) / tiles, p.vc / mm::TILE}));
         p.row = take(sizeof(Row) * p.tp);
         p.at = take(4 * p.tp);
         p.gs = take(8);
-        p.D = take((size_t)p.planes * p.tp * p.vc * 2);
+        p.D = take((size_t)p.planes * p.tp * p.vmax * 2);
         p.dq = take((size_t)p.splits * t * p.ldp * 4);
     }
     p.bytes = o;
@@ -507,21 +591,17 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
 }
 
 template <bool F32>
-int pack(const void *X, int64_t rows, int d, int kp, const int64_t *targets, void *out, hipStream_t s) {
-    hipLaunchKernelGGL(k_pack<F32>, dim3(grid1(rows * kp, 256, 65536)), dim3(256), 0, s, X, rows, d, kp, targets,
-                       (uint16_t *)out);
-    MN_KCHECK(s, "k_pack");
+int prep(const Plan &p, const void *Q, const void *C, const int64_t *targets, char *w, const Rows &r, int64_t row_blocks,
+         hipStream_t s) {
+    auto one = [&](const void *X, size_t out, int64_t n, const int64_t *tg) {
+        Pack k = {X, (uint16_t *)(w + out), tg, n, p.d, p.kp, 0, p.d % (F32 ? 4 : 8) == 0};
+        k.blocks = (int)((n * (p.kp / 8) + 256 * kPackPer - 1) / (256 * kPackPer));
+        return k;
+    };
+    const Pack q = one(Q, p.q, p.t, targets), c = p.pack_c ? one(C, p.c, p.v, nullptr) : Pack{};
+    hipLaunchKernelGGL(k_prep<F32>, dim3((unsigned)(q.blocks + c.blocks + row_blocks)), dim3(256), 0, s, q, c, r);
+    MN_KCHECK(s, "k_prep");
     return MN_OK;
-}
-
-static int operands(const Plan &p, const void *Q, const void *C, bool f32, const int64_t *zero_rows, char *ws,
-                    hipStream_t s) {
-    int rc = f32 ? pack<true>(Q, p.t, p.d, p.kp, zero_rows, ws + p.q, s)
-                 : pack<false>(Q, p.t, p.d, p.kp, zero_rows, ws + p.q, s);
-    if (rc == MN_OK && p.pack_c)
-        rc = f32 ? pack<true>(C, p.v, p.d, p.kp, nullptr, ws + p.c, s)
-                 : pack<false>(C, p.v, p.d, p.kp, nullptr, ws + p.c, s);
-    return rc;
 }
 
 static mm::NtArgs nt_args(const Plan &p, const void *C, char *ws) {
@@ -531,35 +611,39 @@ static mm::NtArgs nt_args(const Plan &p, const void *C, char *ws) {
     return a;
 }
 
-static int stats_impl(const void *Q, const void *C, int32_t x_type, int64_t t, int64_t v, int32_t d,
-                      const int64_t *targets, int64_t c_offset, float scale, float *rest, float *zt, float *loss,
-                      float *mean, void *ws, hipStream_t s) {
-    const bool f32 = x_type == MN_F32;
-    const Plan p = make_plan(t, v, d, f32, false);
+template <bool F32>
+int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, const int64_t *targets, int64_t c_offset,
+               float scale, float *rest, float *zt, float *loss, float *mean, void *ws, hipStream_t s) {
+    const Plan p = make_plan(t, v, d, F32, false);
     char *w = (char *)ws;
-    const int rc = operands(p, Q, C, f32, nullptr, w, s);
+    int32_t *done = (int32_t *)(w + p.done);
+    Rows r = {};
+    r.t = t;
+    r.v = v;
+    r.c_offset = c_offset;
+    r.targets = targets;
+    r.Q = Q;
+    r.C = C;
+    r.d = d;
+    r.zt_out = zt;
+    r.done = done;
+    r.scale = scale;
+    const int rc = prep<F32>(p, Q, C, targets, w, r, (t + 3) / 4, s);
     if (rc != MN_OK) return rc;
-    hipLaunchKernelGGL(k_fill, dim3(grid1(t, 256)), dim3(256), 0, s, zt, t, -__builtin_inff());
-    MN_KCHECK(s, "k_fill");
     const mm::NtArgs a = nt_args(p, C, w);
     StatsEpi epi = {};
     epi.part = (float2 *)(w + p.part);
-    epi.zt = zt;
     epi.targets = targets;
     epi.c_offset = c_offset;
     epi.t = t;
     epi.v = (int)v;
-    epi.scale = scale;
     epi.scale2 = scale * kLog2e;
     hipLaunchKernelGGL((mm::k_nt<mm::Bf16, StatsEpi>), dim3((unsigned)(a.panels * a.slices)), dim3(mm::NT), 0, s, a, epi);
     MN_KCHECK(s, "k_nt");
     hipLaunchKernelGGL(k_join, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, epi.part, (const float *)nullptr,
-                       (const float *)nullptr, (int64_t)a.slices * 2, t, targets, rest, zt, loss);
+                       (const float *)nullptr, (int64_t)a.slices * 2, t, targets, rest, zt, loss, mean,
+                       mean ? done : (int32_t *)nullptr);
     MN_KCHECK(s, "k_join");
-    if (mean) {
-        hipLaunchKernelGGL(k_mean, dim3(1), dim3(1024), 0, s, loss, targets, t, mean);
-        MN_KCHECK(s, "k_mean");
-    }
     return MN_OK;
 }
 
@@ -569,29 +653,44 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
                   int64_t grad_n, const float *grad_scale, void *dQ, void *dC, void *ws, hipStream_t s) {
     const Plan p = make_plan(t, v, d, F32, true);
     char *w = (char *)ws;
-    const int rc = operands(p, Q, C, F32, targets, w, s);
-    if (rc != MN_OK) return rc;
     float *gs = (float *)(w + p.gs);
     Row *row = (Row *)(w + p.row);
     int32_t *at = (int32_t *)(w + p.at);
-    hipLaunchKernelGGL(k_grad_scale, dim3(1), dim3(1024), 0, s, grad, grad_n, grad_scale, targets, scale, gs);
-    MN_KCHECK(s, "k_grad_scale");
-    hipLaunchKernelGGL(k_rows, dim3(grid1(p.tp, 256)), dim3(256), 0, s, rest, zt, targets, c_offset, t, p.tp, v, grad,
-                       grad_n, gs, F32, row, at);
-    MN_KCHECK(s, "k_rows");
+    if (grad_n != 1) {
+        hipLaunchKernelGGL(k_grad_max, dim3(1), dim3(1024), 0, s, grad, t, targets, gs);
+        MN_KCHECK(s, "k_grad_max");
+    }
+    Rows r = {};
+    r.t = t;
+    r.tp = p.tp;
+    r.v = v;
+    r.c_offset = c_offset;
+    r.targets = targets;
+    r.rest = rest;
+    r.zt = zt;
+    r.grad = grad;
+    r.grad_scale = grad_scale;
+    r.grad_n = grad_n;
+    r.scale = scale;
+    r.gs = gs;
+    r.row = row;
+    r.at = at;
+    const int rc = prep<F32>(p, Q, C, targets, w, r, p.tp / 256, s);
+    if (rc != MN_OK) return rc;
     constexpr int PL = F32 ? 3 : 1;
     const char *Cp = p.pack_c ? w + p.c : (const char *)C;
     const int row_tiles = (int)(p.tp / mm::TILE), col_tiles = (d + mm::TILE - 1) / mm::TILE;
-    for (int64_t j0 = 0; j0 < v; j0 += p.vc) {
-        const int64_t vn = std::min(p.vc, v - j0);           // items of this piece
+    int64_t vn = 0;
+    for (int64_t j0 = 0; j0 < v; j0 += vn) {
+        vn = v - j0 <= p.vmax ? v - j0 : p.vc;  // items of this piece
         mm::NtArgs a = nt_args(p, C, w);
         a.B += j0 * a.ldb;
         a.n = vn;
         mm::plan_runs(a);
         DlogitsEpi<PL> epi = {};
         epi.D = (uint16_t *)(w + p.D);
-        epi.ldd = p.vc;
-        epi.plane = p.tp * p.vc;
+        epi.ldd = p.vmax;
+        epi.plane = p.tp * p.vmax;
         epi.v = (int)vn;
         epi.row = row;
         epi.at_ = at;
@@ -602,34 +701,31 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         MN_KCHECK(s, "k_nt");
         mm::KnArgs g = {};
         g.A = w + p.D;
-        g.lda = 2 * p.vc;
+        g.lda = 2 * p.vmax;
         g.ldb = 2 * p.kp;
-        g.planeA = 2 * p.tp * p.vc;
+        g.planeA = 2 * p.tp * p.vmax;
         g.nseg = F32 ? 6 : 1;
-        if (dQ) {
-            g.B = Cp + j0 * g.ldb;
-            g.planeB = v * g.ldb;
-            g.k = vn;
-            g.steps_all = (int)((vn + 31) / 32);
-            g.steps = (g.steps_all + p.splits - 1) / p.splits;
-            PartEpi pe = {(float *)(w + p.dq), t, p.ldp, j0 == 0};
-            hipLaunchKernelGGL((mm::k_kn<false, PartEpi>), dim3(col_tiles, row_tiles, p.splits), dim3(mm::NT), 0, s, g, pe);
-            MN_KCHECK(s, "k_kn");
-        }
-        if (dC) {
-            g.B = w + p.q;
-            g.planeB = t * g.ldb;
-            g.k = t;
-            g.steps_all = g.steps = (int)((t + 31) / 32);
-            GradEpi<F32> ge = {(char *)dC + j0 * d * (F32 ? 4 : 2), vn, d, gs};
-            hipLaunchKernelGGL((mm::k_kn<true, GradEpi<F32>>), dim3(col_tiles, (unsigned)((vn + mm::TILE - 1) / mm::TILE), 1),
-                               dim3(mm::NT), 0, s, g, ge);
-            MN_KCHECK(s, "k_kn");
-        }
+        mm::KnArgs gq = g, gc = g;
+        gq.B = Cp + j0 * g.ldb;
+        gq.planeB = v * g.ldb;
+        gq.k = vn;
+        gq.steps_all = (int)((vn + 31) / 32);
+        gq.steps = (gq.steps_all + p.splits - 1) / p.splits;
+        gc.B = w + p.q;
+        gc.planeB = t * g.ldb;
+        gc.k = t;
+        gc.steps_all = gc.steps = (int)((t + 31) / 32);
+        const mm::KnGrid nq = {dQ ? col_tiles : 0, row_tiles, p.splits};
+        const mm::KnGrid nc = {dC ? col_tiles : 0, (int)((vn + mm::TILE - 1) / mm::TILE), 1};
+        const PartEpi pe = {(float *)(w + p.dq), t, p.ldp, j0 == 0};
+        const GradEpi<F32> ge = {(char *)dC + j0 * d * (F32 ? 4 : 2), vn, d, gs};
+        hipLaunchKernelGGL((mm::k_kn2<PartEpi, GradEpi<F32>>), dim3((unsigned)(nq.blocks() + nc.blocks())), dim3(mm::NT), 0,
+                           s, gq, pe, nq, gc, ge, nc);
+        MN_KCHECK(s, "k_kn2");
     }
     if (dQ) {
-        hipLaunchKernelGGL(k_reduce_dq<F32>, dim3(grid1(t * d, 256, 65536)), dim3(256), 0, s, (const float *)(w + p.dq),
-                           p.splits, p.ldp, t, d, (const uint16_t *)C, row, at, targets, gs, dQ);
+        hipLaunchKernelGGL(k_reduce_dq<F32>, dim3((unsigned)((t * (p.ldp / 4) + 255) / 256)), dim3(256), 0, s,
+                           (const float *)(w + p.dq), p.splits, p.ldp, t, d, (const uint16_t *)C, row, at, targets, gs, dQ);
         MN_KCHECK(s, "k_reduce_dq");
     }
     return MN_OK;
@@ -642,6 +738,7 @@ static int check_args(const char *who, int32_t x_type, int64_t t, int64_t v, int
     MN_REQUIRE(std::isfinite(scale) && scale > 0.f, MN_EINVAL, "%s: scale has to be positive and finite", who);
     MN_REQUIRE(t <= (1 << 24) && v < INT_MAX - 1024 && d <= 65536, MN_ENOTSUP,
                "%s: t <= 2^24, v < 2^31 - 1025, d <= 65536", who);
+    MN_REQUIRE(v * ((d + 31) / 32) / 512 < (1 << 30), MN_ENOTSUP, "%s: v d too large for one call", who);
     MN_REQUIRE((t + 255) / 256 * ((v + 255) / 256) < (1 << 30), MN_ENOTSUP, "%s: t v too large for one call", who);
     return MN_OK;
 }
@@ -682,7 +779,8 @@ extern "C" int mn_softmax_stats(const void *Q, const void *C, int32_t x_type, in
     const size_t need = make_plan(t, v, d, x_type == MN_F32, false).bytes;
     MN_REQUIRE(ws && ws_bytes >= need && aligned16(ws), MN_ECAP,
                "mn_softmax_stats: workspace of %zu bytes (16-byte aligned) needed", need);
-    return stats_impl(Q, C, x_type, t, v, d, targets, c_offset, scale, rest, zt, loss, mean, ws, s);
+    return x_type == MN_F32 ? stats_impl<true>(Q, C, t, v, d, targets, c_offset, scale, rest, zt, loss, mean, ws, s)
+                            : stats_impl<false>(Q, C, t, v, d, targets, c_offset, scale, rest, zt, loss, mean, ws, s);
 }
 
 extern "C" int mn_softmax_merge(const float *rests, const float *zts, int64_t parts, int64_t t,
@@ -696,7 +794,7 @@ extern "C" int mn_softmax_merge(const float *rests, const float *zts, int64_t pa
     hipStream_t s = (hipStream_t)stream;
     if (t > 0) {
         hipLaunchKernelGGL(k_join, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, (const float2 *)nullptr, rests, zts,
-                           parts, t, targets, rest, zt, loss);
+                           parts, t, targets, rest, zt, loss, (float *)nullptr, (int32_t *)nullptr);
         MN_KCHECK(s, "k_join");
     }
     if (mean) {

@@ -1,7 +1,6 @@
 """Device-memory plumbing via PyTorch-ROCm (allocation and streams only)."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import numpy as np
@@ -18,28 +17,36 @@ def require_cuda(t: torch.Tensor, dtype, name: str, ndim: int | None = None) -> 
     return t.contiguous()
 
 
-def require_aligned(t: torch.Tensor, dtype, name: str, ndim: int | None = None) -> torch.Tensor:
+def require_aligned(t: torch.Tensor, dtype, name: str, ndim: int, device=None) -> torch.Tensor:
     """require_cuda, and a copy where the rows start off a 16-byte border (a
-    slice of a larger tensor) or another device than the current one holds them."""
+    slice of a larger tensor); device: where the call's other tensors are."""
     t = require_cuda(t, dtype, name, ndim)
-    if t.device.index is not None and t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, another tensor of the call on cuda:{torch.cuda.current_device()}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, other tensors of the call on {device}")
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-@contextlib.contextmanager
-def enqueue(stream, *tensors):
-    """For calls that return before their work is done: inside, `stream` is the
-    current one, so that what is allocated belongs to it, and the inputs' memory
-    is kept until its work on them is done."""
-    if stream is None:
-        yield
-        return
-    with torch.cuda.stream(stream):
-        for t in tensors:
-            if isinstance(t, torch.Tensor) and t.device.type == "cuda":
-                t.record_stream(stream)
-        yield
+def on_stream(fn):
+    """For calls that return before their work is done: with `stream` given, it
+    is the current stream inside, so that what is allocated belongs to it, and
+    the inputs' memory is kept until its work on them is done."""
+    import functools
+
+    @functools.wraps(fn)
+    def wrapped(*args, stream=None, **kwargs):
+        if stream is None:
+            return fn(*args, **kwargs)
+        with torch.cuda.stream(stream):
+            for a in (*args, *kwargs.values()):
+                for t in (a, getattr(a, "codes", None), getattr(a, "scale", None)):
+                    if isinstance(t, torch.Tensor) and t.device.type == "cuda":
+                        t.record_stream(stream)
+            return fn(*args, **kwargs)
+    return wrapped
+
+
+def current_stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
 
 
 def ptr(t: torch.Tensor) -> C.c_void_p:

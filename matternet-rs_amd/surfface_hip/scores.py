@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._torch import enqueue, on_device, ptr, require_aligned, stream_handle
+from ._torch import current_stream, on_device, on_stream, require_aligned, require_cuda
 
 VALUE_TYPES = {torch.float32: _lib.MN_F32, torch.bfloat16: _lib.MN_BF16}
 
@@ -40,11 +40,11 @@ class Int8Rows:
         return self.codes.shape[0]
 
 
-def _rows(r: Int8Rows, name: str):
+def _rows(r: Int8Rows, name: str, device=None):
     if not isinstance(r, Int8Rows):
         raise TypeError(f"{name} must be Int8Rows (quantize_rows)")
-    codes = require_aligned(r.codes, torch.int8, f"{name}.codes", 2)
-    scale = require_aligned(r.scale, torch.float32, f"{name}.scale", 1)
+    codes = require_aligned(r.codes, torch.int8, f"{name}.codes", 2, device)
+    scale = require_aligned(r.scale, torch.float32, f"{name}.scale", 1, codes.device)
     n, ld = codes.shape
     if scale.shape[0] != n:
         raise ValueError(f"{name} has {n} rows and {scale.shape[0]} scales")
@@ -54,56 +54,60 @@ def _rows(r: Int8Rows, name: str):
 
 
 @on_device
-def quantize_rows(X: torch.Tensor, stream=None) -> Int8Rows:
+@on_stream
+def quantize_rows(X: torch.Tensor) -> Int8Rows:
     """Rows of X [n, d] (f32 or bf16) in 8 bits: scale = max|x| / 127, code =
     rint(x (127 (1 / max|x|))).  A row of zeros gets scale 0; a row that holds an
     infinity or a NaN gets scale NaN, which every score with it shows."""
     if not isinstance(X, torch.Tensor) or X.dtype not in VALUE_TYPES:
         raise TypeError("X must be a float32 or bfloat16 tensor")
-    with enqueue(stream, X):
-        x = require_aligned(X, X.dtype, "X", 2)
-        n, d = x.shape
-        if d < 1:
-            raise ValueError("X has no columns")
-        codes = torch.empty((n, row_stride(d)), dtype=torch.int8, device=x.device)
-        scale = torch.empty(n, dtype=torch.float32, device=x.device)
-        _lib.check(_lib.lib().mn_quantize_rows_i8(ptr(x), VALUE_TYPES[x.dtype], n, d, ptr(codes),
-                                                  codes.shape[1], ptr(scale), stream_handle()))
+    x = require_cuda(X, X.dtype, "X", 2)
+    n, d = x.shape
+    if d < 1:
+        raise ValueError("X has no columns")
+    ld = row_stride(d)
+    codes = torch.empty((n, ld), dtype=torch.int8, device=x.device)
+    scale = torch.empty(n, dtype=torch.float32, device=x.device)
+    _lib.check(_lib.lib().mn_quantize_rows_i8(x.data_ptr(), VALUE_TYPES[x.dtype], n, d, codes.data_ptr(), ld,
+                                              scale.data_ptr(), current_stream()))
     return Int8Rows(codes, scale, d)
 
 
 @on_device
-def dequantize_rows(rows: Int8Rows, dtype=torch.float32, stream=None) -> torch.Tensor:
+@on_stream
+def dequantize_rows(rows: Int8Rows, dtype=torch.float32) -> torch.Tensor:
     """The values [n, d] that the codes stand for, as f32 or rounded to bf16."""
     if dtype not in VALUE_TYPES:
         raise TypeError("dtype must be float32 or bfloat16")
-    with enqueue(stream, rows.codes, rows.scale):
-        codes, scale, n, ld = _rows(rows, "rows")
-        X = torch.empty((n, rows.d), dtype=dtype, device=codes.device)
-        _lib.check(_lib.lib().mn_dequantize_rows_i8(ptr(codes), ld, ptr(scale), n, rows.d, ptr(X),
-                                                    VALUE_TYPES[dtype], stream_handle()))
+    codes, scale, n, ld = _rows(rows, "rows")
+    X = torch.empty((n, rows.d), dtype=dtype, device=codes.device)
+    _lib.check(_lib.lib().mn_dequantize_rows_i8(codes.data_ptr(), ld, scale.data_ptr(), n, rows.d, X.data_ptr(),
+                                                VALUE_TYPES[dtype], current_stream()))
     return X
 
 
 @on_device
-def scores_i8(queries: Int8Rows, items: Int8Rows, dtype=torch.float32, stream=None) -> torch.Tensor:
+@on_stream
+def scores_i8(queries: Int8Rows, items: Int8Rows, dtype=torch.float32) -> torch.Tensor:
     """[m, n] scores of every query with every item: the int8 product (exact
     sums, d <= 131071) times the query's and the item's scale, f32 or rounded
     to bf16."""
     if dtype not in VALUE_TYPES:
         raise TypeError("dtype must be float32 or bfloat16")
-    if not isinstance(queries, Int8Rows) or not isinstance(items, Int8Rows):
-        raise TypeError("queries and items must be Int8Rows (quantize_rows)")
-    if queries.d != items.d:
-        raise ValueError(f"queries have {queries.d} columns, items {items.d}")
-    with enqueue(stream, queries.codes, queries.scale, items.codes, items.scale):
-        q, qs, m, ldq = _rows(queries, "queries")
-        c, cs, n, ldc = _rows(items, "items")
-        L = _lib.lib()
-        need = C.c_size_t()
-        _lib.check(L.mn_scores_i8_workspace(m, queries.d, C.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.int8, device=c.device)
-        Y = torch.empty((m, n), dtype=dtype, device=c.device)
-        _lib.check(L.mn_scores_i8(ptr(q), ldq, ptr(qs), m, ptr(c), ldc, ptr(cs), n, queries.d, ptr(Y),
-                                  VALUE_TYPES[dtype], ptr(ws), need.value, stream_handle()))
+    c, cs, n, ldc = _rows(items, "items")
+    q, qs, m, ldq = _rows(queries, "queries", c.device)
+    d = queries.d
+    if d != items.d:
+        raise ValueError(f"queries have {d} columns, items {items.d}")
+    L = _lib.lib()
+    need = 0
+    if d % 64:  # whole k-steps need no workspace
+        b = C.c_size_t()
+        _lib.check(L.mn_scores_i8_workspace(m, d, C.byref(b)))
+        need = b.value
+    ws = torch.empty(need, dtype=torch.int8, device=c.device) if need else None
+    Y = torch.empty((m, n), dtype=dtype, device=c.device)
+    _lib.check(L.mn_scores_i8(q.data_ptr(), ldq, qs.data_ptr(), m, c.data_ptr(), ldc, cs.data_ptr(), n, d,
+                              Y.data_ptr(), VALUE_TYPES[dtype], ws.data_ptr() if need else None, need,
+                              current_stream()))
     return Y

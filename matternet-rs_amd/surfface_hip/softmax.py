@@ -21,7 +21,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._torch import enqueue, on_device, ptr, require_aligned, stream_handle
+from ._torch import current_stream, on_device, on_stream, require_aligned, require_cuda
 from .scores import VALUE_TYPES
 
 
@@ -40,99 +40,106 @@ def _inputs(Q, items, targets):
     if not isinstance(Q, torch.Tensor) or Q.dtype not in VALUE_TYPES:
         raise TypeError("queries must be a float32 or bfloat16 tensor")
     q = require_aligned(Q, Q.dtype, "queries", 2)
-    c = require_aligned(items, Q.dtype, "items", 2)
+    c = require_aligned(items, Q.dtype, "items", 2, q.device)
     if isinstance(targets, torch.Tensor) and targets.dtype == torch.int32:
         targets = targets.long()
-    t = require_aligned(targets, torch.int64, "targets", 1)
-    if q.shape[1] != c.shape[1]:
-        raise ValueError(f"queries have {q.shape[1]} columns, items {c.shape[1]}")
-    if t.shape[0] != q.shape[0]:
-        raise ValueError(f"{q.shape[0]} queries and {t.shape[0]} targets")
-    if c.shape[0] < 1 or c.shape[1] < 1:
+    t = require_aligned(targets, torch.int64, "targets", 1, q.device)
+    n, d = q.shape
+    v = c.shape[0]
+    if c.shape[1] != d:
+        raise ValueError(f"queries have {d} columns, items {c.shape[1]}")
+    if t.shape[0] != n:
+        raise ValueError(f"{n} queries and {t.shape[0]} targets")
+    if v < 1 or d < 1:
         raise ValueError("items has no rows or no columns")
-    if not q.device == c.device == t.device:
-        raise ValueError("queries, items and targets must be on one device")
-    return q, c, t
+    return q, c, t, n, v, d, VALUE_TYPES[Q.dtype]
 
 
-def _workspace(q, c, backward):
+def _values(x, name, device, *sizes):
+    """A dense f32 vector of one of these sizes."""
+    x = require_cuda(x.reshape(-1), torch.float32, name)
+    if x.shape[0] not in sizes:
+        raise ValueError(f"{name} needs {' or '.join(map(str, sizes))} values, got {x.shape[0]}")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, other tensors of the call on {device}")
+    return x
+
+
+def _workspace(L, n, v, d, kind, backward, device):
     need = C.c_size_t()
-    _lib.check(_lib.lib().mn_softmax_workspace(q.shape[0], c.shape[0], q.shape[1], VALUE_TYPES[q.dtype],
-                                               backward, C.byref(need)))
-    return torch.empty(need.value, dtype=torch.int8, device=q.device)
+    _lib.check(L.mn_softmax_workspace(n, v, d, kind, backward, C.byref(need)))
+    return torch.empty(need.value, dtype=torch.int8, device=device)
+
+
+def _stats_out(n, device):
+    out = torch.empty((3, n), dtype=torch.float32, device=device)
+    mean = torch.empty(2, dtype=torch.float32, device=device)
+    return SoftmaxStats(*out.unbind(), mean), out.data_ptr(), mean.data_ptr()
 
 
 @on_device
+@on_stream
 def softmax_stats(queries: torch.Tensor, items: torch.Tensor, targets: torch.Tensor, scale: float = 1.0,
-                  c_offset: int = 0, stream=None) -> SoftmaxStats:
+                  c_offset: int = 0) -> SoftmaxStats:
     """queries [t, d], items [v, d] (f32 or bf16), targets [t] (int64 or int32,
     global row ids; negative: the query has no part); logits scale q.c, scale >
     0.  items holds the rows c_offset .. c_offset + v - 1 of the table; a target
     among none of a table's rows makes its loss +inf."""
-    with enqueue(stream, queries, items, targets):
-        q, c, t = _inputs(queries, items, targets)
-        out = torch.empty((3, q.shape[0]), dtype=torch.float32, device=q.device)
-        mean = torch.empty(2, dtype=torch.float32, device=q.device)
-        ws = _workspace(q, c, 0)
-        _lib.check(_lib.lib().mn_softmax_stats(
-            ptr(q), ptr(c), VALUE_TYPES[q.dtype], q.shape[0], c.shape[0], q.shape[1], ptr(t), c_offset,
-            float(scale), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(mean), ptr(ws), ws.numel(),
-            stream_handle()))
-    return SoftmaxStats(out[0], out[1], out[2], mean)
+    q, c, t, n, v, d, kind = _inputs(queries, items, targets)
+    st, o, mean = _stats_out(n, q.device)
+    L = _lib.lib()
+    ws = _workspace(L, n, v, d, kind, 0, q.device)
+    _lib.check(L.mn_softmax_stats(q.data_ptr(), c.data_ptr(), kind, n, v, d, t.data_ptr(), c_offset, float(scale),
+                                  o, o + 4 * n, o + 8 * n, mean, ws.data_ptr(), ws.numel(), current_stream()))
+    return st
 
 
 @on_device
-def softmax_merge(rests: torch.Tensor, zts: torch.Tensor, targets: torch.Tensor, stream=None) -> SoftmaxStats:
+@on_stream
+def softmax_merge(rests: torch.Tensor, zts: torch.Tensor, targets: torch.Tensor) -> SoftmaxStats:
     """The stats of a whole table from those of its row ranges: rests and zts
     [parts, t] (softmax_stats' rest and target, gathered over the ranges)."""
-    with enqueue(stream, rests, zts, targets):
-        r = require_aligned(rests, torch.float32, "rests", 2)
-        z = require_aligned(zts, torch.float32, "zts", 2)
-        t = require_aligned(targets.long(), torch.int64, "targets", 1)
-        if r.shape != z.shape or r.shape[1] != t.shape[0] or r.shape[0] < 1:
-            raise ValueError(f"rests {tuple(r.shape)}, zts {tuple(z.shape)} and targets {tuple(t.shape)} do not fit")
-        out = torch.empty((3, t.shape[0]), dtype=torch.float32, device=r.device)
-        mean = torch.empty(2, dtype=torch.float32, device=r.device)
-        _lib.check(_lib.lib().mn_softmax_merge(ptr(r), ptr(z), r.shape[0], t.shape[0], ptr(t), ptr(out[0]),
-                                               ptr(out[1]), ptr(out[2]), ptr(mean), stream_handle()))
-    return SoftmaxStats(out[0], out[1], out[2], mean)
+    r = require_aligned(rests, torch.float32, "rests", 2)
+    z = require_aligned(zts, torch.float32, "zts", 2, r.device)
+    if isinstance(targets, torch.Tensor) and targets.dtype == torch.int32:
+        targets = targets.long()
+    t = require_aligned(targets, torch.int64, "targets", 1, r.device)
+    parts, n = r.shape
+    if r.shape != z.shape or n != t.shape[0] or parts < 1:
+        raise ValueError(f"rests {tuple(r.shape)}, zts {tuple(z.shape)} and targets {tuple(t.shape)} do not fit")
+    st, o, mean = _stats_out(n, r.device)
+    _lib.check(_lib.lib().mn_softmax_merge(r.data_ptr(), z.data_ptr(), parts, n, t.data_ptr(), o, o + 4 * n,
+                                           o + 8 * n, mean, current_stream()))
+    return st
 
 
 @on_device
+@on_stream
 def softmax_backward(queries: torch.Tensor, items: torch.Tensor, targets: torch.Tensor, rest: torch.Tensor,
                      target: torch.Tensor, grad: torch.Tensor, scale: float = 1.0, c_offset: int = 0,
-                     grad_scale: torch.Tensor | None = None, need=(True, True), stream=None):
+                     grad_scale: torch.Tensor | None = None, need=(True, True)):
     """(d queries, d items) of sum(grad * loss), from the WHOLE table's rest and
     target (softmax_stats, or softmax_merge where items is a row range: then d
     queries is the range's part, to be added up).  grad: f32, one value per
     query or one for all; grad_scale: one f32 that multiplies it (mean[1] for
     the mean).  need: which of the two to compute (None for the other)."""
-    with enqueue(stream, queries, items, targets, rest, target, grad, grad_scale):
-        q, c, t = _inputs(queries, items, targets)
-        n = q.shape[0]
-        re = require_aligned(rest, torch.float32, "rest", 1)
-        zt = require_aligned(target, torch.float32, "target", 1)
-        g = require_aligned(grad.reshape(-1), torch.float32, "grad", 1)
-        if re.shape[0] != n or zt.shape[0] != n:
-            raise ValueError(f"rest and target need {n} values")
-        if g.shape[0] not in (1, n):
-            raise ValueError(f"grad needs 1 or {n} values, got {g.shape[0]}")
-        gs = None
-        if grad_scale is not None:
-            gs = require_aligned(grad_scale.reshape(-1), torch.float32, "grad_scale", 1)
-            if gs.shape[0] != 1:
-                raise ValueError("grad_scale needs one value")
-        dq = torch.empty_like(q) if need[0] else None
-        dc = torch.empty_like(c) if need[1] else None
-        if n == 0:
-            return dq, dc.zero_() if need[1] else None
-        if need[0] or need[1]:
-            ws = _workspace(q, c, 1)
-            _lib.check(_lib.lib().mn_softmax_backward(
-                ptr(q), ptr(c), VALUE_TYPES[q.dtype], n, c.shape[0], q.shape[1], ptr(t), c_offset, float(scale),
-                ptr(re), ptr(zt), ptr(g), g.shape[0], ptr(gs) if gs is not None else None,
-                ptr(dq) if need[0] else None, ptr(dc) if need[1] else None, ptr(ws), ws.numel(),
-                stream_handle()))
+    q, c, t, n, v, d, kind = _inputs(queries, items, targets)
+    re = _values(rest, "rest", q.device, n)
+    zt = _values(target, "target", q.device, n)
+    g = _values(grad, "grad", q.device, 1, n)
+    gs = None if grad_scale is None else _values(grad_scale, "grad_scale", q.device, 1)
+    dq = torch.empty_like(q) if need[0] else None
+    dc = torch.empty_like(c) if need[1] else None
+    if n == 0:
+        return dq, dc.zero_() if need[1] else None
+    if need[0] or need[1]:
+        L = _lib.lib()
+        ws = _workspace(L, n, v, d, kind, 1, q.device)
+        _lib.check(L.mn_softmax_backward(
+            q.data_ptr(), c.data_ptr(), kind, n, v, d, t.data_ptr(), c_offset, float(scale), re.data_ptr(),
+            zt.data_ptr(), g.data_ptr(), g.shape[0], None if gs is None else gs.data_ptr(),
+            dq.data_ptr() if need[0] else None, dc.data_ptr() if need[1] else None, ws.data_ptr(), ws.numel(),
+            current_stream()))
     return dq, dc
 
 
@@ -140,19 +147,19 @@ class _SoftmaxLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, queries, items, targets, scale, reduction):
         st = softmax_stats(queries, items, targets, scale)
-        ctx.save_for_backward(queries, items, targets, st.rest, st.target, st.mean)
-        ctx.scale, ctx.reduction = scale, reduction
-        if reduction == "mean":
-            return st.mean[0].clone()
-        return st.loss if reduction == "none" else st.loss.sum()
+        ctx.save_for_backward(queries, items, targets)
+        ctx.stats, ctx.scale, ctx.mean = st, scale, reduction == "mean"
+        # the returned value shares no storage with what backward reads: the
+        # caller may change it in place
+        return (st.mean[0] if reduction == "mean" else st.loss if reduction == "none" else st.loss.sum()).clone()
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        queries, items, targets, rest, target, mean = ctx.saved_tensors
-        dq, dc = softmax_backward(queries, items, targets, rest, target, grad, ctx.scale,
-                                  grad_scale=mean[1] if ctx.reduction == "mean" else None,
-                                  need=ctx.needs_input_grad[:2])
+        queries, items, targets = ctx.saved_tensors
+        st = ctx.stats
+        dq, dc = softmax_backward(queries, items, targets, st.rest, st.target, grad, ctx.scale,
+                                  grad_scale=st.mean[1] if ctx.mean else None, need=ctx.needs_input_grad[:2])
         return dq, dc, None, None, None
 
 
