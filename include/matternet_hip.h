@@ -640,10 +640,10 @@ int mn_bf16_last_stats(mn_knn_stats *out);
  * at the caller's next synchronisation), take their workspace from the caller
  * and may be captured into a graph.  A workspace must not be used by two calls
  * that can run at the same time, two captured graphs that replay side by side
- * among them; its contents mean nothing between calls.  Pointers to X, Q, C,
- * codes and the workspace are 16-byte aligned (MN_EINVAL / MN_ECAP).  Matrices
- * are row-major and dense but for codes, whose rows are `ld` bytes apart (a
- * multiple of 16, >= d). */
+ * among them; its contents mean nothing between calls.  Q, C, codes and the
+ * workspace are 16-byte aligned (MN_EINVAL / MN_ECAP otherwise), X need not be.
+ * Matrices are row-major and dense but for codes, whose rows are `ld` bytes
+ * apart (a multiple of 16, >= d). */
 
 /* Per row a = max |x|: scale = a / 127, code = rint(x (127 (1 / a))) (f32, ties to
  * even), codes d .. ld - 1 of a row 0.  X [n][d] MN_F32 or MN_BF16.  A row of
@@ -670,9 +670,9 @@ int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, 
  * reaches no other row.
  * mn_softmax_stats writes per row rest = log sum exp z over the items but the
  * target, zt = the target's logit (-inf where it is not among the rows here),
- * loss = log(1 + exp(rest - zt)) (may be NULL; +inf where zt is -inf) and mean
- * (2 floats, may be NULL) = the mean of loss over the rows that take part and 1
- * / their number ((0, 1) when there is none).
+ * loss = log(1 + exp(rest - zt)) (+inf where zt is -inf), and where mean is not
+ * NULL the mean of loss over the rows that take part and share = 1 / their
+ * number (0 and 1 when there is none).
  * mn_softmax_merge joins the (rest, zt) [parts][t] of row ranges of a table to
  * those of the whole.
  * mn_softmax_backward takes the whole table's rest and zt, and grad: one value
@@ -688,10 +688,11 @@ int mn_softmax_workspace(int64_t t, int64_t v, int32_t d, int32_t x_type, int32_
                          size_t *bytes);
 int mn_softmax_stats(const void *Q, const void *C, int32_t x_type, int64_t t, int64_t v, int32_t d,
                      const int64_t *targets, int64_t c_offset, float scale, float *rest, float *zt,
-                     float *loss, float *mean, void *ws, size_t ws_bytes, void *stream);
+                     float *loss, float *mean, float *share, void *ws, size_t ws_bytes,
+                     void *stream);
 int mn_softmax_merge(const float *rests, const float *zts, int64_t parts, int64_t t,
                      const int64_t *targets, float *rest, float *zt, float *loss, float *mean,
-                     void *stream);
+                     float *share, void *stream);
 int mn_softmax_backward(const void *Q, const void *C, int32_t x_type, int64_t t, int64_t v,
                         int32_t d, const int64_t *targets, int64_t c_offset, float scale,
                         const float *rest, const float *zt, const float *grad, int64_t grad_n,

@@ -106,14 +106,22 @@ __device__ __forceinline__ void dma4(const char *base, int voff, uint32_t lds) {
                  : "memory", "m0");
 }
 
+// one 16-byte store instruction, to base + voff
+__device__ __forceinline__ void store16(char *base, int voff, uint4 x) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, 0, 0xffffffffu, 0x00020000);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), r, voff, 0, 0);
+}
+
 // the end of a barrier window
 __device__ __forceinline__ void window_end() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
+// N: 8, or 8 and the stores issued since the loads of the step read next
+template <int N>
 __device__ __forceinline__ void read_window_end() {
-    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
     window_end();
 }
 
@@ -154,6 +162,9 @@ inline void plan_runs(NtArgs &a) {
     a.slices = (a.tiles + a.run - 1) / a.run;
 }
 
+// Epilogue: init (before the loop), fetch (a tile's loads to LDS; FETCH: there
+// are any), tile (a tile's accumulators; at least STORES store instructions of
+// each wave, whatever the data), finish.
 // accumulator r of tile (f, g): row i = 16 f + (lane & 15) of the wave's 64,
 // column j = 32 (g >> 1) + 8 (lane >> 4) + 4 (g & 1) + r of its 128, so that a
 // lane holds 8 neighbours of a row in each pair of tiles
@@ -252,7 +263,10 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
             fj[g] = *reinterpret_cast<const u32x4 *>(rj + so + (32 * (g >> 1) + 4 * (g & 1)) * KBY);
         issue();
         if (EPI::FETCH && per < 4) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        read_window_end();
+        // a tile's stores come between the loads of the next two steps and
+        // those of the third: they have two steps to drain
+        if (EPI::STORES > 0 && k < 2 && n >= per) read_window_end<(8 + EPI::STORES < 63 ? 8 + EPI::STORES : 63)>();
+        else read_window_end<8>();
 #pragma unroll
         for (int f = 0; f < 4; ++f)
 #pragma unroll
@@ -375,7 +389,7 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
 #pragma unroll
             for (int g = 0; g < 8; ++g) fj[g] = tr(&rg.b[0][1][0] + so, 8 * wj + g);
             issue();
-            read_window_end();
+            read_window_end<8>();
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll

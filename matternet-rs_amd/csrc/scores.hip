@@ -103,41 +103,42 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64
     if (l == 0) scale[i] = finite ? a / 127.f : __builtin_nanf("");
 }
 
-// 8 codes a thread at a time; a block takes 2048 pieces of 8 in a row
+// 16 bytes of values (4 f32 or 8 bf16) a thread at a time, so that a wave's
+// store is 1 KB in a row; a block takes 8 x 256 pieces.
 template <typename T>
 __global__ __launch_bounds__(256) void k_dequantize(const int8_t *__restrict__ codes, int64_t ld,
                                                     const float *__restrict__ scale, int64_t n, int d, bool vec,
                                                     T *__restrict__ X) {
-    const uint32_t n8 = (uint32_t)(d + 7) / 8;
-    const int64_t base = (int64_t)blockIdx.x * 2048, total = n * n8;
-    const int64_t row0 = base / n8;
-    const uint32_t rem = (uint32_t)(base - row0 * n8);
+    constexpr int P = 16 / sizeof(T);
+    const uint32_t np = (uint32_t)(d + P - 1) / P;
+    const int64_t base = (int64_t)blockIdx.x * 2048, total = n * np;
+    const int64_t row0 = base / np;
+    const uint32_t rem = (uint32_t)(base - row0 * np);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
         const uint32_t l = 256 * u + threadIdx.x;
         if (base + l >= total) return;
-        const uint32_t x = rem + l, q = x / n8;
-        const int k = 8 * (int)(x - q * n8);
+        const uint32_t x = rem + l, q = x / np;
+        const int k = P * (int)(x - q * np);
         const int64_t i = row0 + q;
         const float s = scale[i];
-        const uint2 c = *reinterpret_cast<const uint2 *>(codes + i * ld + k);
-        float v[8];
+        uint32_t c[2];
+        __builtin_memcpy(c, codes + i * ld + k, P);
+        float v[P];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3))) * s;
+        for (int e = 0; e < P; ++e) v[e] = (float)(int8_t)(c[e >> 2] >> (8 * (e & 3))) * s;
         T *out = X + i * d + k;
-        if (vec && k + 8 <= d) {
-            if constexpr (sizeof(T) == 4) {
-                reinterpret_cast<float4 *>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4 *>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
+        if (vec && k + P <= d) {
+            if constexpr (P == 4)
+                *reinterpret_cast<float4 *>(out) = make_float4(v[0], v[1], v[2], v[3]);
+            else
                 *reinterpret_cast<uint4 *>(out) = make_uint4(mm::bf16_pair(v[0], v[1]), mm::bf16_pair(v[2], v[3]),
                                                              mm::bf16_pair(v[4], v[5]), mm::bf16_pair(v[6], v[7]));
-            }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < P; ++e)
                 if (k + e < d) {
-                    if constexpr (sizeof(T) == 4) out[e] = v[e];
+                    if constexpr (P == 4) out[e] = v[e];
                     else out[e] = mm::bf16_bits(v[e]);
                 }
         }
@@ -161,6 +162,7 @@ struct ScoreEpi {
         float cs[2][mm::TILE];  // the items' scales of a tile, two tiles in turn
     };
     static constexpr bool FETCH = true;
+    static constexpr int STORES = 0;  // rows and columns past the end store nothing
     const float *qs, *cs;
     T *Y;
     int64_t m, n;
@@ -247,8 +249,8 @@ extern "C" int mn_quantize_rows_i8(const void *X, int32_t x_type, int64_t n, int
     mn::clear_error();
     MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX, MN_EINVAL,
                "mn_quantize_rows_i8: n >= 0, d >= 1, ld >= d and a multiple of 16 needed");
-    MN_REQUIRE(n < INT_MAX && n * ((d + 7) / 8) / 2048 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
-               "mn_quantize_rows_i8: n < 2^31 - 1 rows and n d < 2^44 needed");
+    MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 2048 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
+               "mn_quantize_rows_i8: n < 2^31 - 1 rows and n d < 2^43 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_quantize_rows_i8: MN_F32 or MN_BF16");
     if (n == 0) return MN_OK;
     MN_REQUIRE(X && codes && scale, MN_EINVAL, "mn_quantize_rows_i8: NULL pointer");
@@ -266,14 +268,15 @@ extern "C" int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const floa
     mn::clear_error();
     MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX, MN_EINVAL,
                "mn_dequantize_rows_i8: n >= 0, d >= 1, ld >= d and a multiple of 16 needed");
-    MN_REQUIRE(n < INT_MAX && n * ((d + 7) / 8) / 2048 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
-               "mn_dequantize_rows_i8: n < 2^31 - 1 rows and n d < 2^44 needed");
+    MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 2048 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
+               "mn_dequantize_rows_i8: n < 2^31 - 1 rows and n d < 2^43 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_dequantize_rows_i8: MN_F32 or MN_BF16");
     if (n == 0) return MN_OK;
     MN_REQUIRE(X && codes && scale, MN_EINVAL, "mn_dequantize_rows_i8: NULL pointer");
     MN_REQUIRE(aligned16(codes), MN_EINVAL, "mn_dequantize_rows_i8: codes not 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)((n * ((d + 7) / 8) + 2047) / 2048));
+    const int per = x_type == MN_F32 ? 4 : 8;
+    const dim3 grid((unsigned)((n * ((d + per - 1) / per) + 2047) / 2048));
     if (x_type == MN_F32)
         hipLaunchKernelGGL(k_dequantize<float>, grid, dim3(256), 0, s, codes, ld, scale, n, d,
                            d % 4 == 0 && aligned16(X), (float *)X);

@@ -102,15 +102,14 @@ __device__ __forceinline__ void pack(const Pack &p, int block) {
 __device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
 
 // What the rows need before the products: forward the targets' logits (a wave
-// a row: f32 sums of the d products) and the count of blocks of k_join that are
-// done; backward Row and the target within the rows of C here.
+// a row: f32 sums of the d products); backward Row and the target within the
+// rows of C here.
 struct Rows {
     int64_t t, tp, v, c_offset;
     const int64_t *targets;
     const void *Q, *C;
     int d;
     float *zt_out;         // forward
-    int32_t *done;
     const float *rest, *zt;  // backward (rest not NULL)
     const float *grad, *grad_scale;
     int64_t grad_n;
@@ -125,7 +124,6 @@ __device__ __forceinline__ void rows(const Rows &p, int block) {
     if (!p.rest) {
         const int lane = threadIdx.x & 63;
         const int64_t i = (int64_t)block * 4 + (threadIdx.x >> 6);
-        if (block == 0 && threadIdx.x == 0) *p.done = 0;
         if (i >= p.t) return;
         const int64_t at = p.targets[i] - p.c_offset;
         if (p.targets[i] < 0 || at < 0 || at >= p.v) {
@@ -187,6 +185,7 @@ __global__ __launch_bounds__(256) void k_prep(Pack q, Pack c, Rows r) {
 struct StatsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;
+    static constexpr int STORES = 0;
     float2 *part;
     const int64_t *targets;
     int64_t c_offset, t;
@@ -277,12 +276,15 @@ __device__ __forceinline__ float block_fold(float x, float *sh, F f) {
     return x;
 }
 
-// out = (mean of the losses of the rows that take part, 1 / their number); no
-// such row: (0, 1).  One block and a fixed order.
-__device__ __forceinline__ void mean_of(const float *loss, const int64_t *targets, int64_t t, float *out) {
+// The mean of the losses of the rows that take part and 1 / their number; no
+// such row: 0 and 1.  One block and a fixed order.  (As the last act of k_join's
+// last block it took 85 us longer at 4096 rows: every block's fence writes its
+// L2 back.)
+__global__ __launch_bounds__(1024) void k_mean(const float *__restrict__ loss, const int64_t *__restrict__ targets,
+                                               int64_t t, float *__restrict__ mean, float *__restrict__ share) {
     __shared__ float sh[16];
     float sum = 0.f, num = 0.f;
-    for (int64_t i = threadIdx.x; i < t; i += blockDim.x) {
+    for (int64_t i = threadIdx.x; i < t; i += 1024) {
         const bool has = targets[i] >= 0;
         sum += has ? loss[i] : 0.f;
         num += has ? 1.f : 0.f;
@@ -291,26 +293,22 @@ __device__ __forceinline__ void mean_of(const float *loss, const int64_t *target
     sum = block_fold(sum, sh, add);
     num = fmaxf(block_fold(num, sh, add), 1.f);
     if (threadIdx.x == 0) {
-        out[0] = sum / num;
-        out[1] = 1.f / num;
+        *mean = sum / num;
+        *share = 1.f / num;
     }
-}
-__global__ __launch_bounds__(1024) void k_mean(const float *loss, const int64_t *targets, int64_t t, float *out) {
-    mean_of(loss, targets, t, out);
 }
 
 // One wave a row: joins n (maximum, sum) pairs (base 2), or with `rests` n
-// values of rest and zt (the ranges of a table).  With `done` the block that
-// ends last takes the mean (it sees the others' losses: each counts itself
-// after a fence, it reads them after one).
+// values of rest and zt (the ranges of a table).
 __global__ __launch_bounds__(256) void k_join(const float2 *__restrict__ part, const float *__restrict__ rests,
                                               const float *__restrict__ zts, int64_t n, int64_t t,
-                                              const int64_t *__restrict__ targets, float *rest, float *zt,
-                                              float *loss, float *mean, int32_t *done) {
+                                              const int64_t *__restrict__ targets, float *__restrict__ rest,
+                                              float *__restrict__ zt, float *__restrict__ loss) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= t) return;
     float top = -__builtin_inff(), sum = 0.f, z = -__builtin_inff();
-    for (int64_t k = lane; k < n && i < t; k += 64) {
+    for (int64_t k = lane; k < n; k += 64) {
         float2 p;
         if (part) {
             p = part[k * t + i];
@@ -337,23 +335,13 @@ __global__ __launch_bounds__(256) void k_join(const float2 *__restrict__ part, c
         top = m;
         z = fmaxf(z, __shfl_xor(z, o));
     }
-    if (lane == 0 && i < t) {
+    if (lane == 0) {
         const float r = sum == 0.f ? -__builtin_inff() : (top == -__builtin_inff() ? sum : (top + log2f(sum)) * kLn2);
         if (!zts) z = zt[i];
         else zt[i] = z;
         rest[i] = r;
-        if (loss) loss[i] = targets[i] < 0 ? 0.f : row_loss(r, z);
+        loss[i] = targets[i] < 0 ? 0.f : row_loss(r, z);
     }
-    if (!done) return;
-    __shared__ int last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0)
-        last = __hip_atomic_fetch_add(done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    mean_of(loss, targets, t, mean);
 }
 
 // gs[1] = the largest |g| of the rows that take part
@@ -372,6 +360,7 @@ template <int PLANES>
 struct DlogitsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;
+    static constexpr int STORES = 16 * PLANES;
     uint16_t *D;
     int64_t ldd, plane;
     int v;  // columns of this piece that exist
@@ -406,8 +395,8 @@ struct DlogitsEpi {
 #pragma unroll
         for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 128u;
         const bool slow = __ballot(hit) != 0;
-        uint16_t *base = D + i0_ * ldd + j0;
-        const int lrow = (lane & 15) * (int)ldd + jl;
+        char *base = (char *)(D + i0_ * ldd + j0);
+        const int lrow = 2 * ((lane & 15) * (int)ldd + jl);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
 #pragma unroll
@@ -424,10 +413,10 @@ struct DlogitsEpi {
                         if (j >= v || !any) x[q] = 0.f;
                     }
                 }
-                uint16_t *p = base + (int64_t)16 * f * ldd + (lrow + 16 * g);
+                const int at_byte = lrow + 32 * f * (int)ldd + 32 * g;
                 if constexpr (PLANES == 1) {
-                    *reinterpret_cast<uint4 *>(p) = make_uint4(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]),
-                                                               mm::bf16_pair(x[4], x[5]), mm::bf16_pair(x[6], x[7]));
+                    mm::store16(base, at_byte, make_uint4(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]),
+                                                          mm::bf16_pair(x[4], x[5]), mm::bf16_pair(x[6], x[7])));
                 } else {
                     uint32_t o[3][4];
 #pragma unroll
@@ -440,7 +429,7 @@ struct DlogitsEpi {
                     }
 #pragma unroll
                     for (int s = 0; s < 3; ++s)
-                        *reinterpret_cast<uint4 *>(p + s * plane) = make_uint4(o[s][0], o[s][1], o[s][2], o[s][3]);
+                        mm::store16(base + 2 * s * plane, at_byte, make_uint4(o[s][0], o[s][1], o[s][2], o[s][3]));
                 }
             }
         }
@@ -448,8 +437,8 @@ struct DlogitsEpi {
     __device__ __forceinline__ void finish(Shared &, int64_t, int, int) {}
 };
 
-// partial sums of dQ: [splits][m][ld] f32 (ld a multiple of 4), added up over
-// the pieces of the table
+// partial sums of dQ: [splits][m][ld] f32 (ld a multiple of 4) of a piece of
+// the table, or added to those of the pieces before
 struct PartEpi {
     float *part;
     int64_t m, ld;
@@ -533,7 +522,9 @@ struct Plan {
     mm::NtArgs nt;      // the whole table's logits
     int64_t vc, vmax;   // items per piece (backward), of the longest piece, in whole tiles
     int splits;         // of dQ's sum over a piece
-    size_t q, c, part, done, row, at, gs, D, dq, bytes;
+    int pieces, parts;  // of the table; partial sums of dQ in all
+    bool apart;         // a piece's partial sums are its own
+    size_t q, c, part, row, at, gs, D, dq, bytes;
 };
 
 inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
@@ -561,7 +552,6 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
     if (!backward) {
         mm::plan_runs(p.nt);
         p.part = take((size_t)p.nt.slices * 2 * t * 8);
-        p.done = take(4);
     } else {
         // Pieces whose D stays below 256 MB and whose tiles fill whole rounds
         // of 256 blocks; a short rest joins the last piece where it fits.
@@ -574,17 +564,40 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         if (all > piece && rest > 0 && piece + rest <= most) longest = piece + rest;
         p.vc = std::min(piece, all) * mm::TILE;
         p.vmax = longest * mm::TILE;
-        // dQ's runs about as long as dC's sums (t), so that the last round of
-        // blocks ends together; more than a round of blocks only where the
-        // partial sums stay small next to the products
-        const int64_t tiles = panels * ((d + mm::TILE - 1) / mm::TILE);
-        const int64_t want = (p.vc / 32 + t / 32) / std::max<int64_t>(1, t / 32);
-        p.splits = (int)std::max<int64_t>(1, std::min({want, (tiles >= 32 ? 768 : 256) / tiles, p.vc / mm::TILE}));
+        // dQ's runs of k: the cut with the least time for the blocks of both
+        // products on 256 processors, dQ's first, in steps: a block of dQ
+        // costs its run and 20 for its part of the sum (256 KB to memory), one
+        // of dC t / 32 and 10.  Free processors take the next block: dC's done
+        // by a time are counted from the two times at which dQ's blocks end.
+        const int64_t cols = (d + mm::TILE - 1) / mm::TILE, tiles = panels * cols;
+        const int64_t steps = p.vc / 32, nc = p.vc / mm::TILE * cols, b = t / 32 + 10;
+        int64_t best = INT64_MAX;
+        for (int64_t s = 1; s <= std::min<int64_t>(steps / 4 + 1, std::max<int64_t>(1, 512 / tiles)); ++s) {
+            const int64_t a = (steps + s - 1) / s + 20, nq = tiles * s, full = nq / 256 * a, more = nq % 256;
+            int64_t end = full + (more ? a : 0);
+            for (int64_t k = (nc + 255) / 256;; ++k) {
+                const int64_t e1 = full + k * b, e2 = std::max<int64_t>(0, e1 - full - a) / b;
+                if ((256 - more) * k + more * e2 >= nc) {
+                    end = std::max(end, e1);
+                    break;
+                }
+            }
+            if (end < best) {
+                best = end;
+                p.splits = (int)s;
+            }
+        }
+        // every piece's partial sums apart (written once, read once) while
+        // they stay below 256 MB, else added up
+        p.pieces = 1;
+        for (int64_t j = 0; v - j > p.vmax; j += p.vc) ++p.pieces;
+        p.apart = (int64_t)p.pieces * p.splits * t * p.ldp * 4 <= ((int64_t)256 << 20);
+        p.parts = p.apart ? p.pieces * p.splits : p.splits;
         p.row = take(sizeof(Row) * p.tp);
         p.at = take(4 * p.tp);
         p.gs = take(8);
         p.D = take((size_t)p.planes * p.tp * p.vmax * 2);
-        p.dq = take((size_t)p.splits * t * p.ldp * 4);
+        p.dq = take((size_t)p.parts * t * p.ldp * 4);
     }
     p.bytes = o;
     return p;
@@ -613,10 +626,9 @@ static mm::NtArgs nt_args(const Plan &p, const void *C, char *ws) {
 
 template <bool F32>
 int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, const int64_t *targets, int64_t c_offset,
-               float scale, float *rest, float *zt, float *loss, float *mean, void *ws, hipStream_t s) {
+               float scale, float *rest, float *zt, float *loss, float *mean, float *share, void *ws, hipStream_t s) {
     const Plan p = make_plan(t, v, d, F32, false);
     char *w = (char *)ws;
-    int32_t *done = (int32_t *)(w + p.done);
     Rows r = {};
     r.t = t;
     r.v = v;
@@ -626,7 +638,6 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
     r.C = C;
     r.d = d;
     r.zt_out = zt;
-    r.done = done;
     r.scale = scale;
     const int rc = prep<F32>(p, Q, C, targets, w, r, (t + 3) / 4, s);
     if (rc != MN_OK) return rc;
@@ -641,9 +652,12 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
     hipLaunchKernelGGL((mm::k_nt<mm::Bf16, StatsEpi>), dim3((unsigned)(a.panels * a.slices)), dim3(mm::NT), 0, s, a, epi);
     MN_KCHECK(s, "k_nt");
     hipLaunchKernelGGL(k_join, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, epi.part, (const float *)nullptr,
-                       (const float *)nullptr, (int64_t)a.slices * 2, t, targets, rest, zt, loss, mean,
-                       mean ? done : (int32_t *)nullptr);
+                       (const float *)nullptr, (int64_t)a.slices * 2, t, targets, rest, zt, loss);
     MN_KCHECK(s, "k_join");
+    if (mean) {
+        hipLaunchKernelGGL(k_mean, dim3(1), dim3(1024), 0, s, loss, targets, t, mean, share);
+        MN_KCHECK(s, "k_mean");
+    }
     return MN_OK;
 }
 
@@ -681,7 +695,8 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
     const char *Cp = p.pack_c ? w + p.c : (const char *)C;
     const int row_tiles = (int)(p.tp / mm::TILE), col_tiles = (d + mm::TILE - 1) / mm::TILE;
     int64_t vn = 0;
-    for (int64_t j0 = 0; j0 < v; j0 += vn) {
+    int piece = 0;
+    for (int64_t j0 = 0; j0 < v; j0 += vn, ++piece) {
         vn = v - j0 <= p.vmax ? v - j0 : p.vc;  // items of this piece
         mm::NtArgs a = nt_args(p, C, w);
         a.B += j0 * a.ldb;
@@ -717,7 +732,8 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         gc.steps_all = gc.steps = (int)((t + 31) / 32);
         const mm::KnGrid nq = {dQ ? col_tiles : 0, row_tiles, p.splits};
         const mm::KnGrid nc = {dC ? col_tiles : 0, (int)((vn + mm::TILE - 1) / mm::TILE), 1};
-        const PartEpi pe = {(float *)(w + p.dq), t, p.ldp, j0 == 0};
+        const PartEpi pe = {(float *)(w + p.dq) + (p.apart ? (int64_t)piece * p.splits * t * p.ldp : 0), t, p.ldp,
+                            p.apart || piece == 0};
         const GradEpi<F32> ge = {(char *)dC + j0 * d * (F32 ? 4 : 2), vn, d, gs};
         hipLaunchKernelGGL((mm::k_kn2<PartEpi, GradEpi<F32>>), dim3((unsigned)(nq.blocks() + nc.blocks())), dim3(mm::NT), 0,
                            s, gq, pe, nq, gc, ge, nc);
@@ -725,7 +741,7 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
     }
     if (dQ) {
         hipLaunchKernelGGL(k_reduce_dq<F32>, dim3((unsigned)((t * (p.ldp / 4) + 255) / 256)), dim3(256), 0, s,
-                           (const float *)(w + p.dq), p.splits, p.ldp, t, d, (const uint16_t *)C, row, at, targets, gs, dQ);
+                           (const float *)(w + p.dq), p.parts, p.ldp, t, d, (const uint16_t *)C, row, at, targets, gs, dQ);
         MN_KCHECK(s, "k_reduce_dq");
     }
     return MN_OK;
@@ -759,46 +775,46 @@ extern "C" int mn_softmax_workspace(int64_t t, int64_t v, int32_t d, int32_t x_t
 
 extern "C" int mn_softmax_stats(const void *Q, const void *C, int32_t x_type, int64_t t, int64_t v, int32_t d,
                                 const int64_t *targets, int64_t c_offset, float scale, float *rest, float *zt,
-                                float *loss, float *mean, void *ws, size_t ws_bytes, void *stream) {
+                                float *loss, float *mean, float *share, void *ws, size_t ws_bytes, void *stream) {
     using namespace mn::sm;
     mn::clear_error();
     const int rc = check_args("mn_softmax_stats", x_type, t, v, d, scale);
     if (rc != MN_OK) return rc;
     MN_REQUIRE(c_offset >= 0, MN_EINVAL, "mn_softmax_stats: c_offset >= 0 needed");
+    MN_REQUIRE(!mean || share, MN_EINVAL, "mn_softmax_stats: mean without share");
     hipStream_t s = (hipStream_t)stream;
     if (t == 0) {
         if (mean) {
-            hipLaunchKernelGGL(k_mean, dim3(1), dim3(1024), 0, s, loss, targets, t, mean);
+            hipLaunchKernelGGL(k_mean, dim3(1), dim3(1024), 0, s, loss, targets, t, mean, share);
             MN_KCHECK(s, "k_mean");
         }
         return MN_OK;
     }
-    MN_REQUIRE(Q && C && targets && rest && zt, MN_EINVAL, "mn_softmax_stats: NULL pointer");
-    MN_REQUIRE(!mean || loss, MN_EINVAL, "mn_softmax_stats: the mean needs loss");
+    MN_REQUIRE(Q && C && targets && rest && zt && loss, MN_EINVAL, "mn_softmax_stats: NULL pointer");
     MN_REQUIRE(aligned16(Q) && aligned16(C), MN_EINVAL, "mn_softmax_stats: Q or C not 16-byte aligned");
     const size_t need = make_plan(t, v, d, x_type == MN_F32, false).bytes;
     MN_REQUIRE(ws && ws_bytes >= need && aligned16(ws), MN_ECAP,
                "mn_softmax_stats: workspace of %zu bytes (16-byte aligned) needed", need);
-    return x_type == MN_F32 ? stats_impl<true>(Q, C, t, v, d, targets, c_offset, scale, rest, zt, loss, mean, ws, s)
-                            : stats_impl<false>(Q, C, t, v, d, targets, c_offset, scale, rest, zt, loss, mean, ws, s);
+    return x_type == MN_F32 ? stats_impl<true>(Q, C, t, v, d, targets, c_offset, scale, rest, zt, loss, mean, share, ws, s)
+                            : stats_impl<false>(Q, C, t, v, d, targets, c_offset, scale, rest, zt, loss, mean, share, ws, s);
 }
 
 extern "C" int mn_softmax_merge(const float *rests, const float *zts, int64_t parts, int64_t t,
                                 const int64_t *targets, float *rest, float *zt, float *loss, float *mean,
-                                void *stream) {
+                                float *share, void *stream) {
     using namespace mn::sm;
     mn::clear_error();
     MN_REQUIRE(parts >= 1 && t >= 0 && t <= (1 << 24), MN_EINVAL, "mn_softmax_merge: parts >= 1, 0 <= t <= 2^24 needed");
-    MN_REQUIRE(t == 0 || (rests && zts && targets && rest && zt), MN_EINVAL, "mn_softmax_merge: NULL pointer");
-    MN_REQUIRE(!mean || loss || t == 0, MN_EINVAL, "mn_softmax_merge: the mean needs loss");
+    MN_REQUIRE(t == 0 || (rests && zts && targets && rest && zt && loss), MN_EINVAL, "mn_softmax_merge: NULL pointer");
+    MN_REQUIRE(!mean || share, MN_EINVAL, "mn_softmax_merge: mean without share");
     hipStream_t s = (hipStream_t)stream;
     if (t > 0) {
         hipLaunchKernelGGL(k_join, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, (const float2 *)nullptr, rests, zts,
-                           parts, t, targets, rest, zt, loss, (float *)nullptr, (int32_t *)nullptr);
+                           parts, t, targets, rest, zt, loss);
         MN_KCHECK(s, "k_join");
     }
     if (mean) {
-        hipLaunchKernelGGL(k_mean, dim3(1), dim3(1024), 0, s, loss, targets, t, mean);
+        hipLaunchKernelGGL(k_mean, dim3(1), dim3(1024), 0, s, loss, targets, t, mean, share);
         MN_KCHECK(s, "k_mean");
     }
     return MN_OK;

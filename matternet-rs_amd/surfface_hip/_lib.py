@@ -169,9 +169,9 @@ SIGNATURES = {
     "mn_scores_i8_workspace": (C.c_int, [I64, I32, C.POINTER(C.c_size_t)]),
     "mn_scores_i8": (C.c_int, [P, I64, P, I64, P, I64, P, I64, I32, P, I32, P, C.c_size_t, P]),
     "mn_softmax_workspace": (C.c_int, [I64, I64, I32, I32, I32, C.POINTER(C.c_size_t)]),
-    "mn_softmax_stats": (C.c_int, [P, P, I32, I64, I64, I32, P, I64, C.c_float, P, P, P, P, P,
+    "mn_softmax_stats": (C.c_int, [P, P, I32, I64, I64, I32, P, I64, C.c_float, P, P, P, P, P, P,
                                    C.c_size_t, P]),
-    "mn_softmax_merge": (C.c_int, [P, P, I64, I64, P, P, P, P, P, P]),
+    "mn_softmax_merge": (C.c_int, [P, P, I64, I64, P, P, P, P, P, P, P]),
     "mn_softmax_backward": (C.c_int, [P, P, I32, I64, I64, I32, P, I64, C.c_float, P, P, P, I64, P,
                                       P, P, P, C.c_size_t, P]),
 }

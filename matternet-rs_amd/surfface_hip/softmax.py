@@ -28,12 +28,13 @@ from .scores import VALUE_TYPES
 @dataclass
 class SoftmaxStats:
     """Per query: rest = log sum exp of the logits but the target's, target =
-    the target's logit (-inf where it is not among the rows), loss.  mean [2] =
-    the mean of loss over the queries that take part, 1 / their number."""
+    the target's logit (-inf where it is not among the rows), loss.  mean = the
+    mean of loss over the queries that take part, share [1] = 1 / their number."""
     rest: torch.Tensor
     target: torch.Tensor
     loss: torch.Tensor
     mean: torch.Tensor
+    share: torch.Tensor
 
 
 def _inputs(Q, items, targets):
@@ -72,9 +73,10 @@ def _workspace(L, n, v, d, kind, backward, device):
 
 
 def _stats_out(n, device):
-    out = torch.empty((3, n), dtype=torch.float32, device=device)
-    mean = torch.empty(2, dtype=torch.float32, device=device)
-    return SoftmaxStats(*out.unbind(), mean), out.data_ptr(), mean.data_ptr()
+    f = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)
+    # tensors of their own: the caller may change loss and mean in place
+    st = SoftmaxStats(f(n), f(n), f(n), f(), f(1))
+    return st, [x.data_ptr() for x in (st.rest, st.target, st.loss, st.mean, st.share)]
 
 
 @on_device
@@ -86,11 +88,11 @@ def softmax_stats(queries: torch.Tensor, items: torch.Tensor, targets: torch.Ten
     0.  items holds the rows c_offset .. c_offset + v - 1 of the table; a target
     among none of a table's rows makes its loss +inf."""
     q, c, t, n, v, d, kind = _inputs(queries, items, targets)
-    st, o, mean = _stats_out(n, q.device)
+    st, out = _stats_out(n, q.device)
     L = _lib.lib()
     ws = _workspace(L, n, v, d, kind, 0, q.device)
     _lib.check(L.mn_softmax_stats(q.data_ptr(), c.data_ptr(), kind, n, v, d, t.data_ptr(), c_offset, float(scale),
-                                  o, o + 4 * n, o + 8 * n, mean, ws.data_ptr(), ws.numel(), current_stream()))
+                                  *out, ws.data_ptr(), ws.numel(), current_stream()))
     return st
 
 
@@ -107,9 +109,9 @@ def softmax_merge(rests: torch.Tensor, zts: torch.Tensor, targets: torch.Tensor)
     parts, n = r.shape
     if r.shape != z.shape or n != t.shape[0] or parts < 1:
         raise ValueError(f"rests {tuple(r.shape)}, zts {tuple(z.shape)} and targets {tuple(t.shape)} do not fit")
-    st, o, mean = _stats_out(n, r.device)
-    _lib.check(_lib.lib().mn_softmax_merge(r.data_ptr(), z.data_ptr(), parts, n, t.data_ptr(), o, o + 4 * n,
-                                           o + 8 * n, mean, current_stream()))
+    st, out = _stats_out(n, r.device)
+    _lib.check(_lib.lib().mn_softmax_merge(r.data_ptr(), z.data_ptr(), parts, n, t.data_ptr(), *out,
+                                           current_stream()))
     return st
 
 
@@ -121,13 +123,17 @@ def softmax_backward(queries: torch.Tensor, items: torch.Tensor, targets: torch.
     """(d queries, d items) of sum(grad * loss), from the WHOLE table's rest and
     target (softmax_stats, or softmax_merge where items is a row range: then d
     queries is the range's part, to be added up).  grad: f32, one value per
-    query or one for all; grad_scale: one f32 that multiplies it (mean[1] for
+    query or one for all; grad_scale: one f32 that multiplies it (share for
     the mean).  need: which of the two to compute (None for the other)."""
     q, c, t, n, v, d, kind = _inputs(queries, items, targets)
     re = _values(rest, "rest", q.device, n)
     zt = _values(target, "target", q.device, n)
     g = _values(grad, "grad", q.device, 1, n)
     gs = None if grad_scale is None else _values(grad_scale, "grad_scale", q.device, 1)
+    return _backward(q, c, t, n, v, d, kind, re, zt, g, scale, c_offset, gs, need)
+
+
+def _backward(q, c, t, n, v, d, kind, re, zt, g, scale, c_offset, gs, need):
     dq = torch.empty_like(q) if need[0] else None
     dc = torch.empty_like(c) if need[1] else None
     if n == 0:
@@ -148,18 +154,18 @@ class _SoftmaxLoss(torch.autograd.Function):
     def forward(ctx, queries, items, targets, scale, reduction):
         st = softmax_stats(queries, items, targets, scale)
         ctx.save_for_backward(queries, items, targets)
-        ctx.stats, ctx.scale, ctx.mean = st, scale, reduction == "mean"
-        # the returned value shares no storage with what backward reads: the
-        # caller may change it in place
-        return (st.mean[0] if reduction == "mean" else st.loss if reduction == "none" else st.loss.sum()).clone()
+        # not the loss and the mean, which the caller may change in place
+        ctx.of = (st.rest, st.target, st.share if reduction == "mean" else None, scale)
+        return st.mean if reduction == "mean" else st.loss if reduction == "none" else st.loss.sum()
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         queries, items, targets = ctx.saved_tensors
-        st = ctx.stats
-        dq, dc = softmax_backward(queries, items, targets, st.rest, st.target, grad, ctx.scale,
-                                  grad_scale=st.mean[1] if ctx.mean else None, need=ctx.needs_input_grad[:2])
+        rest, target, share, scale = ctx.of
+        # on the forward's device: its tensors passed softmax_stats' checks
+        dq, dc = _backward(*_inputs(queries, items, targets), rest, target, grad.reshape(-1).contiguous(), scale, 0,
+                           share, ctx.needs_input_grad[:2])
         return dq, dc, None, None, None
 
 

@@ -56,8 +56,9 @@ def test_softmax_refusals():
         assert L.mn_softmax_workspace(0, 9, 20, 0, bwd, C.byref(need)) == 0 and need.value == 0
     assert L.mn_softmax_workspace(4, 9, 20, 0, 0, None) == E.MN_EINVAL
 
-    def st(Q=A, c=A, ty=0, t=4, v=9, d=20, at=A, off=0, s=1.0, rest=A, zt=A, loss=A, mean=A, ws=A, wb=1 << 30):
-        return L.mn_softmax_stats(Q, c, ty, t, v, d, at, off, s, rest, zt, loss, mean, ws, wb, None)
+    def st(Q=A, c=A, ty=0, t=4, v=9, d=20, at=A, off=0, s=1.0, rest=A, zt=A, loss=A, mean=A, share=A, ws=A,
+           wb=1 << 30):
+        return L.mn_softmax_stats(Q, c, ty, t, v, d, at, off, s, rest, zt, loss, mean, share, ws, wb, None)
 
     def bw(Q=A, c=A, ty=0, t=4, v=9, d=20, at=A, off=0, s=1.0, rest=A, zt=A, g=A, gn=1, gs=A, dq=A, dc=A, ws=A,
            wb=1 << 40):
@@ -71,14 +72,14 @@ def test_softmax_refusals():
         assert f(Q=None) == f(c=None) == f(at=None) == f(rest=None) == f(zt=None) == E.MN_EINVAL
         assert f(Q=ODD) == f(c=ODD) == E.MN_EINVAL
         assert f(ws=None) == f(wb=100) == f(ws=ODD) == E.MN_ECAP
-    assert st(loss=None) == E.MN_EINVAL
+    assert st(loss=None) == st(share=None) == E.MN_EINVAL
     assert bw(gn=3) == bw(g=None) == bw(dq=None, dc=None) == bw(t=0) == E.MN_EINVAL
 
-    def mg(r=A, z=A, p=2, t=4, at=A, rest=A, zt=A, loss=A, mean=A):
-        return L.mn_softmax_merge(r, z, p, t, at, rest, zt, loss, mean, None)
+    def mg(r=A, z=A, p=2, t=4, at=A, rest=A, zt=A, loss=A, mean=A, share=A):
+        return L.mn_softmax_merge(r, z, p, t, at, rest, zt, loss, mean, share, None)
 
     assert mg(p=0) == mg(t=-1) == mg(r=None) == mg(z=None) == mg(at=None) == mg(rest=None) == E.MN_EINVAL
-    assert mg(loss=None) == mg(zt=None) == mg(t=2 ** 24 + 1) == E.MN_EINVAL
+    assert mg(loss=None) == mg(share=None) == mg(zt=None) == mg(t=2 ** 24 + 1) == E.MN_EINVAL
 
 
 def test_python_refuses_host_tensors():

@@ -213,17 +213,17 @@ def test_row_ranges_of_a_table_join(dtype):
     parts = [S.softmax_stats(qd, cd[a:b], ad, 6.0, c_offset=a) for a, b in zip(cut, cut[1:])]
     st = S.softmax_merge(torch.stack([p.rest for p in parts]), torch.stack([p.target for p in parts]), ad)
     one = torch.ones(1).cuda()
-    got = [S.softmax_backward(qd, cd[a:b], ad, st.rest, st.target, one, 6.0, c_offset=a, grad_scale=st.mean[1])
+    got = [S.softmax_backward(qd, cd[a:b], ad, st.rest, st.target, one, 6.0, c_offset=a, grad_scale=st.share)
            for a, b in zip(cut, cut[1:])]
     dq = sum(g[0].double() for g in got).cpu()
     dc = torch.cat([g[1] for g in got])
-    check_step(q, c, at, 6.0, dtype, st.mean[0], None, dc, mean=True)
+    check_step(q, c, at, 6.0, dtype, st.mean, None, dc, mean=True)
     w = formula(q, c, at, 6.0)
     b = B if dtype == torch.bfloat16 else 0.0
     close(dq, w[1], (2 * w[5] + 3000 * U + b + 3 * (b or U)) * w[3] + 1e-40, "dq")
-    only = S.softmax_backward(qd, cd, ad, st.rest, st.target, one, 6.0, grad_scale=st.mean[1], need=(False, True))
+    only = S.softmax_backward(qd, cd, ad, st.rest, st.target, one, 6.0, grad_scale=st.share, need=(False, True))
     assert only[0] is None and torch.equal(only[1], S.softmax_backward(
-        qd, cd, ad, st.rest, st.target, one, 6.0, grad_scale=st.mean[1])[1])
+        qd, cd, ad, st.rest, st.target, one, 6.0, grad_scale=st.share)[1])
 
 
 def test_same_target_many_times_and_int32_targets():
@@ -248,12 +248,12 @@ def test_views_streams_and_repeats():
     for qq, cc in ((q.cuda(), c.cuda()), (more[1:], wide[:, 11:41]), (q.cuda(), c.cuda())):
         st = S.softmax_stats(qq, cc, at.cuda(), 9.0)
         runs.append([st.loss, st.mean, *S.softmax_backward(qq, cc, at.cuda(), st.rest, st.target,
-                                                           torch.ones(1).cuda(), 9.0, grad_scale=st.mean[1])])
+                                                           torch.ones(1).cuda(), 9.0, grad_scale=st.share)])
     s = torch.cuda.Stream()
     qd, cd, ad, one = q.cuda(), c.cuda(), at.cuda(), torch.ones(1).cuda()
     s.wait_stream(torch.cuda.current_stream())
     st = S.softmax_stats(qd, cd, ad, 9.0, stream=s)
-    dq, dc = S.softmax_backward(qd, cd, ad, st.rest, st.target, one, 9.0, grad_scale=st.mean[1], stream=s)
+    dq, dc = S.softmax_backward(qd, cd, ad, st.rest, st.target, one, 9.0, grad_scale=st.share, stream=s)
     torch.cuda.current_stream().wait_stream(s)
     runs.append([st.loss, st.mean, dq, dc])
     for r in runs[1:]:
@@ -270,7 +270,7 @@ def test_captured_steps(dtype):
 
     def step(x, a):
         st = S.softmax_stats(x, cd, a, 8.0)
-        return [st.mean, *S.softmax_backward(x, cd, a, st.rest, st.target, one, 8.0, grad_scale=st.mean[1])]
+        return [st.mean, *S.softmax_backward(x, cd, a, st.rest, st.target, one, 8.0, grad_scale=st.share)]
 
     step(q.cuda(), at.cuda())
     graphs = []
