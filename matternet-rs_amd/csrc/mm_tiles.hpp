@@ -3,6 +3,7 @@
 //
 //   k_nt   Y[i][j] = sum_k A[i][k] B[j][k]   (rows against rows): a block keeps
 //          256 rows of A and goes through a run of 256-row tiles of B
+//   k_few  the same for up to 64 rows of A
 //   k_kn2  Y[m][n] = sum_k A(m,k) B[k][n]    (A [m][k] or [k][m]): one 256 x 256
 //          tile and run of k a block, two such products in a launch
 // with f32 (bf16 operands) or int32 (int8 operands) sums; an epilogue object
@@ -14,7 +15,7 @@
 // 2^-25 of |x||y|, the rounding of one f32 product.  The small ones are added
 // first.  Six products at the bf16 rate are 2.7 times the f32 matrix rate.
 //
-// Schedule (both kernels).  Eight waves, each 64 (i, m) x 128 (j, n) = 4 x 8
+// Schedule (k_nt, k_kn2).  Eight waves, each 64 (i, m) x 128 (j, n) = 4 x 8
 // tiles of 16 x 16: 128 accumulator registers.  A k-step is 64 bytes of k (32
 // bf16, 64 int8) of both operands, 32 KB, in a ring of four slots, filled three
 // steps ahead by loads that go to LDS directly.  Waves w and w + 4 share a SIMD
@@ -34,6 +35,8 @@
 // l of the four rows); the 32-byte slot of 16 columns s of row k is at s ^
 // ((k & 3) | ((k >> 3) & 1) << 2).
 #pragma once
+#include <algorithm>
+
 #include "common.hpp"
 
 namespace mn {
@@ -68,6 +71,17 @@ struct Int8 {
     static __device__ __forceinline__ acc_t mma(u32x4 a, u32x4 b, acc_t c) {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
                                                      __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+    }
+};
+
+// f32 operands as they are: 16 bytes are four k's of one product each
+struct F32 {
+    typedef f32x4 acc_t;
+    static __device__ __forceinline__ acc_t mma(u32x4 a, u32x4 b, acc_t c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+        return c;
     }
 };
 
@@ -163,8 +177,9 @@ inline void plan_runs(NtArgs &a) {
 }
 
 // Epilogue: init (before the loop), fetch (a tile's loads to LDS; FETCH: there
-// are any), tile (a tile's accumulators; at least STORES store instructions of
-// each wave, whatever the data), finish.
+// are any), tile (a tile's accumulators; stage: STAGE bytes of LDS of the
+// wave's own; with `counted` set it issued at least STORES store instructions),
+// finish.
 // accumulator r of tile (f, g): row i = 16 f + (lane & 15) of the wave's 64,
 // column j = 32 (g >> 1) + 8 (lane >> 4) + 4 (g & 1) + r of its 128, so that a
 // lane holds 8 neighbours of a row in each pair of tiles
@@ -172,6 +187,8 @@ template <class OP, class EPI>
 __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     __shared__ Ring rg;
     __shared__ typename EPI::Shared sh;
+    // waves w and w + 4 write their tiles out in different windows
+    __shared__ alignas(16) char stage_[EPI::STAGE ? 4 * EPI::STAGE : 16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = w & 3, wj = w >> 2;
@@ -236,6 +253,7 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     u32x4 fi[4], fj[8];
     const char *ri = &rg.b[0][0][(64 * wi + fr) * KBY + 16 * (fk ^ (((fr >> 3) & 1) << 1))];
     // row of fragment g: 32 (g >> 1) + 4 (g & 1) + 8 (fr >> 2) + (fr & 3)
+    char *stage = stage_ + wi * EPI::STAGE;
     const char *rj = &rg.b[0][1][(128 * wj + 8 * (fr >> 2) + (fr & 3)) * KBY + 16 * (fk ^ (((fr >> 3) & 1) << 1))];
     epi.init(sh, i0 + 64 * wi, lane);
     issue();
@@ -246,9 +264,10 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     if (wj) window_end();
     int k = 0, t = t0;
     const int per = a.nk * a.nseg;
-    for (int n = 0; n < nstep; ++n) {
+    for (int n = 0;; ++n) {
         if (k == 0) {
-            if (n) epi.tile(sh, acc, (int64_t)(t - 1) * TILE + 128 * wj, lane, (t - 1) & 1);
+            if (n) epi.tile(sh, stage, acc, (int64_t)(t - 1) * TILE + 128 * wj, lane, (t - 1) & 1);
+            if (n == nstep) break;
             epi.fetch(sh, (int64_t)t * TILE, tid, t & 1);
 #pragma unroll
             for (int f = 0; f < 4; ++f)
@@ -265,7 +284,7 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
         if (EPI::FETCH && per < 4) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         // a tile's stores come between the loads of the next two steps and
         // those of the third: they have two steps to drain
-        if (EPI::STORES > 0 && k < 2 && n >= per) read_window_end<(8 + EPI::STORES < 63 ? 8 + EPI::STORES : 63)>();
+        if (EPI::STORES > 0 && k < 2 && n >= per && epi.counted) read_window_end<(8 + EPI::STORES < 63 ? 8 + EPI::STORES : 63)>();
         else read_window_end<8>();
 #pragma unroll
         for (int f = 0; f < 4; ++f)
@@ -277,10 +296,104 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
             ++t;
         }
     }
-    if (!wj) window_end();
+    if (!wj) window_end();  // the other half's last products, then its last tile
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    epi.tile(sh, acc, (int64_t)(t1 - 1) * TILE + 128 * wj, lane, (t1 - 1) & 1);
     epi.finish(sh, i0 + 64 * wi, slice * 2 + wj, lane);
+}
+
+// Up to 64 queries against many rows: as many bytes of B as possible in flight
+// is all that counts.  The queries lie in LDS ([k-step][query][64 bytes], pieces
+// at c ^ 2 ((query >> 3) & 1): no bank conflicts), a wave takes 16 rows of B at
+// a time from memory to registers, four k-steps of loads ahead of their
+// products, and the block's waves go through B side by side.
+struct FewArgs {
+    const char *Q, *B;
+    int64_t ldq, ldb;  // bytes, multiples of 16
+    int64_t n;         // rows of B
+    int m;             // queries
+    int qbytes;        // bytes of a query's row that count (zeros behind)
+    int nk, bmax, blocks;
+    bool small;        // queries take at most FEW_SMALL bytes of LDS
+};
+constexpr int FEW_SMALL = 40 << 10, FEW_LARGE = 144 << 10;
+
+// false: the queries do not fit LDS
+inline bool plan_few(FewArgs &a) {
+    a.nk = (a.qbytes + KBY - 1) / KBY;
+    a.bmax = (a.qbytes + 15) / 16 * 16 - 16;
+    const int64_t mf = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4, bytes = mf * 16 * a.nk * KBY;
+    a.small = bytes <= FEW_SMALL;
+    if (bytes > FEW_LARGE) return false;
+    const int64_t groups = (a.n + 15) / 16;
+    a.blocks = (int)std::min<int64_t>((groups + 7) / 8, a.small ? 768 : 256);
+    return true;
+}
+
+template <class OP, int MF, int LDSB, class EPI>
+__global__ __launch_bounds__(NT) void k_few(FewArgs a, EPI epi) {
+    __shared__ alignas(16) char qs[LDSB];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int fr = lane & 15, fk = lane >> 4;
+    for (int p = tid; p < 64 * MF * a.nk; p += NT) {
+        const int c = p & 3, r = (p >> 2) % (16 * MF), kc = (p >> 2) / (16 * MF);
+        const int byte = kc * KBY + 16 * c;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < a.m && byte < a.qbytes && epi.takes(r)) {
+            x = *reinterpret_cast<const uint4 *>(a.Q + r * a.ldq + byte);
+            const int left = a.qbytes - byte;  // bytes of the piece that count
+            if (left < 16) {
+                uint32_t *q = &x.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int keep = left - 4 * e;
+                    q[e] = keep >= 4 ? q[e] : keep <= 0 ? 0u : q[e] & ((1u << (8 * keep)) - 1u);
+                }
+            }
+        }
+        *reinterpret_cast<uint4 *>(qs + (p >> 2) * KBY + 16 * (c ^ (((r >> 3) & 1) << 1))) = x;
+    }
+    epi.init(lane);
+    __syncthreads();
+    const char *qr = qs + fr * KBY + 16 * (fk ^ (((fr >> 3) & 1) << 1));
+    const int64_t groups = (a.n + 15) / 16;
+    for (int64_t g = (int64_t)blockIdx.x * (NT / 64) + w; g < groups; g += (int64_t)gridDim.x * (NT / 64)) {
+        const char *row = a.B + min(16 * g + fr, a.n - 1) * a.ldb;
+        typename OP::acc_t acc[MF];
+#pragma unroll
+        for (int f = 0; f < MF; ++f) acc[f] = (typename OP::acc_t)(0);
+        constexpr int U = 4;
+        u32x4 b[2][U];
+        auto load = [&](u32x4 (&x)[U], int kc) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                x[u] = *reinterpret_cast<const u32x4 *>(row + min((kc + u) * KBY + 16 * fk, a.bmax));
+        };
+        auto use = [&](u32x4 (&x)[U], int kc) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (kc + u >= a.nk) break;
+#pragma unroll
+                for (int f = 0; f < MF; ++f)
+                    acc[f] = OP::mma(x[u], *reinterpret_cast<const u32x4 *>(qr + ((kc + u) * MF + f) * 16 * KBY), acc[f]);
+            }
+        };
+        load(b[0], 0);
+        for (int kc = 0; kc < a.nk; kc += 2 * U) {
+            if (kc + U < a.nk) load(b[1], kc + U);
+            use(b[0], kc);
+            if (kc + U >= a.nk) break;
+            if (kc + 2 * U < a.nk) load(b[0], kc + 2 * U);
+            use(b[1], kc + U);
+        }
+        epi.group(acc, 16 * g, lane);
+    }
+    epi.finish(qs, tid);
+}
+
+template <class OP, int MF, class EPI>
+void launch_few(const FewArgs &a, const EPI &epi, hipStream_t s) {
+    if (a.small) hipLaunchKernelGGL((k_few<OP, MF, FEW_SMALL, EPI>), dim3(a.blocks), dim3(NT), 0, s, a, epi);
+    else hipLaunchKernelGGL((k_few<OP, MF, FEW_LARGE, EPI>), dim3(a.blocks), dim3(NT), 0, s, a, epi);
 }
 
 struct KnArgs {

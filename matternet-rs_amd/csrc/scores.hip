@@ -162,12 +162,13 @@ struct ScoreEpi {
         float cs[2][mm::TILE];  // the items' scales of a tile, two tiles in turn
     };
     static constexpr bool FETCH = true;
-    static constexpr int STORES = 0;  // rows and columns past the end store nothing
+    static constexpr int STORES = 4 * sizeof(T) * 2, STAGE = 16 * 272;
     const float *qs, *cs;
     T *Y;
     int64_t m, n;
     float q[4];
     int64_t i0_;
+    bool counted;
     __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
         i0_ = i0;
 #pragma unroll
@@ -178,45 +179,87 @@ struct ScoreEpi {
         if (w < 4)
             mm::dma4((const char *)(cs + j0), 4 * (int)min<int64_t>(tid, n - 1 - j0), mm::lds_addr(&sh.cs[par][64 * w]));
     }
-    __device__ __forceinline__ void tile(Shared &sh, mm::i32x4 (&acc)[4][8], int64_t j0, int lane, int par) {
+    // 16 rows by 256 bytes at a time through LDS (272 bytes a row), so that a
+    // store of the wave is 256 bytes of each of four rows; rows of Y on 16-byte
+    // borders or not (a store may start anywhere)
+    __device__ __forceinline__ void tile(Shared &sh, char *stage, mm::i32x4 (&acc)[4][8], int64_t j0, int lane, int par) {
+        constexpr int E = 16 / sizeof(T), PASS = sizeof(T) / 2;  // values of a piece; passes of 128 / PASS columns
         const int jl = 8 * (lane >> 4);
+        const bool inside = i0_ + 64 <= m && j0 + 128 <= n;
+        counted = inside;
+        const float *c = &sh.cs[par][(int)(j0 & (mm::TILE - 1)) + jl];
+        char *put = stage + (lane & 15) * 272 + jl * (int)sizeof(T);
+        const char *get = stage + (lane >> 4) * 272 + 16 * (lane & 15);
+        const int64_t row = i0_ + (lane >> 4), col = j0 + E * (lane & 15);
+        T *to = Y + row * n + col;
 #pragma unroll
-        for (int g = 0; g < 8; g += 2) {
-            const int64_t j = j0 + jl + 16 * g;
-            float c[8];
+        for (int f = 0; f < 4; ++f)
 #pragma unroll
-            for (int q8 = 0; q8 < 8; ++q8) c[q8] = sh.cs[par][(int)(j0 & (mm::TILE - 1)) + jl + 16 * g + q8];
+            for (int p = 0; p < PASS; ++p) {
 #pragma unroll
-            for (int f = 0; f < 4; ++f) {
-                const int64_t i = i0_ + 16 * f + (lane & 15);
-                float x[8];
+                for (int g2 = 0; g2 < 4 / PASS; ++g2) {
+                    const int g = 2 * (g2 + p * (4 / PASS));
+                    float x[8];
 #pragma unroll
-                for (int q8 = 0; q8 < 8; ++q8) x[q8] = (float)acc[f][g + (q8 >> 2)][q8 & 3] * q[f] * c[q8];
-                if (i >= m) continue;
-                T *p = Y + i * n + j;
-                if constexpr (sizeof(T) == 4) {
-                    if (j + 8 <= n) {
-                        __builtin_memcpy(p, x, 32);
+                    for (int e = 0; e < 8; ++e) x[e] = (float)acc[f][g + (e >> 2)][e & 3] * q[f] * c[16 * g + e];
+                    uint4 *o = reinterpret_cast<uint4 *>(put + 32 * g2 * sizeof(T));
+                    if constexpr (sizeof(T) == 4) {
+                        o[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+                        o[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
                     } else {
-#pragma unroll
-                        for (int q8 = 0; q8 < 8; ++q8)
-                            if (j + q8 < n) p[q8] = x[q8];
+                        o[0] = make_uint4(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]),
+                                          mm::bf16_pair(x[4], x[5]), mm::bf16_pair(x[6], x[7]));
                     }
-                } else {
-                    if (j + 8 <= n) {
-                        const uint4 y = make_uint4(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]),
-                                                   mm::bf16_pair(x[4], x[5]), mm::bf16_pair(x[6], x[7]));
-                        __builtin_memcpy(p, &y, 16);
-                    } else {
+                }
 #pragma unroll
-                        for (int q8 = 0; q8 < 8; ++q8)
-                            if (j + q8 < n) p[q8] = mm::bf16_bits(x[q8]);
+                for (int u = 0; u < 4; ++u) {
+                    const uint4 y = *reinterpret_cast<const uint4 *>(get + 4 * u * 272);
+                    T *dst = to + (int64_t)(16 * f + 4 * u) * n + p * (128 / PASS);
+                    if (inside) {
+                        __builtin_memcpy(dst, &y, 16);
+                    } else if (row + 16 * f + 4 * u < m) {
+                        const int64_t left = n - col - p * (128 / PASS);
+                        T e[E];
+                        __builtin_memcpy(e, &y, 16);
+#pragma unroll
+                        for (int k = 0; k < E; ++k)
+                            if (k < left) dst[k] = e[k];
                     }
                 }
             }
-        }
     }
     __device__ __forceinline__ void finish(Shared &, int64_t, int, int) {}
+};
+
+// As ScoreEpi, for mm::k_few
+template <typename T, int MF>
+struct FewScoreEpi {
+    const float *qs, *cs;
+    T *Y;
+    int64_t n;
+    int m;
+    float q[MF];
+    __device__ __forceinline__ bool takes(int) const { return true; }
+    __device__ __forceinline__ void init(int lane) {
+#pragma unroll
+        for (int f = 0; f < MF; ++f) q[f] = qs[min(16 * f + (lane & 15), m - 1)];
+    }
+    __device__ __forceinline__ void group(mm::i32x4 (&acc)[MF], int64_t j0, int lane) {
+        const int64_t j = j0 + 4 * (lane >> 4);
+        float c[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] = cs[min(j + r, n - 1)];
+#pragma unroll
+        for (int f = 0; f < MF; ++f) {
+            const int i = 16 * f + (lane & 15);
+            if (i >= m || j >= n) continue;
+            mm::f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = (float)acc[f][r] * q[f] * c[r];
+            mm::store4<sizeof(T) == 4>(Y, i * n + j, (int)min<int64_t>(4, n - j), x);
+        }
+    }
+    __device__ __forceinline__ void finish(char *, int) {}
 };
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -239,6 +282,17 @@ void quantize(const T *X, int64_t n, int d, int8_t *codes, int64_t ld, float *sc
 }
 
 inline int padded(int d) { return (d + mm::KBY - 1) / mm::KBY * mm::KBY; }
+
+// up to 64 queries of up to 144 KB go to k_few, which needs none
+inline bool few_args(mm::FewArgs &a, int64_t m, int d) {
+    a.m = (int)std::min<int64_t>(m, 65);
+    a.qbytes = d;
+    return m <= 64 && mm::plan_few(a);
+}
+inline size_t workspace(int64_t m, int d) {
+    mm::FewArgs few = {};
+    return d % mm::KBY == 0 || few_args(few, m, d) ? 0 : (size_t)m * padded(d);
+}
 
 }  // namespace i8
 }  // namespace mn
@@ -290,7 +344,7 @@ extern "C" int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const floa
 extern "C" int mn_scores_i8_workspace(int64_t m, int32_t d, size_t *bytes) {
     mn::clear_error();
     MN_REQUIRE(bytes && m >= 0 && d >= 1 && d <= 131071, MN_EINVAL, "mn_scores_i8_workspace: bad args");
-    *bytes = d % mn::mm::KBY == 0 ? 0 : (size_t)m * mn::i8::padded(d);
+    *bytes = mn::i8::workspace(m, d);
     return MN_OK;
 }
 
@@ -311,10 +365,37 @@ extern "C" int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, 
     MN_REQUIRE(Q && q_scale && C && c_scale && Y, MN_EINVAL, "mn_scores_i8: NULL pointer");
     MN_REQUIRE(aligned16(Q) && aligned16(C), MN_EINVAL, "mn_scores_i8: codes not 16-byte aligned");
     const int ldp = padded(d);
-    const size_t need = d % mm::KBY == 0 ? 0 : (size_t)m * ldp;
+    hipStream_t s = (hipStream_t)stream;
+    mm::FewArgs few = {};
+    few.Q = (const char *)Q;
+    few.B = (const char *)C;
+    few.ldq = ldq;
+    few.ldb = ldc;
+    few.n = n;
+    if (few_args(few, m, d)) {
+        auto go = [&](auto out, auto MF) {
+            typedef decltype(out) T;
+            FewScoreEpi<T, decltype(MF)::value> epi = {};
+            epi.qs = q_scale;
+            epi.cs = c_scale;
+            epi.Y = (T *)Y;
+            epi.n = n;
+            epi.m = (int)m;
+            mm::launch_few<mm::Int8, decltype(MF)::value>(few, epi, s);
+        };
+        auto size = [&](auto out) {
+            if (m <= 16) go(out, std::integral_constant<int, 1>());
+            else if (m <= 32) go(out, std::integral_constant<int, 2>());
+            else go(out, std::integral_constant<int, 4>());
+        };
+        if (y_type == MN_F32) size(float());
+        else size(uint16_t());
+        MN_KCHECK(s, "k_few");
+        return MN_OK;
+    }
+    const size_t need = workspace(m, d);
     MN_REQUIRE(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), MN_ECAP,
                "mn_scores_i8: workspace of %zu bytes (16-byte aligned) needed", need);
-    hipStream_t s = (hipStream_t)stream;
     const int8_t *A = Q;
     int64_t lda = ldq;
     if (need) {

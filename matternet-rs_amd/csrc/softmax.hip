@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 #include "mm_tiles.hpp"
@@ -98,6 +99,72 @@ __device__ __forceinline__ void pack(const Pack &p, int block) {
         }
     }
 }
+
+// As StatsEpi, for k_few: 16 items at a time, MF groups of 16 queries.
+template <int MF>
+struct FewStatsEpi {
+    float2 *part;  // [blocks][t]
+    const int64_t *targets;
+    int64_t c_offset, v;
+    int t;
+    float scale2;
+    int at[MF];
+    float m2[MF], sum[MF];
+    __device__ __forceinline__ bool takes(int i) const { return targets[i] >= 0; }
+    __device__ __forceinline__ void init(int lane) {
+#pragma unroll
+        for (int f = 0; f < MF; ++f) {
+            const int i = 16 * f + (lane & 15);
+            const int64_t x = i < t ? targets[i] : -1;
+            at[f] = x >= c_offset && x - c_offset < v ? (int)(x - c_offset) : -1;
+            m2[f] = -__builtin_inff();
+            sum[f] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void group(mm::f32x4 (&acc)[MF], int64_t j0, int lane) {
+        const int j = (int)j0 + 4 * (lane >> 4);
+#pragma unroll
+        for (int f = 0; f < MF; ++f) {
+            float z[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[r] = j + r >= v || j + r == at[f] ? -__builtin_inff() : acc[f][r];
+            const float m = fmaxf(m2[f], fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])) * scale2);
+            const float mz = m == -__builtin_inff() ? 0.f : m;
+            float s = 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[r], scale2, -mz));
+            sum[f] = sum[f] * __builtin_amdgcn_exp2f(m2[f] - mz) + s;
+            m2[f] = m;
+        }
+    }
+    // joined over the lanes, then over the block's waves
+    __device__ __forceinline__ void finish(char *lds, int tid) {
+        float2 *sh = reinterpret_cast<float2 *>(lds);
+        const int lane = tid & 63, w = tid >> 6;
+        auto join = [](float &m, float &s, float mo, float so) {
+            const float x = fmaxf(m, mo), z = x == -__builtin_inff() ? 0.f : x;
+            s = s * __builtin_amdgcn_exp2f(m - z) + so * __builtin_amdgcn_exp2f(mo - z);
+            m = x;
+        };
+        __syncthreads();
+#pragma unroll
+        for (int f = 0; f < MF; ++f) {
+#pragma unroll
+            for (int o = 16; o <= 32; o <<= 1) {
+                const float mo = __shfl_xor(m2[f], o), so = __shfl_xor(sum[f], o);
+                join(m2[f], sum[f], mo, so);
+            }
+            if (lane < 16) sh[w * 16 * MF + 16 * f + lane] = make_float2(m2[f], sum[f]);
+        }
+        __syncthreads();
+        if (tid < t) {
+            float2 x = sh[tid];
+#pragma unroll
+            for (int k = 1; k < mm::NT / 64; ++k) join(x.x, x.y, sh[k * 16 * MF + tid].x, sh[k * 16 * MF + tid].y);
+            part[(int64_t)blockIdx.x * t + tid] = x;
+        }
+    }
+};
 
 __device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
 
@@ -185,7 +252,8 @@ __global__ __launch_bounds__(256) void k_prep(Pack q, Pack c, Rows r) {
 struct StatsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;
-    static constexpr int STORES = 0;
+    static constexpr int STORES = 0, STAGE = 0;
+    static constexpr bool counted = false;
     float2 *part;
     const int64_t *targets;
     int64_t c_offset, t;
@@ -205,7 +273,7 @@ struct StatsEpi {
         }
     }
     __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
-    __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][8], int64_t j0, int lane, int) {
+    __device__ __forceinline__ void tile(Shared &, char *, mm::f32x4 (&acc)[4][8], int64_t j0, int lane, int) {
         const int jw = (int)j0, jl = jw + 8 * (lane >> 4);
         bool hit = jw + 128 > v;
 #pragma unroll
@@ -355,12 +423,16 @@ __global__ __launch_bounds__(1024) void k_grad_max(const float *__restrict__ gra
 }
 
 // D of a piece of the table, [tp][ldd] (three planes for f32 operands); zeros
-// in the rows and columns that only fill tiles.
+// in the rows and columns that only fill tiles.  A store is 64 bytes of each of
+// 16 rows; through LDS, 256 bytes of each of 4 (as the scores', whose row
+// stride is the caller's), it measured slower: 232 against 221 us for 4096 x
+// 32768 x 768.
 template <int PLANES>
 struct DlogitsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;
-    static constexpr int STORES = 16 * PLANES;
+    static constexpr int STORES = 16 * PLANES, STAGE = 0;
+    static constexpr bool counted = true;
     uint16_t *D;
     int64_t ldd, plane;
     int v;  // columns of this piece that exist
@@ -389,14 +461,14 @@ struct DlogitsEpi {
         any = __ballot(any) != 0;
     }
     __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
-    __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][8], int64_t j0, int lane, int) {
+    __device__ __forceinline__ void tile(Shared &, char *, mm::f32x4 (&acc)[4][8], int64_t j0, int lane, int) {
         const int jw = (int)j0, jl = 8 * (lane >> 4);
         bool hit = jw + 128 > v || !any;
 #pragma unroll
         for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 128u;
         const bool slow = __ballot(hit) != 0;
         char *base = (char *)(D + i0_ * ldd + j0);
-        const int lrow = 2 * ((lane & 15) * (int)ldd + jl);
+        const int to = 2 * ((lane & 15) * (int)ldd + jl);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
 #pragma unroll
@@ -409,27 +481,22 @@ struct DlogitsEpi {
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
                         const int j = jw + jl + 16 * g + q;
-                        if (j == at[f]) x[q] = dt[f];
-                        if (j >= v || !any) x[q] = 0.f;
+                        const float y = j == at[f] ? dt[f] : x[q];
+                        x[q] = j >= v || !any ? 0.f : y;
                     }
                 }
-                const int at_byte = lrow + 32 * f * (int)ldd + 32 * g;
-                if constexpr (PLANES == 1) {
-                    mm::store16(base, at_byte, make_uint4(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]),
-                                                          mm::bf16_pair(x[4], x[5]), mm::bf16_pair(x[6], x[7])));
-                } else {
-                    uint32_t o[3][4];
 #pragma unroll
-                    for (int q = 0; q < 8; q += 2) {
-                        uint16_t a[3], b[3];
-                        mm::split3(x[q], a);
-                        mm::split3(x[q + 1], b);
+                for (int s = 0; s < PLANES; ++s) {
+                    uint32_t o[4];
 #pragma unroll
-                        for (int s = 0; s < 3; ++s) o[s][q / 2] = (uint32_t)a[s] | ((uint32_t)b[s] << 16);
+                    for (int q = 0; q < 4; ++q) {
+                        o[q] = mm::bf16_pair(x[2 * q], x[2 * q + 1]);
+                        if (s + 1 < PLANES) {  // what is left for the next plane (|x| <= 1)
+                            x[2 * q] -= mm::bf16_value((uint16_t)o[q]);
+                            x[2 * q + 1] -= mm::bf16_value((uint16_t)(o[q] >> 16));
+                        }
                     }
-#pragma unroll
-                    for (int s = 0; s < 3; ++s)
-                        mm::store16(base + 2 * s * plane, at_byte, make_uint4(o[s][0], o[s][1], o[s][2], o[s][3]));
+                    mm::store16(base + 2 * s * plane, to + 32 * f * (int)ldd + 32 * g, make_uint4(o[0], o[1], o[2], o[3]));
                 }
             }
         }
@@ -520,6 +587,9 @@ struct Plan {
     int d, kp, ldp, planes;
     bool pack_c;
     mm::NtArgs nt;      // the whole table's logits
+    mm::FewArgs few;    // the same for few queries; blocks 0: not so
+    bool few_packed;    // on packed operands
+    int64_t ldd;        // row stride of D
     int64_t vc, vmax;   // items per piece (backward), of the longest piece, in whole tiles
     int splits;         // of dQ's sum over a piece
     int pieces, parts;  // of the table; partial sums of dQ in all
@@ -548,13 +618,31 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += up(b); return at; };
     p.q = take((size_t)p.planes * t * p.kp * 2);
-    p.c = take(p.pack_c ? (size_t)p.planes * v * p.kp * 2 : 0);
+    const size_t packed = (size_t)p.planes * v * p.kp * 2;
     if (!backward) {
+        // few queries: items straight to registers (f32: as they are)
+        p.few = {};
+        p.few.m = (int)t;
+        p.few.n = v;
+        if (f32) {
+            p.few.ldq = p.few.ldb = p.few.qbytes = 4 * d;
+            if (t > 32 || d % 4) p.few.n = 0;
+        } else {
+            p.few.ldq = p.few.ldb = p.few.qbytes = 2 * (d % 8 ? p.kp : d);
+        }
+        if (t > 64 || p.few.n == 0 || !mm::plan_few(p.few)) p.few.blocks = 0;
+        else p.pack_c = !f32 && d % 8 != 0;
+        p.few_packed = p.few.blocks && p.pack_c;
+        p.c = take(p.pack_c ? packed : 0);
         mm::plan_runs(p.nt);
-        p.part = take((size_t)p.nt.slices * 2 * t * 8);
+        p.part = take((size_t)std::max(p.nt.slices * 2, p.few.blocks) * t * 8);
     } else {
-        // Pieces whose D stays below 256 MB and whose tiles fill whole rounds
-        // of 256 blocks; a short rest joins the last piece where it fits.
+        p.c = take(p.pack_c ? packed : 0);
+        // Pieces whose D stays below 256 MB (the last-level cache; 128, 512 and
+        // 1024 MB take 3.22, 3.05 and 3.06 ms for 4096 x 131072 x 768, 256 MB
+        // 3.05, and 3.73, 3.70 and 3.73 ms for 1024 x 100000 x 768 in f32, 256
+        // MB 3.55) and whose tiles fill whole rounds of 256 blocks; a short
+        // rest joins the last piece where it fits.
         const int64_t all = (v + mm::TILE - 1) / mm::TILE, panels = p.tp / mm::TILE;
         const int64_t most = std::max<int64_t>(1, std::min<int64_t>(4096, ((int64_t)256 << 20) / (p.tp * mm::TILE * 2 * p.planes)));
         const int64_t unit = std::max<int64_t>(1, 256 / panels);
@@ -596,7 +684,8 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         p.row = take(sizeof(Row) * p.tp);
         p.at = take(4 * p.tp);
         p.gs = take(8);
-        p.D = take((size_t)p.planes * p.tp * p.vmax * 2);
+        p.ldd = p.vmax + 64;  // an odd number of 128-byte lines: rows on different memory channels
+        p.D = take((size_t)p.planes * p.tp * p.ldd * 2);
         p.dq = take((size_t)p.parts * t * p.ldp * 4);
     }
     p.bytes = o;
@@ -611,7 +700,7 @@ int prep(const Plan &p, const void *Q, const void *C, const int64_t *targets, ch
         k.blocks = (int)((n * (p.kp / 8) + 256 * kPackPer - 1) / (256 * kPackPer));
         return k;
     };
-    const Pack q = one(Q, p.q, p.t, targets), c = p.pack_c ? one(C, p.c, p.v, nullptr) : Pack{};
+    const Pack q = p.few.blocks && !p.few_packed ? Pack{} : one(Q, p.q, p.t, targets), c = p.pack_c ? one(C, p.c, p.v, nullptr) : Pack{};
     hipLaunchKernelGGL(k_prep<F32>, dim3((unsigned)(q.blocks + c.blocks + row_blocks)), dim3(256), 0, s, q, c, r);
     MN_KCHECK(s, "k_prep");
     return MN_OK;
@@ -641,18 +730,43 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
     r.scale = scale;
     const int rc = prep<F32>(p, Q, C, targets, w, r, (t + 3) / 4, s);
     if (rc != MN_OK) return rc;
-    const mm::NtArgs a = nt_args(p, C, w);
-    StatsEpi epi = {};
-    epi.part = (float2 *)(w + p.part);
-    epi.targets = targets;
-    epi.c_offset = c_offset;
-    epi.t = t;
-    epi.v = (int)v;
-    epi.scale2 = scale * kLog2e;
-    hipLaunchKernelGGL((mm::k_nt<mm::Bf16, StatsEpi>), dim3((unsigned)(a.panels * a.slices)), dim3(mm::NT), 0, s, a, epi);
-    MN_KCHECK(s, "k_nt");
-    hipLaunchKernelGGL(k_join, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, epi.part, (const float *)nullptr,
-                       (const float *)nullptr, (int64_t)a.slices * 2, t, targets, rest, zt, loss);
+    float2 *part = (float2 *)(w + p.part);
+    int64_t pieces;
+    if (p.few.blocks) {
+        mm::FewArgs a = p.few;
+        a.Q = p.few_packed ? w + p.q : (const char *)Q;
+        a.B = p.few_packed ? w + p.c : (const char *)C;
+        pieces = a.blocks;
+        auto go = [&](auto MF) {
+            FewStatsEpi<decltype(MF)::value> epi = {};
+            epi.part = part;
+            epi.targets = targets;
+            epi.c_offset = c_offset;
+            epi.v = v;
+            epi.t = (int)t;
+            epi.scale2 = scale * kLog2e;
+            mm::launch_few<std::conditional_t<F32, mm::F32, mm::Bf16>, decltype(MF)::value>(a, epi, s);
+        };
+        if (t <= 16) go(std::integral_constant<int, 1>());
+        else if (t <= 32) go(std::integral_constant<int, 2>());
+        else if constexpr (!F32) go(std::integral_constant<int, 4>());
+        MN_KCHECK(s, "k_few");
+    } else {
+        const mm::NtArgs a = nt_args(p, C, w);
+        pieces = (int64_t)a.slices * 2;
+        StatsEpi epi = {};
+        epi.part = part;
+        epi.targets = targets;
+        epi.c_offset = c_offset;
+        epi.t = t;
+        epi.v = (int)v;
+        epi.scale2 = scale * kLog2e;
+        hipLaunchKernelGGL((mm::k_nt<mm::Bf16, StatsEpi>), dim3((unsigned)(a.panels * a.slices)), dim3(mm::NT), 0, s, a,
+                           epi);
+        MN_KCHECK(s, "k_nt");
+    }
+    hipLaunchKernelGGL(k_join, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, part, (const float *)nullptr,
+                       (const float *)nullptr, pieces, t, targets, rest, zt, loss);
     MN_KCHECK(s, "k_join");
     if (mean) {
         hipLaunchKernelGGL(k_mean, dim3(1), dim3(1024), 0, s, loss, targets, t, mean, share);
@@ -704,8 +818,8 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         mm::plan_runs(a);
         DlogitsEpi<PL> epi = {};
         epi.D = (uint16_t *)(w + p.D);
-        epi.ldd = p.vmax;
-        epi.plane = p.tp * p.vmax;
+        epi.ldd = p.ldd;
+        epi.plane = p.tp * p.ldd;
         epi.v = (int)vn;
         epi.row = row;
         epi.at_ = at;
@@ -716,9 +830,9 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         MN_KCHECK(s, "k_nt");
         mm::KnArgs g = {};
         g.A = w + p.D;
-        g.lda = 2 * p.vmax;
+        g.lda = 2 * p.ldd;
         g.ldb = 2 * p.kp;
-        g.planeA = 2 * p.tp * p.vmax;
+        g.planeA = 2 * p.tp * p.ldd;
         g.nseg = F32 ? 6 : 1;
         mm::KnArgs gq = g, gc = g;
         gq.B = Cp + j0 * g.ldb;

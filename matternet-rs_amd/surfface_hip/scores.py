@@ -101,7 +101,7 @@ def scores_i8(queries: Int8Rows, items: Int8Rows, dtype=torch.float32) -> torch.
         raise ValueError(f"queries have {d} columns, items {items.d}")
     L = _lib.lib()
     need = 0
-    if d % 64:  # whole k-steps need no workspace
+    if d % 64 and m:  # whole k-steps need no workspace
         b = C.c_size_t()
         _lib.check(L.mn_scores_i8_workspace(m, d, C.byref(b)))
         need = b.value

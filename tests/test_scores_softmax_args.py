@@ -39,11 +39,13 @@ def test_scores_refusals():
     assert f(ty=1) == E.MN_ENOTSUP
     assert f(Q=None) == f(c=None) == f(qs=None) == f(cs=None) == f(Y=None) == E.MN_EINVAL
     assert f(Q=ODD) == f(c=ODD) == E.MN_EINVAL
-    assert f(ws=None) == f(wb=4 * 64 - 1) == f(ws=ODD) == E.MN_ECAP
+    assert f(m=65, ws=None) == f(m=65, wb=65 * 64 - 1) == f(m=65, ws=ODD) == E.MN_ECAP
     assert f(m=0) == f(n=0) == E.MN_OK
     b = C.c_size_t()
-    assert L.mn_scores_i8_workspace(4, 20, C.byref(b)) == 0 and b.value == 4 * 64
-    assert L.mn_scores_i8_workspace(4, 128, C.byref(b)) == 0 and b.value == 0
+    assert L.mn_scores_i8_workspace(65, 20, C.byref(b)) == 0 and b.value == 65 * 64
+    assert L.mn_scores_i8_workspace(64, 20, C.byref(b)) == 0 and b.value == 0
+    assert L.mn_scores_i8_workspace(64, 131071, C.byref(b)) == 0 and b.value == 64 * 131072
+    assert L.mn_scores_i8_workspace(65, 128, C.byref(b)) == 0 and b.value == 0
     assert L.mn_scores_i8_workspace(4, 131072, C.byref(b)) == E.MN_EINVAL
     assert L.mn_scores_i8_workspace(4, 20, None) == E.MN_EINVAL
 
