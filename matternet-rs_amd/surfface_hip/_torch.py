@@ -20,33 +20,44 @@ def require_cuda(t: torch.Tensor, dtype, name: str, ndim: int | None = None) -> 
 def require_aligned(t: torch.Tensor, dtype, name: str, ndim: int, device=None) -> torch.Tensor:
     """require_cuda, and a copy where the rows start off a 16-byte border (a
     slice of a larger tensor); device: where the call's other tensors are."""
-    t = require_cuda(t, dtype, name, ndim)
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.dim() == ndim:
+        if not t.is_contiguous():
+            t = t.contiguous()
+    else:
+        t = require_cuda(t, dtype, name, ndim)
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, other tensors of the call on {device}")
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def on_stream(fn):
-    """For calls that return before their work is done: with `stream` given, it
-    is the current stream inside, so that what is allocated belongs to it, and
-    the inputs' memory is kept until its work on them is done."""
+def enqueues(fn):
+    """For calls that return before their work is done (first argument: a
+    tensor, or something with codes): on_device, and with `stream` given it is
+    the current stream inside, so that what is allocated belongs to it, and the
+    inputs' memory is kept until its work on them is done."""
     import functools
 
     @functools.wraps(fn)
     def wrapped(*args, stream=None, **kwargs):
         if stream is None:
-            return fn(*args, **kwargs)
+            t = args[0] if args else None
+            t = getattr(t, "codes", t)
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() == torch.cuda.current_device():
+                return fn(*args, **kwargs)
+            with torch.cuda.device(t.device):
+                return fn(*args, **kwargs)
         with torch.cuda.stream(stream):
             for a in (*args, *kwargs.values()):
                 for t in (a, getattr(a, "codes", None), getattr(a, "scale", None)):
-                    if isinstance(t, torch.Tensor) and t.device.type == "cuda":
+                    if isinstance(t, torch.Tensor) and t.is_cuda:
                         t.record_stream(stream)
             return fn(*args, **kwargs)
     return wrapped
 
 
-def current_stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+def raw_stream(t: torch.Tensor) -> int:
+    """The handle of the current stream of t's device."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def ptr(t: torch.Tensor) -> C.c_void_p:

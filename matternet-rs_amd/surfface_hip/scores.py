@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._torch import current_stream, on_device, on_stream, require_aligned, require_cuda
+from ._torch import enqueues, raw_stream, require_aligned, require_cuda
 
 VALUE_TYPES = {torch.float32: _lib.MN_F32, torch.bfloat16: _lib.MN_BF16}
 
@@ -53,8 +53,7 @@ def _rows(r: Int8Rows, name: str, device=None):
     return codes, scale, n, ld
 
 
-@on_device
-@on_stream
+@enqueues
 def quantize_rows(X: torch.Tensor) -> Int8Rows:
     """Rows of X [n, d] (f32 or bf16) in 8 bits: scale = max|x| / 127, code =
     rint(x (127 (1 / max|x|))).  A row of zeros gets scale 0; a row that holds an
@@ -69,12 +68,11 @@ def quantize_rows(X: torch.Tensor) -> Int8Rows:
     codes = torch.empty((n, ld), dtype=torch.int8, device=x.device)
     scale = torch.empty(n, dtype=torch.float32, device=x.device)
     _lib.check(_lib.lib().mn_quantize_rows_i8(x.data_ptr(), VALUE_TYPES[x.dtype], n, d, codes.data_ptr(), ld,
-                                              scale.data_ptr(), current_stream()))
+                                              scale.data_ptr(), raw_stream(x)))
     return Int8Rows(codes, scale, d)
 
 
-@on_device
-@on_stream
+@enqueues
 def dequantize_rows(rows: Int8Rows, dtype=torch.float32) -> torch.Tensor:
     """The values [n, d] that the codes stand for, as f32 or rounded to bf16."""
     if dtype not in VALUE_TYPES:
@@ -82,12 +80,11 @@ def dequantize_rows(rows: Int8Rows, dtype=torch.float32) -> torch.Tensor:
     codes, scale, n, ld = _rows(rows, "rows")
     X = torch.empty((n, rows.d), dtype=dtype, device=codes.device)
     _lib.check(_lib.lib().mn_dequantize_rows_i8(codes.data_ptr(), ld, scale.data_ptr(), n, rows.d, X.data_ptr(),
-                                                VALUE_TYPES[dtype], current_stream()))
+                                                VALUE_TYPES[dtype], raw_stream(X)))
     return X
 
 
-@on_device
-@on_stream
+@enqueues
 def scores_i8(queries: Int8Rows, items: Int8Rows, dtype=torch.float32) -> torch.Tensor:
     """[m, n] scores of every query with every item: the int8 product (exact
     sums, d <= 131071) times the query's and the item's scale, f32 or rounded
@@ -109,5 +106,5 @@ def scores_i8(queries: Int8Rows, items: Int8Rows, dtype=torch.float32) -> torch.
     Y = torch.empty((m, n), dtype=dtype, device=c.device)
     _lib.check(L.mn_scores_i8(q.data_ptr(), ldq, qs.data_ptr(), m, c.data_ptr(), ldc, cs.data_ptr(), n, d,
                               Y.data_ptr(), VALUE_TYPES[dtype], ws.data_ptr() if need else None, need,
-                              current_stream()))
+                              raw_stream(Y)))
     return Y

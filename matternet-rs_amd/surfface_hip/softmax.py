@@ -21,7 +21,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._torch import current_stream, on_device, on_stream, require_aligned, require_cuda
+from ._torch import enqueues, raw_stream, require_aligned, require_cuda
 from .scores import VALUE_TYPES
 
 
@@ -79,25 +79,27 @@ def _stats_out(n, device):
     return st, [x.data_ptr() for x in (st.rest, st.target, st.loss, st.mean, st.share)]
 
 
-@on_device
-@on_stream
+@enqueues
 def softmax_stats(queries: torch.Tensor, items: torch.Tensor, targets: torch.Tensor, scale: float = 1.0,
                   c_offset: int = 0) -> SoftmaxStats:
     """queries [t, d], items [v, d] (f32 or bf16), targets [t] (int64 or int32,
     global row ids; negative: the query has no part); logits scale q.c, scale >
     0.  items holds the rows c_offset .. c_offset + v - 1 of the table; a target
     among none of a table's rows makes its loss +inf."""
-    q, c, t, n, v, d, kind = _inputs(queries, items, targets)
+    return _stats(_inputs(queries, items, targets), scale, c_offset)
+
+
+def _stats(inputs, scale, c_offset):
+    q, c, t, n, v, d, kind = inputs
     st, out = _stats_out(n, q.device)
     L = _lib.lib()
     ws = _workspace(L, n, v, d, kind, 0, q.device)
     _lib.check(L.mn_softmax_stats(q.data_ptr(), c.data_ptr(), kind, n, v, d, t.data_ptr(), c_offset, float(scale),
-                                  *out, ws.data_ptr(), ws.numel(), current_stream()))
+                                  *out, ws.data_ptr(), ws.numel(), raw_stream(q)))
     return st
 
 
-@on_device
-@on_stream
+@enqueues
 def softmax_merge(rests: torch.Tensor, zts: torch.Tensor, targets: torch.Tensor) -> SoftmaxStats:
     """The stats of a whole table from those of its row ranges: rests and zts
     [parts, t] (softmax_stats' rest and target, gathered over the ranges)."""
@@ -111,12 +113,11 @@ def softmax_merge(rests: torch.Tensor, zts: torch.Tensor, targets: torch.Tensor)
         raise ValueError(f"rests {tuple(r.shape)}, zts {tuple(z.shape)} and targets {tuple(t.shape)} do not fit")
     st, out = _stats_out(n, r.device)
     _lib.check(_lib.lib().mn_softmax_merge(r.data_ptr(), z.data_ptr(), parts, n, t.data_ptr(), *out,
-                                           current_stream()))
+                                           raw_stream(r)))
     return st
 
 
-@on_device
-@on_stream
+@enqueues
 def softmax_backward(queries: torch.Tensor, items: torch.Tensor, targets: torch.Tensor, rest: torch.Tensor,
                      target: torch.Tensor, grad: torch.Tensor, scale: float = 1.0, c_offset: int = 0,
                      grad_scale: torch.Tensor | None = None, need=(True, True)):
@@ -145,31 +146,34 @@ def _backward(q, c, t, n, v, d, kind, re, zt, g, scale, c_offset, gs, need):
             q.data_ptr(), c.data_ptr(), kind, n, v, d, t.data_ptr(), c_offset, float(scale), re.data_ptr(),
             zt.data_ptr(), g.data_ptr(), g.shape[0], None if gs is None else gs.data_ptr(),
             dq.data_ptr() if need[0] else None, dc.data_ptr() if need[1] else None, ws.data_ptr(), ws.numel(),
-            current_stream()))
+            raw_stream(q)))
     return dq, dc
 
 
 class _SoftmaxLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, queries, items, targets, scale, reduction):
-        st = softmax_stats(queries, items, targets, scale)
+        inputs = _inputs(queries, items, targets)
+        st = _stats(inputs, scale, 0)
         ctx.save_for_backward(queries, items, targets)
-        # not the loss and the mean, which the caller may change in place
-        ctx.of = (st.rest, st.target, st.share if reduction == "mean" else None, scale)
+        # what the caller may change in place (loss, mean) is not kept, nor is
+        # a dense copy of an input
+        same = inputs[0] is queries and inputs[1] is items and inputs[2] is targets
+        ctx.of = (inputs[3:] if same else None, st.rest, st.target, st.share if reduction == "mean" else None, scale)
         return st.mean if reduction == "mean" else st.loss if reduction == "none" else st.loss.sum()
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        queries, items, targets = ctx.saved_tensors
-        rest, target, share, scale = ctx.of
-        # on the forward's device: its tensors passed softmax_stats' checks
-        dq, dc = _backward(*_inputs(queries, items, targets), rest, target, grad.reshape(-1).contiguous(), scale, 0,
-                           share, ctx.needs_input_grad[:2])
+        tensors = ctx.saved_tensors
+        sizes, rest, target, share, scale = ctx.of
+        inputs = (*tensors, *sizes) if sizes else _inputs(*tensors)
+        dq, dc = _backward(*inputs, rest, target, grad.reshape(-1).contiguous(), scale, 0, share,
+                           ctx.needs_input_grad[:2])
         return dq, dc, None, None, None
 
 
-@on_device
+@enqueues
 def softmax_loss(queries: torch.Tensor, items: torch.Tensor, targets: torch.Tensor, scale: float = 1.0,
                  reduction: str = "mean") -> torch.Tensor:
     """Softmax cross entropy of queries [t, d] over all rows of items [v, d]
