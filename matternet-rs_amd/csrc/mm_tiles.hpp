@@ -54,6 +54,7 @@ constexpr int KBY = 64;                // bytes of k in a step
 constexpr int NSLOT = 4;
 constexpr int HALF = TILE * KBY;       // one operand's step, 16 KB
 constexpr int NT = 512;
+constexpr int GP = 8;
 
 // planes of A and B in the six products, smallest first
 __device__ __forceinline__ int seg_a(int s) { return (0x001021 >> (4 * s)) & 3; }
@@ -193,12 +194,13 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = w & 3, wj = w >> 2;
     const int fr = lane & 15, fk = lane >> 4;
-    // four panels by eight runs on an XCD at a time
+    // GP panels by 32 / GP runs on an XCD at a time (1, 2, 4, 8, 16: 3.11, 3.11,
+    // 3.11, 3.09, 3.13 ms for a step of 4096 x 131072 x 768)
     int v = xcd_range((int)blockIdx.x, (int)gridDim.x);
-    const int grp = v / (4 * a.slices);
-    v -= grp * 4 * a.slices;
-    const int gp = min(4, a.panels - 4 * grp);
-    const int slice = v / gp, panel = 4 * grp + v % gp;
+    const int grp = v / (GP * a.slices);
+    v -= grp * GP * a.slices;
+    const int gp = min(GP, a.panels - GP * grp);
+    const int slice = v / gp, panel = GP * grp + v % gp;
     const int64_t i0 = (int64_t)panel * TILE;
     const int t0 = slice * a.run, t1 = min(a.tiles, t0 + a.run);
     const int nstep = a.nk * a.nseg * (t1 - t0);
@@ -406,9 +408,11 @@ struct KnArgs {
     int nseg;
 };
 
-// One tile: accumulator r of (f, g) is row m = 16 f + (lane & 15) of the wave's
-// 64, column n = 16 g + 4 (lane >> 4) + r of its 128; z: which run of k-steps.
-template <bool A_T, class EPI>
+// One tile of 256 rows and 32 NF columns (the rest of a step's 256 columns of B
+// is loaded and not used): accumulator r of (f, g) is row m = 16 f + (lane & 15)
+// of the wave's 64, column n = 16 g + 4 (lane >> 4) + r of its 16 NF; z: which
+// run of k-steps.  NF 8 wherever more than 128 columns are wanted, else 4 or 2.
+template <int NF, bool A_T, class EPI>
 __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &epi, int64_t m0, int64_t n0, int z) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -468,12 +472,12 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
         }
     };
 
-    f32x4 acc[4][8];
+    f32x4 acc[4][NF];
 #pragma unroll
     for (int f = 0; f < 4; ++f)
 #pragma unroll
-        for (int g = 0; g < 8; ++g) acc[f][g] = (f32x4)(0.f);
-    u32x4 fi[4], fj[8];
+        for (int g = 0; g < NF; ++g) acc[f][g] = (f32x4)(0.f);
+    u32x4 fi[4], fj[NF];
     // transposed reads: row 8 fk + (fr >> 2) (and 4 below), 16-column slot s
     const int fx = (fr >> 2) | ((fk & 1) << 2);
     const int trow = (8 * fk + (fr >> 2)) * 512 + 8 * (fr & 3);
@@ -500,19 +504,19 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
                 else fi[f] = *reinterpret_cast<const u32x4 *>(ri + so + 16 * f * KBY);
             }
 #pragma unroll
-            for (int g = 0; g < 8; ++g) fj[g] = tr(&rg.b[0][1][0] + so, 8 * wj + g);
+            for (int g = 0; g < NF; ++g) fj[g] = tr(&rg.b[0][1][0] + so, NF * wj + g);
             issue();
             read_window_end<8>();
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int g = 0; g < 8; ++g) acc[f][g] = Bf16::mma(fj[g], fi[f], acc[f][g]);
+                for (int g = 0; g < NF; ++g) acc[f][g] = Bf16::mma(fj[g], fi[f], acc[f][g]);
             window_end();
         }
         if (!wj) window_end();
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    epi(acc, m0 + 64 * wi, n0 + 128 * wj, lane, z);
+    epi(acc, m0 + 64 * wi, n0 + 16 * NF * wj, lane, z);
 }
 
 // What a launch of k_kn2 has of one product: blocks = splits x rows x cols of
@@ -525,16 +529,16 @@ struct KnGrid {
 // Two products in one launch, so that the tiles of the second fill the
 // processors that the last round of the first leaves idle: A [m][k] first, then
 // A [k][m].
-template <class E1, class E2>
+template <int NF, class E1, class E2>
 __global__ __launch_bounds__(NT, 2) void k_kn2(KnArgs a1, E1 e1, KnGrid g1, KnArgs a2, E2 e2, KnGrid g2) {
     __shared__ Ring rg;
     const int b = (int)blockIdx.x, n1 = g1.blocks();
     if (b < n1) {
         const int v = xcd_range(b, n1), r = v / g1.cols;
-        kn_tile<false>(rg, a1, e1, (int64_t)(r % g1.rows) * TILE, (int64_t)(v % g1.cols) * TILE, r / g1.rows);
+        kn_tile<NF, false>(rg, a1, e1, (int64_t)(r % g1.rows) * TILE, (int64_t)(v % g1.cols) * 32 * NF, r / g1.rows);
     } else {
         const int v = xcd_range(b - n1, g2.blocks()), r = v / g2.cols;
-        kn_tile<true>(rg, a2, e2, (int64_t)(r % g2.rows) * TILE, (int64_t)(v % g2.cols) * TILE, r / g2.rows);
+        kn_tile<NF, true>(rg, a2, e2, (int64_t)(r % g2.rows) * TILE, (int64_t)(v % g2.cols) * 32 * NF, r / g2.rows);
     }
 }
 

@@ -40,19 +40,18 @@ struct Pack {
     uint16_t *out;
     const int64_t *targets;  // or NULL
     int64_t rows;
-    int d, kp, blocks;
+    int d, kp, per, blocks;  // per: pieces a thread
     bool vec;                // rows start on 16-byte borders
 };
-constexpr int kPackPer = 8;  // pieces of 8 values a thread
+constexpr int kPackPer = 8;  // at most so many pieces of 8 values a thread
 
 template <bool F32>
 __device__ __forceinline__ void pack(const Pack &p, int block) {
     const int n8 = p.kp / 8;
-    const int64_t base = (int64_t)block * (256 * kPackPer), total = p.rows * n8;
+    const int64_t base = (int64_t)block * (256 * p.per), total = p.rows * n8;
     const int64_t row0 = base / n8;
     const uint32_t rem = (uint32_t)(base - row0 * n8);
-#pragma unroll
-    for (int u = 0; u < kPackPer; ++u) {
+    for (int u = 0; u < p.per; ++u) {
         const uint32_t l = 256 * u + threadIdx.x;
         if (base + l >= total) return;
         const uint32_t x = rem + l, q = x / (uint32_t)n8, k = 8 * (x - q * n8);
@@ -412,6 +411,47 @@ __global__ __launch_bounds__(256) void k_join(const float2 *__restrict__ part, c
     }
 }
 
+// k_join and k_mean in one block of a thread a row, for few rows and pieces:
+// a launch less (4 us of the host) where the rows are not what takes the time
+__global__ __launch_bounds__(1024) void k_join_few(const float2 *__restrict__ part, int n, int t,
+                                                   const int64_t *__restrict__ targets, float *__restrict__ rest,
+                                                   const float *__restrict__ zt, float *__restrict__ loss,
+                                                   float *__restrict__ mean, float *__restrict__ share) {
+    __shared__ float sh[16];
+    const int i = threadIdx.x;
+    float l = 0.f, num = 0.f;
+    if (i < t) {
+        float top = -__builtin_inff(), sum = 0.f;
+        for (int k0 = 0; k0 < n; k0 += 8) {
+            float2 p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = k0 + k < n ? part[(k0 + k) * t + i] : make_float2(-__builtin_inff(), 0.f);
+            float m = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) m = fmaxf(m, p[k].x);
+            const float mz = m == -__builtin_inff() ? 0.f : m;
+            sum *= __builtin_amdgcn_exp2f(top - mz);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum += p[k].y * __builtin_amdgcn_exp2f(p[k].x - mz);
+            top = m;
+        }
+        const float r = sum == 0.f ? -__builtin_inff() : (top == -__builtin_inff() ? sum : (top + log2f(sum)) * kLn2);
+        const bool has = targets[i] >= 0;
+        l = has ? row_loss(r, zt[i]) : 0.f;
+        num = has ? 1.f : 0.f;
+        rest[i] = r;
+        loss[i] = l;
+    }
+    if (!mean) return;
+    auto add = [](float a, float b) { return a + b; };
+    l = block_fold(l, sh, add);
+    num = fmaxf(block_fold(num, sh, add), 1.f);
+    if (i == 0) {
+        *mean = l / num;
+        *share = 1.f / num;
+    }
+}
+
 // gs[1] = the largest |g| of the rows that take part
 __global__ __launch_bounds__(1024) void k_grad_max(const float *__restrict__ grad, int64_t t,
                                                    const int64_t *__restrict__ targets, float *__restrict__ gs) {
@@ -510,13 +550,14 @@ struct PartEpi {
     float *part;
     int64_t m, ld;
     bool first;
-    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][8], int64_t m0, int64_t n0, int lane, int z) const {
+    template <int NF>
+    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][NF], int64_t m0, int64_t n0, int lane, int z) const {
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             const int64_t i = m0 + 16 * f + (lane & 15);
             if (i >= m) continue;
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
+            for (int g = 0; g < NF; ++g) {
                 const int64_t c = n0 + 16 * g + 4 * (lane >> 4);
                 if (c >= ld) continue;
                 mm::f32x4 *p = reinterpret_cast<mm::f32x4 *>(part + ((int64_t)z * m + i) * ld + c);
@@ -531,14 +572,15 @@ struct GradEpi {
     void *out;
     int64_t m, n;
     const float *gs;
-    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][8], int64_t m0, int64_t n0, int lane, int) const {
+    template <int NF>
+    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][NF], int64_t m0, int64_t n0, int lane, int) const {
         const float s = gs[0];
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             const int64_t i = m0 + 16 * f + (lane & 15);
             if (i >= m) continue;
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
+            for (int g = 0; g < NF; ++g) {
                 const int64_t c = n0 + 16 * g + 4 * (lane >> 4);
                 if (c < n) mm::store4<F32>(out, i * n + c, (int)min<int64_t>(4, n - c), acc[f][g] * s);
             }
@@ -591,6 +633,7 @@ struct Plan {
     bool few_packed;    // on packed operands
     int64_t ldd;        // row stride of D
     int64_t vc, vmax;   // items per piece (backward), of the longest piece, in whole tiles
+    int nf;             // 32 nf columns a tile of dQ and dC
     int splits;         // of dQ's sum over a piece
     int pieces, parts;  // of the table; partial sums of dQ in all
     bool apart;         // a piece's partial sums are its own
@@ -657,7 +700,8 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         // costs its run and 20 for its part of the sum (256 KB to memory), one
         // of dC t / 32 and 10.  Free processors take the next block: dC's done
         // by a time are counted from the two times at which dQ's blocks end.
-        const int64_t cols = (d + mm::TILE - 1) / mm::TILE, tiles = panels * cols;
+        p.nf = d > 128 ? 8 : d > 64 ? 4 : 2;
+        const int64_t cols = (d + 32 * p.nf - 1) / (32 * p.nf), tiles = panels * cols;
         const int64_t steps = p.vc / 32, nc = p.vc / mm::TILE * cols, b = t / 32 + 10;
         int64_t best = INT64_MAX;
         for (int64_t s = 1; s <= std::min<int64_t>(steps / 4 + 1, std::max<int64_t>(1, 512 / tiles)); ++s) {
@@ -696,8 +740,10 @@ template <bool F32>
 int prep(const Plan &p, const void *Q, const void *C, const int64_t *targets, char *w, const Rows &r, int64_t row_blocks,
          hipStream_t s) {
     auto one = [&](const void *X, size_t out, int64_t n, const int64_t *tg) {
-        Pack k = {X, (uint16_t *)(w + out), tg, n, p.d, p.kp, 0, p.d % (F32 ? 4 : 8) == 0};
-        k.blocks = (int)((n * (p.kp / 8) + 256 * kPackPer - 1) / (256 * kPackPer));
+        const int64_t pieces = n * (p.kp / 8);
+        const int per = (int)std::max<int64_t>(1, std::min<int64_t>(kPackPer, pieces / (256 * 1024)));
+        Pack k = {X, (uint16_t *)(w + out), tg, n, p.d, p.kp, per, 0, p.d % (F32 ? 4 : 8) == 0};
+        k.blocks = (int)((pieces + 256 * per - 1) / (256 * per));
         return k;
     };
     const Pack q = p.few.blocks && !p.few_packed ? Pack{} : one(Q, p.q, p.t, targets), c = p.pack_c ? one(C, p.c, p.v, nullptr) : Pack{};
@@ -765,6 +811,12 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
                            epi);
         MN_KCHECK(s, "k_nt");
     }
+    if (t <= 1024 && pieces <= 64) {
+        hipLaunchKernelGGL(k_join_few, dim3(1), dim3(1024), 0, s, part, (int)pieces, (int)t, targets, rest, zt, loss, mean,
+                           share);
+        MN_KCHECK(s, "k_join_few");
+        return MN_OK;
+    }
     hipLaunchKernelGGL(k_join, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, part, (const float *)nullptr,
                        (const float *)nullptr, pieces, t, targets, rest, zt, loss);
     MN_KCHECK(s, "k_join");
@@ -807,7 +859,7 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
     if (rc != MN_OK) return rc;
     constexpr int PL = F32 ? 3 : 1;
     const char *Cp = p.pack_c ? w + p.c : (const char *)C;
-    const int row_tiles = (int)(p.tp / mm::TILE), col_tiles = (d + mm::TILE - 1) / mm::TILE;
+    const int row_tiles = (int)(p.tp / mm::TILE), col_tiles = (d + 32 * p.nf - 1) / (32 * p.nf);
     int64_t vn = 0;
     int piece = 0;
     for (int64_t j0 = 0; j0 < v; j0 += vn, ++piece) {
@@ -849,8 +901,13 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         const PartEpi pe = {(float *)(w + p.dq) + (p.apart ? (int64_t)piece * p.splits * t * p.ldp : 0), t, p.ldp,
                             p.apart || piece == 0};
         const GradEpi<F32> ge = {(char *)dC + j0 * d * (F32 ? 4 : 2), vn, d, gs};
-        hipLaunchKernelGGL((mm::k_kn2<PartEpi, GradEpi<F32>>), dim3((unsigned)(nq.blocks() + nc.blocks())), dim3(mm::NT), 0,
-                           s, gq, pe, nq, gc, ge, nc);
+        auto go = [&](auto NF) {
+            hipLaunchKernelGGL((mm::k_kn2<decltype(NF)::value, PartEpi, GradEpi<F32>>), dim3((unsigned)(nq.blocks() + nc.blocks())),
+                               dim3(mm::NT), 0, s, gq, pe, nq, gc, ge, nc);
+        };
+        if (p.nf == 8) go(std::integral_constant<int, 8>());
+        else if (p.nf == 4) go(std::integral_constant<int, 4>());
+        else go(std::integral_constant<int, 2>());
         MN_KCHECK(s, "k_kn2");
     }
     if (dQ) {
