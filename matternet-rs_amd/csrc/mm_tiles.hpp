@@ -307,7 +307,10 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
 // is all that counts.  The queries lie in LDS ([k-step][query][64 bytes], pieces
 // at c ^ 2 ((query >> 3) & 1): no bank conflicts), a wave takes 16 rows of B at
 // a time from memory to registers, four k-steps of loads ahead of their
-// products, and the block's waves go through B side by side.
+// products, and the block's waves go through B side by side.  One query on 1M
+// rows of 768 codes (768 MB): 135 us, 5.7 TB/s; 512 blocks, not 768 (145), 384
+// (146) or 256 (144), loads of 4 steps, not 3 (139) or 6 (143), and through the
+// caches (past them: 150).
 struct FewArgs {
     const char *Q, *B;
     int64_t ldq, ldb;  // bytes, multiples of 16
@@ -327,7 +330,7 @@ inline bool plan_few(FewArgs &a) {
     a.small = bytes <= FEW_SMALL;
     if (bytes > FEW_LARGE) return false;
     const int64_t groups = (a.n + 15) / 16;
-    a.blocks = (int)std::min<int64_t>((groups + 7) / 8, a.small ? 768 : 256);
+    a.blocks = (int)std::min<int64_t>((groups + 7) / 8, a.small ? 512 : 256);
     return true;
 }
 

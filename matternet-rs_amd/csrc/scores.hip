@@ -17,17 +17,18 @@ namespace mn {
 namespace i8 {
 
 // 8 values of a row from column k (a multiple of 8), zeros past column d.
-// vec: rows start on 16-byte borders.
-template <typename T>
+// vec: rows start on 16-byte borders.  NT: past the caches.
+template <bool NT, typename T>
 __device__ __forceinline__ void load8(const T *row, int k, int d, bool vec, float (&v)[8]) {
     if (vec && k + 8 <= d) {
         if constexpr (sizeof(T) == 4) {
-            const float4 a = reinterpret_cast<const float4 *>(row + k)[0], b = reinterpret_cast<const float4 *>(row + k)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            const mm::f32x4 *p = reinterpret_cast<const mm::f32x4 *>(row + k);
+            const mm::f32x4 a = NT ? __builtin_nontemporal_load(p) : p[0], b = NT ? __builtin_nontemporal_load(p + 1) : p[1];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e < 4 ? a[e] : b[e - 4];
         } else {
-            const uint4 a = *reinterpret_cast<const uint4 *>(row + k);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+            const mm::u32x4 *p = reinterpret_cast<const mm::u32x4 *>(row + k);
+            const mm::u32x4 w = NT ? __builtin_nontemporal_load(p) : *p;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = mm::bf16_value((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
         }
@@ -42,8 +43,9 @@ __device__ __forceinline__ void load8(const T *row, int k, int d, bool vec, floa
 }
 
 // L lanes take a row, 8 values a lane at a time; up to 16 values a lane stay in
-// registers between the two passes (longer rows are read again, from L2).  A
-// row's largest |x| is folded as bits: NaN > inf > every finite value, so one
+// registers between the two passes: such rows are read once, past the caches
+// (262144 x 768 f32 and back: 316 us, 339 with ordinary loads); longer ones are
+// read again, from L2.  A row's largest |x| is folded as bits: NaN > inf > every finite value, so one
 // integer maximum also tells whether the row holds something that is not
 // finite.
 // Below 2^-100 the reciprocal 1 / a could overflow, above 2^100 be subnormal:
@@ -63,7 +65,8 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int k = 8 * (L * u + l);
-        if (u == 0 || k < d) load8(row, k, d, vec, v[u]);
+        if (k < d && d <= 16 * L) load8<true>(row, k, d, vec, v[u]);
+        else if (k < d) load8<false>(row, k, d, vec, v[u]);
         else
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
@@ -72,7 +75,7 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64
     }
     for (int k = 8 * (2 * L + l); k < d; k += 8 * L) {
         float x[8];
-        load8(row, k, d, vec, x);
+        load8<false>(row, k, d, vec, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
     }
@@ -90,7 +93,7 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = u == 0 ? v[0][e] : v[1][e];
         } else {
-            load8(row, k, d, vec, x);
+            load8<false>(row, k, d, vec, x);
         }
         uint32_t w[2] = {0, 0};
 #pragma unroll
@@ -104,40 +107,51 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64
 }
 
 // 16 bytes of values (4 f32 or 8 bf16) a thread at a time, so that a wave's
-// store is 1 KB in a row; a block takes 8 x 256 pieces.
-template <typename T>
+// store is 1 KB in a row; a block takes U x 256 pieces, all loads first.  From
+// 2^21 pieces (32 MB of values) on U is 4 and the stores pass the caches by:
+// quantise + dequantise of 262144 x 768 f32 took 339 us so, 361 with ordinary
+// stores, 398 with U 1 (U 2 and 8: 361, 366).
+template <typename T, int U>
 __global__ __launch_bounds__(256) void k_dequantize(const int8_t *__restrict__ codes, int64_t ld,
                                                     const float *__restrict__ scale, int64_t n, int d, bool vec,
                                                     T *__restrict__ X) {
     constexpr int P = 16 / sizeof(T);
     const uint32_t np = (uint32_t)(d + P - 1) / P;
-    const int64_t base = (int64_t)blockIdx.x * 2048, total = n * np;
+    const int64_t base = (int64_t)blockIdx.x * (256 * U), total = n * np;
     const int64_t row0 = base / np;
     const uint32_t rem = (uint32_t)(base - row0 * np);
+    const uint32_t left = (uint32_t)min<int64_t>(256 * U, total - base);
+    uint32_t q[U], c[U][2];
+    int k[U];
+    float s[U];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-        const uint32_t l = 256 * u + threadIdx.x;
-        if (base + l >= total) return;
-        const uint32_t x = rem + l, q = x / np;
-        const int k = P * (int)(x - q * np);
-        const int64_t i = row0 + q;
-        const float s = scale[i];
-        uint32_t c[2];
-        __builtin_memcpy(c, codes + i * ld + k, P);
+    for (int u = 0; u < U; ++u) {
+        const uint32_t l = min(256 * u + threadIdx.x, left - 1), x = rem + l;
+        q[u] = x / np;
+        k[u] = P * (int)(x - q[u] * np);
+        s[u] = scale[row0 + q[u]];
+        __builtin_memcpy(c[u], codes + (row0 + q[u]) * ld + k[u], P);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (256 * u + threadIdx.x >= left) return;
         float v[P];
 #pragma unroll
-        for (int e = 0; e < P; ++e) v[e] = (float)(int8_t)(c[e >> 2] >> (8 * (e & 3))) * s;
-        T *out = X + i * d + k;
-        if (vec && k + P <= d) {
+        for (int e = 0; e < P; ++e) v[e] = (float)(int8_t)(c[u][e >> 2] >> (8 * (e & 3))) * s[u];
+        T *out = X + (row0 + q[u]) * d + k[u];
+        if (vec && k[u] + P <= d) {
+            mm::u32x4 y;
             if constexpr (P == 4)
-                *reinterpret_cast<float4 *>(out) = make_float4(v[0], v[1], v[2], v[3]);
+                y = (mm::u32x4){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
             else
-                *reinterpret_cast<uint4 *>(out) = make_uint4(mm::bf16_pair(v[0], v[1]), mm::bf16_pair(v[2], v[3]),
-                                                             mm::bf16_pair(v[4], v[5]), mm::bf16_pair(v[6], v[7]));
+                y = (mm::u32x4){mm::bf16_pair(v[0], v[1]), mm::bf16_pair(v[2], v[3]), mm::bf16_pair(v[4], v[5]),
+                                mm::bf16_pair(v[6], v[7])};
+            if constexpr (U > 1) __builtin_nontemporal_store(y, reinterpret_cast<mm::u32x4 *>(out));
+            else *reinterpret_cast<mm::u32x4 *>(out) = y;
         } else {
 #pragma unroll
             for (int e = 0; e < P; ++e)
-                if (k + e < d) {
+                if (k[u] + e < d) {
                     if constexpr (P == 4) out[e] = v[e];
                     else out[e] = mm::bf16_bits(v[e]);
                 }
@@ -181,7 +195,10 @@ struct ScoreEpi {
     }
     // 16 rows by 256 bytes at a time through LDS (272 bytes a row), so that a
     // store of the wave is 256 bytes of each of four rows; rows of Y on 16-byte
-    // borders or not (a store may start anywhere)
+    // borders or not (a store may start anywhere).  4096 x 131072 x 768 to bf16:
+    // 560 us so, 605 with 128 bytes of each of 8 rows, 830 with 64 of each of 16
+    // (D of the softmax loss, whose row stride is ours, takes the same time with
+    // all three); without any store 475, without this whole step 337.
     __device__ __forceinline__ void tile(Shared &sh, char *stage, mm::i32x4 (&acc)[4][8], int64_t j0, int lane, int par) {
         constexpr int E = 16 / sizeof(T), PASS = sizeof(T) / 2;  // values of a piece; passes of 128 / PASS columns
         const int jl = 8 * (lane >> 4);
@@ -303,8 +320,8 @@ extern "C" int mn_quantize_rows_i8(const void *X, int32_t x_type, int64_t n, int
     mn::clear_error();
     MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX, MN_EINVAL,
                "mn_quantize_rows_i8: n >= 0, d >= 1, ld >= d and a multiple of 16 needed");
-    MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 2048 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
-               "mn_quantize_rows_i8: n < 2^31 - 1 rows and n d < 2^43 needed");
+    MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 256 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
+               "mn_quantize_rows_i8: n < 2^31 - 1 rows and n d < 2^40 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_quantize_rows_i8: MN_F32 or MN_BF16");
     if (n == 0) return MN_OK;
     MN_REQUIRE(X && codes && scale, MN_EINVAL, "mn_quantize_rows_i8: NULL pointer");
@@ -322,21 +339,26 @@ extern "C" int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const floa
     mn::clear_error();
     MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX, MN_EINVAL,
                "mn_dequantize_rows_i8: n >= 0, d >= 1, ld >= d and a multiple of 16 needed");
-    MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 2048 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
-               "mn_dequantize_rows_i8: n < 2^31 - 1 rows and n d < 2^43 needed");
+    MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 256 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
+               "mn_dequantize_rows_i8: n < 2^31 - 1 rows and n d < 2^40 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_dequantize_rows_i8: MN_F32 or MN_BF16");
     if (n == 0) return MN_OK;
     MN_REQUIRE(X && codes && scale, MN_EINVAL, "mn_dequantize_rows_i8: NULL pointer");
     MN_REQUIRE(aligned16(codes), MN_EINVAL, "mn_dequantize_rows_i8: codes not 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const int per = x_type == MN_F32 ? 4 : 8;
-    const dim3 grid((unsigned)((n * ((d + per - 1) / per) + 2047) / 2048));
-    if (x_type == MN_F32)
-        hipLaunchKernelGGL(k_dequantize<float>, grid, dim3(256), 0, s, codes, ld, scale, n, d,
-                           d % 4 == 0 && aligned16(X), (float *)X);
-    else
-        hipLaunchKernelGGL(k_dequantize<uint16_t>, grid, dim3(256), 0, s, codes, ld, scale, n, d,
-                           d % 8 == 0 && aligned16(X), (uint16_t *)X);
+    const int64_t pieces = n * (x_type == MN_F32 ? (d + 3) / 4 : (d + 7) / 8);
+    auto go = [&](auto U, auto *x) {
+        typedef std::remove_pointer_t<decltype(x)> T;
+        constexpr int u = decltype(U)::value;
+        hipLaunchKernelGGL((k_dequantize<T, u>), dim3((unsigned)((pieces + 256 * u - 1) / (256 * u))), dim3(256), 0, s, codes,
+                           ld, scale, n, d, (d * sizeof(T)) % 16 == 0 && aligned16(X), x);
+    };
+    auto size = [&](auto *x) {
+        if (pieces >= 1 << 21) go(std::integral_constant<int, 4>(), x);
+        else go(std::integral_constant<int, 1>(), x);
+    };
+    if (x_type == MN_F32) size((float *)X);
+    else size((uint16_t *)X);
     MN_KCHECK(s, "k_dequantize");
     return MN_OK;
 }

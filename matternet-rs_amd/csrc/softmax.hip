@@ -40,61 +40,64 @@ struct Pack {
     uint16_t *out;
     const int64_t *targets;  // or NULL
     int64_t rows;
-    int d, kp, per, blocks;  // per: pieces a thread
+    int d, kp, per, blocks;  // per: 1 or kPackPer
     bool vec;                // rows start on 16-byte borders
 };
-constexpr int kPackPer = 8;  // at most so many pieces of 8 values a thread
+constexpr int kPackPer = 4;  // pieces of 8 values a thread of a large matrix (a small one: 1)
 
-template <bool F32>
+template <bool F32, int U>
 __device__ __forceinline__ void pack(const Pack &p, int block) {
-    const int n8 = p.kp / 8;
-    const int64_t base = (int64_t)block * (256 * p.per), total = p.rows * n8;
+    const uint32_t n8 = p.kp / 8;
+    const int64_t base = (int64_t)block * (256 * U), total = p.rows * n8;
     const int64_t row0 = base / n8;
-    const uint32_t rem = (uint32_t)(base - row0 * n8);
-    for (int u = 0; u < p.per; ++u) {
-        const uint32_t l = 256 * u + threadIdx.x;
-        if (base + l >= total) return;
-        const uint32_t x = rem + l, q = x / (uint32_t)n8, k = 8 * (x - q * n8);
+    const uint32_t rem = (uint32_t)(base - row0 * n8), left = (uint32_t)min<int64_t>(256 * U, total - base);
+    mm::u32x4 v[U][F32 ? 2 : 1];  // all loads first
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t x = rem + min(256 * u + threadIdx.x, left - 1), q = x / n8;
+        const int k = 8 * (int)(x - q * n8);
         const int64_t i = row0 + q;
         const bool has = !p.targets || p.targets[i] >= 0;
-        uint16_t *o = p.out + 8 * (base + l);
-        if constexpr (F32) {
-            const float *src = (const float *)p.X + i * p.d + k;
-            float v[8];
-            if (p.vec && k + 8 <= (uint32_t)p.d) {
-                const float4 v0 = reinterpret_cast<const float4 *>(src)[0], v1 = reinterpret_cast<const float4 *>(src)[1];
-                v[0] = v0.x, v[1] = v0.y, v[2] = v0.z, v[3] = v0.w;
-                v[4] = v1.x, v[5] = v1.y, v[6] = v1.z, v[7] = v1.w;
+        constexpr int E = F32 ? 4 : 8;  // values of 16 bytes
+#pragma unroll
+        for (int h = 0; h < (F32 ? 2 : 1); ++h) {
+            const int c = k + E * h;
+            if (p.vec && has && c + E <= p.d) {
+                const mm::u32x4 *src = reinterpret_cast<const mm::u32x4 *>((const char *)p.X + (i * p.d + c) * (16 / E));
+                v[u][h] = *src;
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = k + e < (uint32_t)p.d ? src[e] : 0.f;
-            }
-            uint32_t w[3][4];
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                uint16_t a[3], b[3];
-                mm::split3(has ? v[e] : 0.f, a);
-                mm::split3(has ? v[e + 1] : 0.f, b);
-#pragma unroll
-                for (int s = 0; s < 3; ++s) w[s][e / 2] = (uint32_t)a[s] | ((uint32_t)b[s] << 16);
-            }
-#pragma unroll
-            for (int s = 0; s < 3; ++s)
-                *reinterpret_cast<uint4 *>(o + s * (8 * total)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
-        } else {
-            const uint16_t *src = (const uint16_t *)p.X + i * p.d + k;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (has) {
-                if (p.vec && k + 8 <= (uint32_t)p.d) {
-                    v = *reinterpret_cast<const uint4 *>(src);
-                } else {
-                    uint32_t e[8];
-#pragma unroll
-                    for (int q8 = 0; q8 < 8; ++q8) e[q8] = k + q8 < (uint32_t)p.d ? src[q8] : 0u;
-                    v = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (F32) {
+                        v[u][h][e] = has && c + e < p.d ? ((const uint32_t *)p.X)[i * p.d + c + e] : 0u;
+                    } else {
+                        const uint16_t *src = (const uint16_t *)p.X + i * p.d + c + 2 * e;
+                        const uint32_t lo = has && c + 2 * e < p.d ? src[0] : 0u, hi = has && c + 2 * e + 1 < p.d ? src[1] : 0u;
+                        v[u][h][e] = lo | (hi << 16);
+                    }
                 }
             }
-            *reinterpret_cast<uint4 *>(o) = v;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t l = 256 * u + threadIdx.x;
+        if (l >= left) return;
+        uint16_t *o = p.out + 8 * (base + l);
+        if constexpr (F32) {
+            mm::u32x4 w[3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint16_t a[3], b[3];
+                mm::split3(__uint_as_float(v[u][e >> 1][2 * e & 3]), a);
+                mm::split3(__uint_as_float(v[u][e >> 1][(2 * e + 1) & 3]), b);
+#pragma unroll
+                for (int s = 0; s < 3; ++s) w[s][e] = (uint32_t)a[s] | ((uint32_t)b[s] << 16);
+            }
+#pragma unroll
+            for (int s = 0; s < 3; ++s) *reinterpret_cast<mm::u32x4 *>(o + s * (8 * total)) = w[s];
+        } else {
+            *reinterpret_cast<mm::u32x4 *>(o) = v[u][0];
         }
     }
 }
@@ -237,9 +240,9 @@ __device__ __forceinline__ void rows(const Rows &p, int block) {
 template <bool F32>
 __global__ __launch_bounds__(256) void k_prep(Pack q, Pack c, Rows r) {
     int b = (int)blockIdx.x;
-    if (b < q.blocks) return pack<F32>(q, b);
+    if (b < q.blocks) return q.per == 1 ? pack<F32, 1>(q, b) : pack<F32, kPackPer>(q, b);
     b -= q.blocks;
-    if (b < c.blocks) return pack<F32>(c, b);
+    if (b < c.blocks) return c.per == 1 ? pack<F32, 1>(c, b) : pack<F32, kPackPer>(c, b);
     rows<F32>(r, b - c.blocks);
 }
 
@@ -741,7 +744,7 @@ int prep(const Plan &p, const void *Q, const void *C, const int64_t *targets, ch
          hipStream_t s) {
     auto one = [&](const void *X, size_t out, int64_t n, const int64_t *tg) {
         const int64_t pieces = n * (p.kp / 8);
-        const int per = (int)std::max<int64_t>(1, std::min<int64_t>(kPackPer, pieces / (256 * 1024)));
+        const int per = pieces >= kPackPer * 256 * 1024 ? kPackPer : 1;
         Pack k = {X, (uint16_t *)(w + out), tg, n, p.d, p.kp, per, 0, p.d % (F32 ? 4 : 8) == 0};
         k.blocks = (int)((pieces + 256 * per - 1) / (256 * per));
         return k;
