@@ -7,13 +7,7 @@
 //   k_kn2  Y[m][n] = sum_k A(m,k) B[k][n]    (A [m][k] or [k][m]): one 256 x 256
 //          tile and run of k a block, two such products in a launch
 // with f32 (bf16 operands) or int32 (int8 operands) sums; an epilogue object
-// takes each wave's accumulators.
-//
-// f32 operands come as three bf16 planes x = h + m + l (8 + 8 + 8 significant
-// bits: exact but for subnormal tails).  Their product is the sum of six bf16
-// products (hh, hm, mh, hl, lh, mm); what is left out (ml, lm, ll) is below
-// 2^-25 of |x||y|, the rounding of one f32 product.  The small ones are added
-// first.  Six products at the bf16 rate are 2.7 times the f32 matrix rate.
+// takes each wave's accumulators.  f32 operands: mm_f32.hpp.
 //
 // Schedule (k_nt, k_kn2).  Eight waves, each 64 (i, m) x 128 (j, n) = 4 x 8
 // tiles of 16 x 16: 128 accumulator registers.  A k-step is 64 bytes of k (32
@@ -55,10 +49,6 @@ constexpr int NSLOT = 4;
 constexpr int HALF = TILE * KBY;       // one operand's step, 16 KB
 constexpr int NT = 512;
 constexpr int GP = 8;
-
-// planes of A and B in the six products, smallest first
-__device__ __forceinline__ int seg_a(int s) { return (0x001021 >> (4 * s)) & 3; }
-__device__ __forceinline__ int seg_b(int s) { return (0x010201 >> (4 * s)) & 3; }
 
 struct Bf16 {
     typedef f32x4 acc_t;
@@ -148,12 +138,11 @@ __device__ __forceinline__ int xcd_range(int b, int n) {
 }
 
 struct NtArgs {
-    const char *A;      // [planes][m][lda] bytes, rows zero from their end to nk * KBY
-    const char *B;      // [planes][n][ldb]; bytes past bmax + 16 of a row are never read
-    int64_t lda, ldb, planeA, planeB;
+    const char *A;      // [m][lda] bytes, rows zero from their end to the end of nk steps
+    const char *B;      // [n][ldb]; bytes past bmax + 16 of a row are never read
+    int64_t lda, ldb;
     int64_t m, n;
     int nk;             // k-steps of a row
-    int nseg;           // 1, or 6 (f32 planes)
     int bmax;           // last 16-byte piece of a row of B
     int panels, slices; // 256-row panels of A; runs of tiles of B
     int tiles, run;     // tiles of B, tiles of a run
@@ -177,6 +166,18 @@ inline void plan_runs(NtArgs &a) {
     a.slices = (a.tiles + a.run - 1) / a.run;
 }
 
+// A block's panel of A and run of tiles of B: GP panels by 32 / GP runs on an
+// XCD at a time (1, 2, 4, 8, 16: 3.11, 3.11, 3.11, 3.09, 3.13 ms for a step of
+// 4096 x 131072 x 768).
+__device__ __forceinline__ void block_of(const NtArgs &a, int b, int n, int &panel, int &slice) {
+    int v = xcd_range(b, n);
+    const int grp = v / (GP * a.slices);
+    v -= grp * GP * a.slices;
+    const int gp = min(GP, a.panels - GP * grp);
+    slice = v / gp;
+    panel = GP * grp + v % gp;
+}
+
 // Epilogue: init (before the loop), fetch (a tile's loads to LDS; FETCH: there
 // are any), tile (a tile's accumulators; stage: STAGE bytes of LDS of the
 // wave's own; with `counted` set it issued at least STORES store instructions),
@@ -194,16 +195,11 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = w & 3, wj = w >> 2;
     const int fr = lane & 15, fk = lane >> 4;
-    // GP panels by 32 / GP runs on an XCD at a time (1, 2, 4, 8, 16: 3.11, 3.11,
-    // 3.11, 3.09, 3.13 ms for a step of 4096 x 131072 x 768)
-    int v = xcd_range((int)blockIdx.x, (int)gridDim.x);
-    const int grp = v / (GP * a.slices);
-    v -= grp * GP * a.slices;
-    const int gp = min(GP, a.panels - GP * grp);
-    const int slice = v / gp, panel = GP * grp + v % gp;
+    int slice, panel;
+    block_of(a, (int)blockIdx.x, (int)gridDim.x, panel, slice);
     const int64_t i0 = (int64_t)panel * TILE;
     const int t0 = slice * a.run, t1 = min(a.tiles, t0 + a.run);
-    const int nstep = a.nk * a.nseg * (t1 - t0);
+    const int nstep = a.nk * (t1 - t0);
 
     // ---- loads: wave w stages rows 32 w .. 32 w + 31 of both operands
     const int r0 = 32 * w + (lane >> 2), r1 = r0 + 16;
@@ -212,19 +208,15 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     const int pcj0 = 16 * ((lane & 3) ^ (((r0 >> 4) & 1) << 1)), pcj1 = 16 * ((lane & 3) ^ (((r1 >> 4) & 1) << 1));
     const int vi0 = min(r0, ilast) * (int)a.lda + pci, vi1 = min(r1, ilast) * (int)a.lda + pci;
     int vj0 = 0, vj1 = 0;
-    int st = t0, ss = 0, sk = 0;   // the staged step: tile, product, k
+    int st = t0, sk = 0;   // the staged step: tile, k
     uint32_t slot = 0;
-    const char *pa, *pb;
-    auto bases = [&]() __attribute__((always_inline)) {
-        pa = a.A + i0 * a.lda + (a.nseg == 1 ? 0 : seg_a(ss) * a.planeA);
-        pb = a.B + (int64_t)st * TILE * a.ldb + (a.nseg == 1 ? 0 : seg_b(ss) * a.planeB);
-    };
+    const char *pa = a.A + i0 * a.lda, *pb;
     auto rows_j = [&]() __attribute__((always_inline)) {
+        pb = a.B + (int64_t)st * TILE * a.ldb;
         const int jlast = (int)min<int64_t>(TILE - 1, a.n - 1 - (int64_t)st * TILE);
         vj0 = min(r0, jlast) * (int)a.ldb;
         vj1 = min(r1, jlast) * (int)a.ldb;
     };
-    bases();
     rows_j();
     const uint32_t li = lds_addr(&rg.b[0][0][32 * w * KBY]), lj = lds_addr(&rg.b[0][1][32 * w * KBY]);
     auto issue = [&]() __attribute__((always_inline)) {
@@ -236,18 +228,13 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
         dma16(pb + ko, vj1 + min(pcj1, left), lj + slot + 1024);
         slot = (slot + 2 * HALF) & (NSLOT * 2 * HALF - 1);
         if (++sk == a.nk) {
-            sk = 0;
-            if (++ss == a.nseg) {
-                ss = 0;
-                if (st + 1 < t1) {
-                    ++st;
-                    rows_j();
-                } else {  // past the end: the last step again
-                    ss = a.nseg - 1;
-                    sk = a.nk - 1;
-                }
+            if (st + 1 < t1) {
+                sk = 0;
+                ++st;
+                rows_j();
+            } else {  // past the end: the last step again
+                sk = a.nk - 1;
             }
-            bases();
         }
     };
 
@@ -265,10 +252,13 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     window_end();
     if (wj) window_end();
     int k = 0, t = t0;
-    const int per = a.nk * a.nseg;
+    const int per = a.nk;
     for (int n = 0;; ++n) {
         if (k == 0) {
-            if (n) epi.tile(sh, stage, acc, (int64_t)(t - 1) * TILE + 128 * wj, lane, (t - 1) & 1);
+            if (n) {
+                if constexpr (EPI::STAGE > 0) epi.tile(sh, stage, acc, (int64_t)(t - 1) * TILE + 128 * wj, lane, (t - 1) & 1);
+                else epi.tile(sh, acc, (int64_t)(t - 1) * TILE + 128 * wj, lane);
+            }
             if (n == nstep) break;
             epi.fetch(sh, (int64_t)t * TILE, tid, t & 1);
 #pragma unroll
@@ -402,13 +392,12 @@ void launch_few(const FewArgs &a, const EPI &epi, hipStream_t s) {
 }
 
 struct KnArgs {
-    const char *A;      // [planes][m][lda] (A_T false) or [planes][k][lda] (A_T true); whole tiles exist
-    const char *B;      // [planes][k][ldb]; columns past ldb and rows past k are never read
-    int64_t lda, ldb, planeA, planeB;  // bytes; ldb a multiple of 16
+    const char *A;      // [m][lda] (A_T false) or [k][lda] (A_T true); whole tiles exist
+    const char *B;      // [k][ldb]; columns past ldb and rows past k are never read
+    int64_t lda, ldb;   // bytes; ldb a multiple of 16
     int64_t k;          // rows of B; A's entries past k are zero
     int steps;          // k-steps of 32 of a run (a block takes one)
     int steps_all;
-    int nseg;
 };
 
 // One tile of 256 rows and 32 NF columns (the rest of a step's 256 columns of B
@@ -422,7 +411,7 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
     const int wi = w & 3, wj = w >> 2;
     const int fr = lane & 15, fk = lane >> 4;
     const int s0 = z * a.steps, s1 = min(a.steps_all, s0 + a.steps);
-    const int per = s1 - s0, nstep = max(0, per) * a.nseg;
+    const int nstep = max(0, s1 - s0);
 
     // ---- loads.  [k][256]: wave w stages rows 4 w .. 4 w + 3 in two pieces of
     // two rows; [256][k]: rows 32 w .. as k_nt
@@ -446,14 +435,10 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
         vi1 = (r0 + 16) * (int)a.lda + pc;
         astep = KBY;
     }
-    int ss = 0, sk = s0;
+    int sk = s0;
     uint32_t slot = 0;
-    const char *pa, *pb;
-    auto bases = [&]() __attribute__((always_inline)) {
-        pa = a.A + (a.nseg == 1 ? 0 : seg_a(ss) * a.planeA) + (A_T ? 2 * m0 : m0 * a.lda) + sk * astep;
-        pb = a.B + (a.nseg == 1 ? 0 : seg_b(ss) * a.planeB) + 2 * n0 + sk * kstep;
-    };
-    bases();
+    const char *pa = a.A + (A_T ? 2 * m0 : m0 * a.lda) + sk * astep;
+    const char *pb = a.B + 2 * n0 + sk * kstep;
     const uint32_t li = lds_addr(&rg.b[0][0][2048 * w]), lj = lds_addr(&rg.b[0][1][2048 * w]);
     auto issue = [&]() __attribute__((always_inline)) {
         const int last = (int)min<int64_t>(31, a.k - 1 - (int64_t)sk * 32);
@@ -462,16 +447,10 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
         dma16(pb, min(kr0, last) * (int)a.ldb + cj0, lj + slot);
         dma16(pb, min(kr0 + 2, last) * (int)a.ldb + cj1, lj + slot + 1024);
         slot = (slot + 2 * HALF) & (NSLOT * 2 * HALF - 1);
-        pa += astep;
-        pb += kstep;
-        if (++sk == s1) {
-            if (ss + 1 < a.nseg) {
-                ++ss;
-                sk = s0;
-            } else {  // past the end: the last step again
-                sk = s1 - 1;
-            }
-            bases();
+        if (sk + 1 < s1) {  // past the end: the last step again
+            ++sk;
+            pa += astep;
+            pb += kstep;
         }
     };
 
@@ -570,18 +549,6 @@ __device__ __forceinline__ void store4(void *out, int64_t e, int n, f32x4 x) {
             for (int q = 0; q < n; ++q) p[q] = (uint16_t)((q < 2 ? y.x : y.y) >> (16 * (q & 1)));
         }
     }
-}
-
-// x = h + m + l.  A finite x whose nearest bf16 is infinite takes the one
-// below; m and l of a non-finite x are 0.
-__device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
-    uint16_t h = bf16_bits(x);
-    const bool finite = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
-    if (finite && (h & 0x7f80u) == 0x7f80u) h = (uint16_t)(__float_as_uint(x) >> 16);
-    const float r = finite ? x - bf16_value(h) : 0.f;
-    p[0] = h;
-    p[1] = bf16_bits(r);
-    p[2] = bf16_bits(r - bf16_value(p[1]));
 }
 
 }  // namespace mm

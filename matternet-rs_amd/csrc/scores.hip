@@ -435,7 +435,6 @@ extern "C" int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, 
     a.m = m;
     a.n = n;
     a.nk = ldp / mm::KBY;
-    a.nseg = 1;
     a.bmax = (d + 15) / 16 * 16 - 16;
     mm::plan_runs(a);
     const dim3 grid((unsigned)(a.panels * a.slices));

@@ -18,7 +18,7 @@
 #include <type_traits>
 
 #include "common.hpp"
-#include "mm_tiles.hpp"
+#include "mm_f32.hpp"
 
 namespace mn {
 namespace sm {
@@ -32,49 +32,44 @@ struct Row {
     float rel, lse2, dt, resid;
 };
 
-// A matrix [rows][d] on its way into planes [rows][kp] of bf16, zero past d.
+// A matrix [rows][d] on its way to rows of kp values, zero past d, whole k-steps.
 // Rows whose target is < 0 become zeros, so that what they hold (a NaN, say)
-// reaches no sum.  A thread takes 8 values at a time.
+// reaches no sum.  A thread takes 16 bytes at a time, all loads first.
 struct Pack {
     const void *X;
-    uint16_t *out;
+    char *out;
     const int64_t *targets;  // or NULL
     int64_t rows;
-    int d, kp, per, blocks;  // per: 1 or kPackPer
+    int d, kp, per, blocks;  // per: pieces a thread, 1 or kPackPer
     bool vec;                // rows start on 16-byte borders
 };
-constexpr int kPackPer = 4;  // pieces of 8 values a thread of a large matrix (a small one: 1)
+constexpr int kPackPer = 4;  // of a large matrix
 
 template <bool F32, int U>
 __device__ __forceinline__ void pack(const Pack &p, int block) {
-    const uint32_t n8 = p.kp / 8;
-    const int64_t base = (int64_t)block * (256 * U), total = p.rows * n8;
-    const int64_t row0 = base / n8;
-    const uint32_t rem = (uint32_t)(base - row0 * n8), left = (uint32_t)min<int64_t>(256 * U, total - base);
-    mm::u32x4 v[U][F32 ? 2 : 1];  // all loads first
+    constexpr int E = F32 ? 4 : 8;  // values of a piece
+    const uint32_t np = p.kp / E;
+    const int64_t base = (int64_t)block * (256 * U), total = p.rows * np;
+    const int64_t row0 = base / np;
+    const uint32_t rem = (uint32_t)(base - row0 * np), left = (uint32_t)min<int64_t>(256 * U, total - base);
+    mm::u32x4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t x = rem + min(256 * u + threadIdx.x, left - 1), q = x / n8;
-        const int k = 8 * (int)(x - q * n8);
+        const uint32_t x = rem + min(256 * u + threadIdx.x, left - 1), q = x / np;
+        const int c = E * (int)(x - q * np);
         const int64_t i = row0 + q;
         const bool has = !p.targets || p.targets[i] >= 0;
-        constexpr int E = F32 ? 4 : 8;  // values of 16 bytes
+        if (p.vec && has && c + E <= p.d) {
+            v[u] = *reinterpret_cast<const mm::u32x4 *>((const char *)p.X + (i * p.d + c) * (16 / E));
+        } else {
 #pragma unroll
-        for (int h = 0; h < (F32 ? 2 : 1); ++h) {
-            const int c = k + E * h;
-            if (p.vec && has && c + E <= p.d) {
-                const mm::u32x4 *src = reinterpret_cast<const mm::u32x4 *>((const char *)p.X + (i * p.d + c) * (16 / E));
-                v[u][h] = *src;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (F32) {
-                        v[u][h][e] = has && c + e < p.d ? ((const uint32_t *)p.X)[i * p.d + c + e] : 0u;
-                    } else {
-                        const uint16_t *src = (const uint16_t *)p.X + i * p.d + c + 2 * e;
-                        const uint32_t lo = has && c + 2 * e < p.d ? src[0] : 0u, hi = has && c + 2 * e + 1 < p.d ? src[1] : 0u;
-                        v[u][h][e] = lo | (hi << 16);
-                    }
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (F32) {
+                    v[u][e] = has && c + e < p.d ? ((const uint32_t *)p.X)[i * p.d + c + e] : 0u;
+                } else {
+                    const uint16_t *src = (const uint16_t *)p.X + i * p.d + c + 2 * e;
+                    const uint32_t lo = has && c + 2 * e < p.d ? src[0] : 0u, hi = has && c + 2 * e + 1 < p.d ? src[1] : 0u;
+                    v[u][e] = lo | (hi << 16);
                 }
             }
         }
@@ -82,23 +77,7 @@ __device__ __forceinline__ void pack(const Pack &p, int block) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t l = 256 * u + threadIdx.x;
-        if (l >= left) return;
-        uint16_t *o = p.out + 8 * (base + l);
-        if constexpr (F32) {
-            mm::u32x4 w[3];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint16_t a[3], b[3];
-                mm::split3(__uint_as_float(v[u][e >> 1][2 * e & 3]), a);
-                mm::split3(__uint_as_float(v[u][e >> 1][(2 * e + 1) & 3]), b);
-#pragma unroll
-                for (int s = 0; s < 3; ++s) w[s][e] = (uint32_t)a[s] | ((uint32_t)b[s] << 16);
-            }
-#pragma unroll
-            for (int s = 0; s < 3; ++s) *reinterpret_cast<mm::u32x4 *>(o + s * (8 * total)) = w[s];
-        } else {
-            *reinterpret_cast<mm::u32x4 *>(o) = v[u][0];
-        }
+        if (l < left) *reinterpret_cast<mm::u32x4 *>(p.out + 16 * (base + l)) = v[u];
     }
 }
 
@@ -251,8 +230,12 @@ __global__ __launch_bounds__(256) void k_prep(Pack q, Pack c, Rows r) {
 // target's left out; joined over the lanes and written per run of tiles and
 // half of the columns.  An element costs a max, an fma, an exp and an add: for
 // 768 columns of operands about a seventh of its time on the matrix pipe.
+template <bool F32>
 struct StatsEpi {
-    struct Shared {};
+    // f32's products leave no registers for the state: it lies in LDS
+    struct Shared {
+        float2 s[F32 ? 4 : 1][F32 ? mm::NT : 1];
+    };
     static constexpr bool FETCH = false;
     static constexpr int STORES = 0, STAGE = 0;
     static constexpr bool counted = false;
@@ -263,23 +246,34 @@ struct StatsEpi {
     float scale2;  // scale log2(e)
     int at[4];
     float m2[4], sum[4];
-    int64_t row0;
-    __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
-        row0 = i0 + (lane & 15);
+    int64_t i0_;
+    __device__ __forceinline__ void targets_of(int (&a)[4], int lane) const {
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            const int64_t i = row0 + 16 * f, x = i < t ? targets[i] : -1;
-            at[f] = x >= c_offset && x - c_offset < v ? (int)(x - c_offset) : -1;
-            m2[f] = -__builtin_inff();
-            sum[f] = 0.f;
+            const int64_t i = i0_ + (lane & 15) + 16 * f, x = i < t ? targets[i] : -1;
+            a[f] = x >= c_offset && x - c_offset < v ? (int)(x - c_offset) : -1;
+        }
+    }
+    __device__ __forceinline__ void init(Shared &sh, int64_t i0, int lane) {
+        i0_ = i0;
+        if constexpr (!F32) targets_of(at, lane);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            if constexpr (F32) sh.s[f][threadIdx.x] = make_float2(-__builtin_inff(), 0.f);
+            else m2[f] = -__builtin_inff(), sum[f] = 0.f;
         }
     }
     __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
-    __device__ __forceinline__ void tile(Shared &, char *, mm::f32x4 (&acc)[4][8], int64_t j0, int lane, int) {
+    __device__ __forceinline__ void tile(Shared &sh, mm::f32x4 (&acc)[4][8], int64_t j0, int lane) {
         const int jw = (int)j0, jl = jw + 8 * (lane >> 4);
+        int a[4];
+        if constexpr (F32) targets_of(a, lane);
+        else
+#pragma unroll
+            for (int f = 0; f < 4; ++f) a[f] = at[f];
         bool hit = jw + 128 > v;
 #pragma unroll
-        for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 128u;
+        for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(a[f] - jw) < 128u;
         if (__ballot(hit)) {
 #pragma unroll
             for (int g = 0; g < 8; ++g)
@@ -288,17 +282,20 @@ struct StatsEpi {
 #pragma unroll
                     for (int f = 0; f < 4; ++f) {
                         const int j = jl + 32 * (g >> 1) + 4 * (g & 1) + r;
-                        acc[f][g][r] = j >= v || j == at[f] ? -__builtin_inff() : acc[f][g][r];
+                        acc[f][g][r] = j >= v || j == a[f] ? -__builtin_inff() : acc[f][g][r];
                     }
         }
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
+            float2 old;
+            if constexpr (F32) old = sh.s[f][threadIdx.x];
+            else old = make_float2(m2[f], sum[f]);
             float top = acc[f][0][0];
 #pragma unroll
             for (int g = 0; g < 8; ++g)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[f][g][r]);
-            const float m = fmaxf(m2[f], top * scale2);
+            const float m = fmaxf(old.x, top * scale2);
             const float mz = m == -__builtin_inff() ? 0.f : m;
             float s0 = 0.f, s1 = 0.f;
 #pragma unroll
@@ -308,13 +305,15 @@ struct StatsEpi {
                     s0 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g][r], scale2, -mz));
                     s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g + 1][r], scale2, -mz));
                 }
-            sum[f] = sum[f] * __builtin_amdgcn_exp2f(m2[f] - mz) + (s0 + s1);
-            m2[f] = m;
+            const float s = old.y * __builtin_amdgcn_exp2f(old.x - mz) + (s0 + s1);
+            if constexpr (F32) sh.s[f][threadIdx.x] = make_float2(m, s);
+            else m2[f] = m, sum[f] = s;
         }
     }
-    __device__ __forceinline__ void finish(Shared &, int64_t, int piece, int lane) {
+    __device__ __forceinline__ void finish(Shared &sh, int64_t, int piece, int lane) {
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
+            if constexpr (F32) m2[f] = sh.s[f][threadIdx.x].x, sum[f] = sh.s[f][threadIdx.x].y;
 #pragma unroll
             for (int o = 16; o <= 32; o <<= 1) {
                 const float mo = __shfl_xor(m2[f], o), so = __shfl_xor(sum[f], o);
@@ -322,7 +321,7 @@ struct StatsEpi {
                 sum[f] = sum[f] * __builtin_amdgcn_exp2f(m2[f] - mz) + so * __builtin_amdgcn_exp2f(mo - mz);
                 m2[f] = m;
             }
-            const int64_t i = row0 + 16 * f;
+            const int64_t i = i0_ + (lane & 15) + 16 * f;
             if (lane < 16 && i < t) part[piece * t + i] = make_float2(m2[f], sum[f]);
         }
     }
@@ -465,19 +464,16 @@ __global__ __launch_bounds__(1024) void k_grad_max(const float *__restrict__ gra
     if (threadIdx.x == 0) gs[1] = top;
 }
 
-// D of a piece of the table, [tp][ldd] (three planes for f32 operands); zeros
-// in the rows and columns that only fill tiles.  A store is 64 bytes of each of
-// 16 rows; through LDS, 256 bytes of each of 4 (as the scores', whose row
-// stride is the caller's), it measured slower: 232 against 221 us for 4096 x
-// 32768 x 768.
-template <int PLANES>
+// D of a piece of the table, [tp][ldd], f32 or rounded to bf16; zeros in the
+// rows and columns that only fill tiles.
+template <bool F32>
 struct DlogitsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;
-    static constexpr int STORES = 16 * PLANES, STAGE = 0;
+    static constexpr int STORES = F32 ? 32 : 16, STAGE = 0;
     static constexpr bool counted = true;
-    uint16_t *D;
-    int64_t ldd, plane;
+    char *D;
+    int64_t ldd;
     int v;  // columns of this piece that exist
     const Row *row;
     const int32_t *at_;
@@ -488,11 +484,15 @@ struct DlogitsEpi {
     bool any;
     int64_t i0_;
     __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
-        any = false;
         i0_ = i0;
+        if constexpr (!F32) rows_of(lane);
+    }
+    // f32's products leave no registers for these: read again for every tile
+    __device__ __forceinline__ void rows_of(int lane) {
+        any = false;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            const int64_t i = i0 + 16 * f + (lane & 15);
+            const int64_t i = i0_ + 16 * f + (lane & 15);
             const Row r = row[i];
             rel[f] = r.rel;
             lse2[f] = r.lse2;
@@ -504,14 +504,16 @@ struct DlogitsEpi {
         any = __ballot(any) != 0;
     }
     __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
-    __device__ __forceinline__ void tile(Shared &, char *, mm::f32x4 (&acc)[4][8], int64_t j0, int lane, int) {
+    __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][8], int64_t j0, int lane) {
+        constexpr int SZ = F32 ? 4 : 2;
+        if constexpr (F32) rows_of(lane);
         const int jw = (int)j0, jl = 8 * (lane >> 4);
         bool hit = jw + 128 > v || !any;
 #pragma unroll
         for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 128u;
         const bool slow = __ballot(hit) != 0;
-        char *base = (char *)(D + i0_ * ldd + j0);
-        const int to = 2 * ((lane & 15) * (int)ldd + jl);
+        char *base = D + SZ * (i0_ * ldd + j0);
+        const int to = SZ * ((lane & 15) * (int)ldd + jl);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
 #pragma unroll
@@ -528,18 +530,15 @@ struct DlogitsEpi {
                         x[q] = j >= v || !any ? 0.f : y;
                     }
                 }
-#pragma unroll
-                for (int s = 0; s < PLANES; ++s) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        o[q] = mm::bf16_pair(x[2 * q], x[2 * q + 1]);
-                        if (s + 1 < PLANES) {  // what is left for the next plane (|x| <= 1)
-                            x[2 * q] -= mm::bf16_value((uint16_t)o[q]);
-                            x[2 * q + 1] -= mm::bf16_value((uint16_t)(o[q] >> 16));
-                        }
-                    }
-                    mm::store16(base + 2 * s * plane, to + 32 * f * (int)ldd + 32 * g, make_uint4(o[0], o[1], o[2], o[3]));
+                const int off = to + SZ * (16 * f * (int)ldd + 16 * g);
+                if constexpr (F32) {
+                    mm::store16(base, off, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                                                      __float_as_uint(x[3])));
+                    mm::store16(base, off + 16, make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]),
+                                                           __float_as_uint(x[6]), __float_as_uint(x[7])));
+                } else {
+                    mm::store16(base, off, make_uint4(mm::bf16_pair(x[0], x[1]), mm::bf16_pair(x[2], x[3]),
+                                                      mm::bf16_pair(x[4], x[5]), mm::bf16_pair(x[6], x[7])));
                 }
             }
         }
@@ -629,11 +628,13 @@ inline unsigned grid1(int64_t n, int per, int64_t most = 1 << 20) {
 // Sizes of one call and where its workspace holds what.
 struct Plan {
     int64_t t, v, tp;   // tp: t in whole tiles
-    int d, kp, ldp, planes;
-    bool pack_c;
+    int d, kp, ldp;     // values of a packed row, of a row of dQ's partial sums
+    int size;           // bytes of a value
+    bool pack_c;        // C's rows start off 16-byte borders
+    int64_t ldc;        // bytes of a row of C as the products read it
     mm::NtArgs nt;      // the whole table's logits
     mm::FewArgs few;    // the same for few queries; blocks 0: not so
-    bool few_packed;    // on packed operands
+    bool few_q;         // on the queries as they are
     int64_t ldd;        // row stride of D
     int64_t vc, vmax;   // items per piece (backward), of the longest piece, in whole tiles
     int nf;             // 32 nf columns a tile of dQ and dC
@@ -648,49 +649,39 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
     p.t = t;
     p.v = v;
     p.d = d;
+    p.size = f32 ? 4 : 2;
     p.kp = (d + 31) / 32 * 32;
     p.ldp = (d + 3) / 4 * 4;
-    p.planes = f32 ? 3 : 1;
-    p.pack_c = f32 || p.kp != d;
+    p.pack_c = (d * p.size) % 16 != 0;
+    p.ldc = (int64_t)(p.pack_c ? p.kp : d) * p.size;
     p.tp = (t + mm::TILE - 1) / mm::TILE * mm::TILE;
-    p.nt.lda = p.nt.ldb = p.kp * 2;
-    p.nt.planeA = t * p.kp * 2;
-    p.nt.planeB = v * p.kp * 2;
+    p.nt.lda = (int64_t)p.kp * p.size;
+    p.nt.ldb = p.ldc;
     p.nt.m = t;
     p.nt.n = v;
     p.nt.nk = p.kp / 32;
-    p.nt.nseg = f32 ? 6 : 1;
-    p.nt.bmax = p.kp * 2 - 16;
+    p.nt.bmax = (int)p.ldc - 16;
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += up(b); return at; };
-    p.q = take((size_t)p.planes * t * p.kp * 2);
-    const size_t packed = (size_t)p.planes * v * p.kp * 2;
+    p.q = take((size_t)t * p.kp * p.size);
+    p.c = take(p.pack_c ? (size_t)v * p.kp * p.size : 0);
     if (!backward) {
-        // few queries: items straight to registers (f32: as they are)
-        p.few = {};
-        p.few.m = (int)t;
+        // few queries: items straight to registers
+        p.few.m = (int)std::min<int64_t>(t, 65);
         p.few.n = v;
-        if (f32) {
-            p.few.ldq = p.few.ldb = p.few.qbytes = 4 * d;
-            if (t > 32 || d % 4) p.few.n = 0;
-        } else {
-            p.few.ldq = p.few.ldb = p.few.qbytes = 2 * (d % 8 ? p.kp : d);
-        }
-        if (t > 64 || p.few.n == 0 || !mm::plan_few(p.few)) p.few.blocks = 0;
-        else p.pack_c = !f32 && d % 8 != 0;
-        p.few_packed = p.few.blocks && p.pack_c;
-        p.c = take(p.pack_c ? packed : 0);
+        p.few_q = !p.pack_c;
+        p.few.ldq = p.few.ldb = p.ldc;
+        p.few.qbytes = (int)p.ldc;
+        if (t > (f32 ? 32 : 64) || !mm::plan_few(p.few)) p.few.blocks = 0;
         mm::plan_runs(p.nt);
         p.part = take((size_t)std::max(p.nt.slices * 2, p.few.blocks) * t * 8);
     } else {
-        p.c = take(p.pack_c ? packed : 0);
         // Pieces whose D stays below 256 MB (the last-level cache; 128, 512 and
         // 1024 MB take 3.22, 3.05 and 3.06 ms for 4096 x 131072 x 768, 256 MB
-        // 3.05, and 3.73, 3.70 and 3.73 ms for 1024 x 100000 x 768 in f32, 256
-        // MB 3.55) and whose tiles fill whole rounds of 256 blocks; a short
+        // 3.05) and whose tiles fill whole rounds of 256 blocks; a short
         // rest joins the last piece where it fits.
         const int64_t all = (v + mm::TILE - 1) / mm::TILE, panels = p.tp / mm::TILE;
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(4096, ((int64_t)256 << 20) / (p.tp * mm::TILE * 2 * p.planes)));
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(4096, ((int64_t)256 << 20) / (p.tp * mm::TILE * p.size)));
         const int64_t unit = std::max<int64_t>(1, 256 / panels);
         const int64_t piece = most >= unit ? most / unit * unit : most;
         const int64_t rest = all % piece;
@@ -701,14 +692,14 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         // dQ's runs of k: the cut with the least time for the blocks of both
         // products on 256 processors, dQ's first, in steps: a block of dQ
         // costs its run and 20 for its part of the sum (256 KB to memory), one
-        // of dC t / 32 and 10.  Free processors take the next block: dC's done
+        // of dC t / 32 and 10 (f32, whose steps take four times as long: 5 and 3).  Free processors take the next block: dC's done
         // by a time are counted from the two times at which dQ's blocks end.
         p.nf = d > 128 ? 8 : d > 64 ? 4 : 2;
         const int64_t cols = (d + 32 * p.nf - 1) / (32 * p.nf), tiles = panels * cols;
-        const int64_t steps = p.vc / 32, nc = p.vc / mm::TILE * cols, b = t / 32 + 10;
+        const int64_t steps = p.vc / 32, nc = p.vc / mm::TILE * cols, b = t / 32 + (f32 ? 3 : 10);
         int64_t best = INT64_MAX;
         for (int64_t s = 1; s <= std::min<int64_t>(steps / 4 + 1, std::max<int64_t>(1, 512 / tiles)); ++s) {
-            const int64_t a = (steps + s - 1) / s + 20, nq = tiles * s, full = nq / 256 * a, more = nq % 256;
+            const int64_t a = (steps + s - 1) / s + (f32 ? 5 : 20), nq = tiles * s, full = nq / 256 * a, more = nq % 256;
             int64_t end = full + (more ? a : 0);
             for (int64_t k = (nc + 255) / 256;; ++k) {
                 const int64_t e1 = full + k * b, e2 = std::max<int64_t>(0, e1 - full - a) / b;
@@ -731,8 +722,8 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         p.row = take(sizeof(Row) * p.tp);
         p.at = take(4 * p.tp);
         p.gs = take(8);
-        p.ldd = p.vmax + 64;  // an odd number of 128-byte lines: rows on different memory channels
-        p.D = take((size_t)p.planes * p.tp * p.ldd * 2);
+        p.ldd = p.vmax + 128 / p.size;  // an odd number of 128-byte lines: rows on different memory channels
+        p.D = take((size_t)p.tp * p.ldd * p.size);
         p.dq = take((size_t)p.parts * t * p.ldp * 4);
     }
     p.bytes = o;
@@ -743,13 +734,13 @@ template <bool F32>
 int prep(const Plan &p, const void *Q, const void *C, const int64_t *targets, char *w, const Rows &r, int64_t row_blocks,
          hipStream_t s) {
     auto one = [&](const void *X, size_t out, int64_t n, const int64_t *tg) {
-        const int64_t pieces = n * (p.kp / 8);
+        const int64_t pieces = n * (p.kp * p.size / 16);
         const int per = pieces >= kPackPer * 256 * 1024 ? kPackPer : 1;
-        Pack k = {X, (uint16_t *)(w + out), tg, n, p.d, p.kp, per, 0, p.d % (F32 ? 4 : 8) == 0};
-        k.blocks = (int)((pieces + 256 * per - 1) / (256 * per));
-        return k;
+        const int blocks = (int)((pieces + 256 * per - 1) / (256 * per));
+        return Pack{X, w + out, tg, n, p.d, p.kp, per, blocks, !p.pack_c};
     };
-    const Pack q = p.few.blocks && !p.few_packed ? Pack{} : one(Q, p.q, p.t, targets), c = p.pack_c ? one(C, p.c, p.v, nullptr) : Pack{};
+    const Pack q = p.few.blocks && p.few_q ? Pack{} : one(Q, p.q, p.t, targets);
+    const Pack c = p.pack_c ? one(C, p.c, p.v, nullptr) : Pack{};
     hipLaunchKernelGGL(k_prep<F32>, dim3((unsigned)(q.blocks + c.blocks + row_blocks)), dim3(256), 0, s, q, c, r);
     MN_KCHECK(s, "k_prep");
     return MN_OK;
@@ -760,6 +751,13 @@ static mm::NtArgs nt_args(const Plan &p, const void *C, char *ws) {
     a.A = ws + p.q;
     a.B = p.pack_c ? ws + p.c : (const char *)C;
     return a;
+}
+
+template <bool F32, class EPI>
+void launch_nt(const mm::NtArgs &a, const EPI &epi, hipStream_t s) {
+    const dim3 grid((unsigned)(a.panels * a.slices));
+    if constexpr (F32) hipLaunchKernelGGL((mm::k_nt32<EPI>), grid, dim3(mm::NT), 0, s, a, epi);
+    else hipLaunchKernelGGL((mm::k_nt<mm::Bf16, EPI>), grid, dim3(mm::NT), 0, s, a, epi);
 }
 
 template <bool F32>
@@ -783,8 +781,8 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
     int64_t pieces;
     if (p.few.blocks) {
         mm::FewArgs a = p.few;
-        a.Q = p.few_packed ? w + p.q : (const char *)Q;
-        a.B = p.few_packed ? w + p.c : (const char *)C;
+        a.Q = p.few_q ? (const char *)Q : w + p.q;
+        a.B = p.pack_c ? w + p.c : (const char *)C;
         pieces = a.blocks;
         auto go = [&](auto MF) {
             FewStatsEpi<decltype(MF)::value> epi = {};
@@ -803,15 +801,14 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
     } else {
         const mm::NtArgs a = nt_args(p, C, w);
         pieces = (int64_t)a.slices * 2;
-        StatsEpi epi = {};
+        StatsEpi<F32> epi = {};
         epi.part = part;
         epi.targets = targets;
         epi.c_offset = c_offset;
         epi.t = t;
         epi.v = (int)v;
         epi.scale2 = scale * kLog2e;
-        hipLaunchKernelGGL((mm::k_nt<mm::Bf16, StatsEpi>), dim3((unsigned)(a.panels * a.slices)), dim3(mm::NT), 0, s, a,
-                           epi);
+        launch_nt<F32>(a, epi, s);
         MN_KCHECK(s, "k_nt");
     }
     if (t <= 1024 && pieces <= 64) {
@@ -860,7 +857,6 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
     r.at = at;
     const int rc = prep<F32>(p, Q, C, targets, w, r, p.tp / 256, s);
     if (rc != MN_OK) return rc;
-    constexpr int PL = F32 ? 3 : 1;
     const char *Cp = p.pack_c ? w + p.c : (const char *)C;
     const int row_tiles = (int)(p.tp / mm::TILE), col_tiles = (d + 32 * p.nf - 1) / (32 * p.nf);
     int64_t vn = 0;
@@ -871,32 +867,27 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         a.B += j0 * a.ldb;
         a.n = vn;
         mm::plan_runs(a);
-        DlogitsEpi<PL> epi = {};
-        epi.D = (uint16_t *)(w + p.D);
+        DlogitsEpi<F32> epi = {};
+        epi.D = w + p.D;
         epi.ldd = p.ldd;
-        epi.plane = p.tp * p.ldd;
         epi.v = (int)vn;
         epi.row = row;
         epi.at_ = at;
         epi.j_first = j0;
         epi.scale2 = scale * kLog2e;
-        hipLaunchKernelGGL((mm::k_nt<mm::Bf16, DlogitsEpi<PL>>), dim3((unsigned)(a.panels * a.slices)), dim3(mm::NT), 0, s,
-                           a, epi);
+        launch_nt<F32>(a, epi, s);
         MN_KCHECK(s, "k_nt");
         mm::KnArgs g = {};
         g.A = w + p.D;
-        g.lda = 2 * p.ldd;
-        g.ldb = 2 * p.kp;
-        g.planeA = 2 * p.tp * p.ldd;
-        g.nseg = F32 ? 6 : 1;
+        g.lda = p.size * p.ldd;
         mm::KnArgs gq = g, gc = g;
-        gq.B = Cp + j0 * g.ldb;
-        gq.planeB = v * g.ldb;
+        gq.ldb = p.ldc;
+        gq.B = Cp + j0 * p.ldc;
         gq.k = vn;
         gq.steps_all = (int)((vn + 31) / 32);
         gq.steps = (gq.steps_all + p.splits - 1) / p.splits;
+        gc.ldb = (int64_t)p.kp * p.size;
         gc.B = w + p.q;
-        gc.planeB = t * g.ldb;
         gc.k = t;
         gc.steps_all = gc.steps = (int)((t + 31) / 32);
         const mm::KnGrid nq = {dQ ? col_tiles : 0, row_tiles, p.splits};
@@ -905,8 +896,12 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
                             p.apart || piece == 0};
         const GradEpi<F32> ge = {(char *)dC + j0 * d * (F32 ? 4 : 2), vn, d, gs};
         auto go = [&](auto NF) {
-            hipLaunchKernelGGL((mm::k_kn2<decltype(NF)::value, PartEpi, GradEpi<F32>>), dim3((unsigned)(nq.blocks() + nc.blocks())),
-                               dim3(mm::NT), 0, s, gq, pe, nq, gc, ge, nc);
+            constexpr int n = decltype(NF)::value;
+            const dim3 grid((unsigned)(nq.blocks() + nc.blocks()));
+            if constexpr (F32)
+                hipLaunchKernelGGL((mm::k_kn2_32<n, PartEpi, GradEpi<F32>>), grid, dim3(mm::NT), 0, s, gq, pe, nq, gc, ge, nc);
+            else
+                hipLaunchKernelGGL((mm::k_kn2<n, PartEpi, GradEpi<F32>>), grid, dim3(mm::NT), 0, s, gq, pe, nq, gc, ge, nc);
         };
         if (p.nf == 8) go(std::integral_constant<int, 8>());
         else if (p.nf == 4) go(std::integral_constant<int, 4>());
