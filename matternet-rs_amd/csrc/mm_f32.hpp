@@ -7,110 +7,140 @@
 // below: the size of an f32 product's rounding.  Six at the bf16 rate are 2.7
 // times the f32 matrix rate.
 //
-// Operands stay f32 in memory and LDS; a wave splits its fragments after it has
-// read them: 44 vector instructions for 8 values a lane.  That is 2100 cycles a
-// wave for a step of 32 k's next to 3070 of its 192 matrix instructions, and
-// they run side by side: waves w and w + 4 share a SIMD and are one barrier
-// window apart, one reads and splits while the other multiplies.  A step has
-// four windows (fragments of i and half of j, products, other half, products);
-// registers hold 4 + 4 split fragments beside the 128 accumulators.
+// A block has a tile of 256 x 128 (or 64 columns), eight waves of 64 x 64 = 4 x
+// 4 tiles of 16 x 16.  A step is 32 k's.  Each thread loads 24 values of a step
+// to registers, two steps ahead, splits them (44 vector instructions for 8
+// values) and writes three times 8 bf16 to LDS: every value is split once, and a
+// matrix with k in its rows is turned on the way (a thread's 8 values are 8 k's
+// of one column).  LDS holds the three planes of two steps, 144 KB.
 //
-// LDS: two slots of a step (64 KB), filled by loads that go there directly.
-// Waves 0-3 issue a step's loads in their first window, 4-7 at the same time, in
-// their last; both wait for them three windows later, before the barrier after
-// which they are read.
-// Rows of k: 128 bytes a step, piece c (16 bytes) at c ^ s, s = fr / 2 for row
-// fr of a fragment's 16; a lane takes pieces lane / 16 and 4 + lane / 16 (the
-// order of k is the same for both operands).  Rows of k by columns: 1 KB, the
-// 64 bytes of 16 columns s of row k at s ^ ((k / 4) & 3), read a value at a
-// time.  Both are free of bank conflicts.
+// Waves w and w + 4 share a SIMD and run one barrier window apart: while one
+// issues its 96 matrix instructions, the other reads its 24 fragments, splits
+// and writes its part of the next step and starts the loads of the third.  A
+// plane buffer is written in the windows after those in which both halves have
+// read it (lgkmcnt(0) before every barrier).
+//
+// LDS rows: 64 bytes (32 k's of a plane), piece c of row r at c ^ f(r's quad),
+// f = 0, 2, 3, 1: writes of 16 rows and reads of a fragment (16 rows by 4
+// pieces) are free of bank conflicts.  A quad is 4 rows of a fragment's 16.
 #pragma once
 #include "mm_tiles.hpp"
 
 namespace mn {
 namespace mm {
 
-constexpr int KBY32 = 128;             // bytes of k in a step of rows of k
-constexpr int HALF32 = TILE * KBY32;   // one operand's step, 32 KB
+constexpr int COLS32 = 128;                     // columns of a tile of k_nt32
+constexpr int PLANE = (TILE + COLS32) * KBY;    // a plane of a step, 24 KB
 
-struct alignas(1024) Ring32 {
-    char b[2][2][HALF32];
+struct alignas(1024) Planes {
+    char b[2][3][PLANE];  // [step & 1][h, m, l][rows of i, rows of j]
 };
 
-struct Split {
-    u32x4 h, m, l;
-};
+__device__ __forceinline__ int quad_swizzle(int a) { return ((a & 1) << 1) ^ ((a >> 1) & 1) * 3; }
 
-// 8 values to three times 8 bf16 (the upper halves of x, x - h, x - h - m)
-__device__ __forceinline__ Split split8(f32x4 a, f32x4 b) {
-    Split s;
+// 8 values to three times 8 bf16: the upper halves of x, x - h, x - h - m
+__device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&s)[3]) {
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        const float x = p < 2 ? a[2 * p] : b[2 * p - 4], y = p < 2 ? a[2 * p + 1] : b[2 * p - 3];
-        auto upper = [](float u, float v) __attribute__((always_inline)) {  // v's, u's upper halves
-            return __builtin_amdgcn_perm(__float_as_uint(v), __float_as_uint(u), 0x07060302u);
+        auto upper = [](float u, float w) __attribute__((always_inline)) {  // w's, u's upper halves
+            return __builtin_amdgcn_perm(__float_as_uint(w), __float_as_uint(u), 0x07060302u);
         };
         auto rest = [](float u) __attribute__((always_inline)) {
             return u - __uint_as_float(__float_as_uint(u) & 0xffff0000u);
         };
-        s.h[p] = upper(x, y);
-        const float x1 = rest(x), y1 = rest(y);
-        s.m[p] = upper(x1, y1);
-        s.l[p] = upper(rest(x1), rest(y1));
+        const float x = v[2 * p], y = v[2 * p + 1], x1 = rest(x), y1 = rest(y);
+        s[0][p] = upper(x, y);
+        s[1][p] = upper(x1, y1);
+        s[2][p] = upper(rest(x1), rest(y1));
     }
-    return s;
 }
 
-template <int NJ, int NF>
-__device__ __forceinline__ void products(f32x4 (&acc)[4][NF], int g0, const Split (&fi)[4], const Split (&fj)[NJ]) {
-    auto one = [&](auto pj, auto pi) __attribute__((always_inline)) {
+// 8 values of a row of k: two 16-byte pieces
+__device__ __forceinline__ void load_row(float (&v)[8], const char *base, uint32_t lo, uint32_t hi) {
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(base + lo), b = *reinterpret_cast<const f32x4 *>(base + hi);
 #pragma unroll
-        for (int f = 0; f < 4; ++f)
+    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+}
+// 8 values of a column: rows k0 .. k0 + 7, at most `last`
+__device__ __forceinline__ void load_col(float (&v)[8], const char *base, uint32_t col, int k0, uint32_t ld, int last) {
+    if (last >= 31) {
 #pragma unroll
-            for (int g = 0; g < NJ; ++g) acc[f][g0 + g] = Bf16::mma(pj(fj[g]), pi(fi[f]), acc[f][g0 + g]);
+        for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const float *>(base + e * (uint64_t)ld + (k0 * ld + col));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const float *>(base + (min(k0 + e, last) * ld + col));
+    }
+}
+
+// The loop of both kernels.  load(set): the next step's values (a thread's
+// pieces: two of i, one of j); put[k]: where in a plane piece k goes; start(n):
+// before step n (a tile's end, zeroed accumulators), false ends the loop.
+template <int NJ, class LOAD, class START>
+__device__ __forceinline__ void steps32(Planes &pl, f32x4 (&acc)[4][NJ], int nstep, const int (&put)[3], bool j_half,
+                                        int ri, int rj, int jstep0, int jstep1, LOAD load, START start) {
+    const int wj = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    float v[2][3][8];
+    auto write = [&](float (&x)[3][8], int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            if (k == 2 && !j_half) break;
+            u32x4 s[3];
+            split8(x[k], s);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(&pl.b[buf][p][put[k]]) = s[p];
+        }
     };
-    auto h = [](const Split &s) __attribute__((always_inline)) { return s.h; };
-    auto m = [](const Split &s) __attribute__((always_inline)) { return s.m; };
-    auto l = [](const Split &s) __attribute__((always_inline)) { return s.l; };
-    one(m, m);
-    one(l, h);
-    one(h, l);
-    one(m, h);
-    one(h, m);
-    one(h, h);
-}
-
-__device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-// the split belongs to the window it is written in: nothing else keeps the
-// compiler from moving it next to the products that use it
-template <int N>
-__device__ __forceinline__ void here(Split (&s)[N]) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) asm volatile("" : "+v"(s[k].h), "+v"(s[k].m), "+v"(s[k].l));
-}
-__device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-// the order of a window's reads and splits: DS LDS reads a fragment, those of
-// fragment k + 2 before the split of fragment k + 1
-template <int N, int DS>
-__device__ __forceinline__ void read_ahead() {
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * DS, 0);
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        __builtin_amdgcn_sched_group_barrier(0x002, 44, 0);
-        if (k + 2 < N) __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
+    auto lds_end = []() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        window_end();
+    };
+    if (nstep == 0) {
+        start(0);
+        return;
     }
+    load(v[0]);
+    if (nstep > 1) load(v[1]);
+    write(v[0], 0);
+    if (nstep > 2) load(v[0]);
+    lds_end();
+    if (wj) window_end();
+    u32x4 fi[4][3], fj[NJ][3];
+    auto step = [&](int n, int buf, float (&x)[3][8]) __attribute__((always_inline)) {
+        const char *b = &pl.b[buf][0][0];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) fi[f][p] = *reinterpret_cast<const u32x4 *>(b + p * PLANE + ri + 16 * f * KBY);
+#pragma unroll
+            for (int g = 0; g < NJ; ++g)
+                fj[g][p] = *reinterpret_cast<const u32x4 *>(b + p * PLANE + rj + (g >> 1) * jstep1 + (g & 1) * jstep0);
+        }
+        if (n + 1 < nstep) write(x, buf ^ 1);
+        if (n + 3 < nstep) load(x);
+        lds_end();
+        constexpr int PI[6] = {1, 0, 2, 0, 1, 0}, PJ[6] = {1, 2, 0, 1, 0, 0};  // smallest first
+#pragma unroll
+        for (int q = 0; q < 6; ++q)
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int g = 0; g < NJ; ++g) acc[f][g] = Bf16::mma(fj[g][PJ[q]], fi[f][PI[q]], acc[f][g]);
+        window_end();
+    };
+    for (int n = 0;; n += 2) {
+        if (!start(n)) break;
+        step(n, 0, v[1]);
+        if (!start(n + 1)) break;
+        step(n + 1, 1, v[0]);
+    }
+    if (!wj) window_end();  // the other half's last products
 }
 
-// rows of k: fragment row fr, both pieces of the lane
-__device__ __forceinline__ Split read_rows(const char *lo, const char *hi, int off) {
-    return split8(*reinterpret_cast<const f32x4 *>(lo + off), *reinterpret_cast<const f32x4 *>(hi + off));
-}
-
-// k_nt of f32: nk is steps of 128 bytes, bmax the last 16-byte piece of a row of B.
+// k_nt of f32: a tile has 128 rows of B; nk counts steps of 32 k's, bmax is the
+// last 16-byte piece of a row of B.  Accumulators as k_nt's, a wave's 64 columns.
 template <class EPI>
 __global__ __launch_bounds__(NT, 2) void k_nt32(NtArgs a, EPI epi) {
-    __shared__ Ring32 rg;
+    __shared__ Planes pl;
     __shared__ typename EPI::Shared sh;
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -122,202 +152,108 @@ __global__ __launch_bounds__(NT, 2) void k_nt32(NtArgs a, EPI epi) {
     const int t0 = slice * a.run, t1 = min(a.tiles, t0 + a.run);
     const int nstep = a.nk * (t1 - t0);
 
-    // ---- loads: wave w stages rows 32 w .. 32 w + 31 of both operands, 8 a piece
-    const int r0 = 32 * w + (lane >> 3), l4 = lane >> 4;
+    // pieces: rows tid / 4 and 128 more of i, tid / 4 of j, 32 bytes at 32 (tid & 3)
+    const int row = tid >> 2, c = tid & 3;
     const int ilast = (int)min<int64_t>(TILE - 1, a.m - 1 - i0);
-    int st = t0, sk = 0, staged = 0;
-    const char *pa = a.A + i0 * a.lda;
-    const uint32_t li = lds_addr(&rg.b[0][0][32 * w * KBY32]), lj = lds_addr(&rg.b[0][1][32 * w * KBY32]);
-    auto issue = [&]() __attribute__((always_inline)) {  // the next step, if there is one
-        if (staged >= nstep) return;
-        const int ko = sk * KBY32, left = a.bmax - ko;  // pieces past a row's last one repeat it
-        const int jlast = (int)min<int64_t>(TILE - 1, a.n - 1 - (int64_t)st * TILE);
-        const char *pb = a.B + (int64_t)st * TILE * a.ldb;
-        const uint32_t slot = (staged & 1) * 2 * HALF32;
-        // (offsets worked out here: kept, they would spill)
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const int vi = (int)__umul24(min(r0 + 8 * p, ilast), (int)a.lda) + 16 * ((lane & 7) ^ ((4 * (p & 1) + l4) & 7));
-            const int vj = (int)__umul24(min(r0 + 8 * p, jlast), (int)a.ldb) + min(16 * ((lane & 7) ^ (2 * p + (l4 & 1))), left);
-            dma16(pa + ko, vi, li + slot + 1024 * p);
-            dma16(pb + ko, vj, lj + slot + 1024 * p);
-        }
-        ++staged;
+    const uint32_t vi0 = min(row, ilast) * (uint32_t)a.lda + 32 * c, vi1 = min(row + 128, ilast) * (uint32_t)a.lda + 32 * c;
+    const int ci = 16 * (c ^ quad_swizzle((row >> 2) & 3)), cj = 16 * (c ^ quad_swizzle((row >> 3) & 3));
+    const int put[3] = {row * KBY + ci, (row + 128) * KBY + ci, (TILE + row) * KBY + cj};
+    int st = t0, sk = 0;  // of the next load
+    auto load = [&](float (&v)[3][8]) __attribute__((always_inline)) {
+        const int ko = sk * 128;
+        const char *pa = a.A + i0 * a.lda + ko, *pb = a.B + (int64_t)st * COLS32 * a.ldb;
+        const int jlast = (int)min<int64_t>(COLS32 - 1, a.n - 1 - (int64_t)st * COLS32);
+        const uint32_t vj = min(row, jlast) * (uint32_t)a.ldb;
+        load_row(v[0], pa, vi0, vi0 + 16);
+        load_row(v[1], pa, vi1, vi1 + 16);
+        load_row(v[2], pb, vj + min(ko + 32 * c, a.bmax), vj + min(ko + 32 * c + 16, a.bmax));
         if (++sk == a.nk) {
             sk = 0;
             ++st;
         }
     };
-
-    f32x4 acc[4][8];
-    Split fi[4], fj[4];
-    const int pc = 16 * (fk ^ (fr >> 1));
-    const char *ri = &rg.b[0][0][(64 * wi + fr) * KBY32];
-    const char *rj = &rg.b[0][1][(128 * wj + 8 * (fr >> 2) + (fr & 3)) * KBY32];
-    auto read_j = [&](int so, int g0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            fj[g] = read_rows(rj + pc, rj + (pc ^ 64), so + (32 * ((g0 + g) >> 1) + 4 * (g & 1)) * KBY32);
-    };
+    f32x4 acc[4][4];
     epi.init(sh, i0 + 64 * wi, lane);
-    issue();
-    vm_wait();
-    window_end();
-    if (wj) {
-        issue();
-        window_end();
-    }
     int k = 0, t = t0;
-    for (int n = 0;; ++n) {
+    auto start = [&](int n) __attribute__((always_inline)) {
         if (k == 0) {
-            if (n) epi.tile(sh, acc, (int64_t)(t - 1) * TILE + 128 * wj, lane);
-            if (n == nstep) break;
+            if (n) epi.tile(sh, acc, (int64_t)(t - 1) * COLS32 + 64 * wj, lane);
+            if (n == nstep) return false;
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int g = 0; g < 8; ++g) acc[f][g] = (f32x4)(0.f);
+                for (int g = 0; g < 4; ++g) acc[f][g] = (f32x4)(0.f);
         }
-        if (!wj) issue();
-        const int so = (n & 1) * 2 * HALF32;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) fi[f] = read_rows(ri + pc, ri + (pc ^ 64), so + 16 * f * KBY32);
-        read_j(so, 0);
-        here(fi);
-        here(fj);
-        read_ahead<8, 2>();
-        lds_wait();
-        window_end();
-        products<4>(acc, 0, fi, fj);
-        window_end();
-        read_j(so, 4);
-        here(fj);
-        read_ahead<4, 2>();
-        lds_wait();
-        if (wj) vm_wait();
-        window_end();
-        if (wj) issue();
-        products<4>(acc, 4, fi, fj);
-        if (!wj) vm_wait();
-        window_end();
         if (++k == a.nk) {
             k = 0;
             ++t;
         }
-    }
-    if (!wj) window_end();  // the other half's last products, then its last tile
-    vm_wait();
+        return true;
+    };
+    const int q = fk ^ quad_swizzle(fr >> 2);
+    // row of fragment g: 32 (g >> 1) + 4 (g & 1) + 8 (fr >> 2) + (fr & 3)
+    steps32<4>(pl, acc, nstep, put, true, (64 * wi + fr) * KBY + 16 * q,
+               (TILE + 64 * wj + 8 * (fr >> 2) + (fr & 3)) * KBY + 16 * q, 4 * KBY, 32 * KBY, load, start);
     epi.finish(sh, i0 + 64 * wi, slice * 2 + wj, lane);
 }
 
-// kn_tile of f32.  NF 8: j in two halves; 4, 2: in one.
-template <int NF, bool A_T, class EPI>
-__device__ __forceinline__ void kn32_tile(Ring32 &rg, const KnArgs &a, const EPI &epi, int64_t m0, int64_t n0, int z) {
-    constexpr int NJ = NF == 8 ? 4 : NF;
+// kn_tile of f32: 256 rows and 32 NJ columns, accumulators as kn_tile's, a
+// wave's 16 NJ columns.
+template <int NJ, bool A_T, class EPI>
+__device__ __forceinline__ void kn32_tile(Planes &pl, const KnArgs &a, const EPI &epi, int64_t m0, int64_t n0, int z) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = w & 3, wj = w >> 2;
     const int fr = lane & 15, fk = lane >> 4;
     const int s0 = z * a.steps, s1 = min(a.steps_all, s0 + a.steps), nstep = max(0, s1 - s0);
 
-    // ---- loads.  [k][256]: wave w stages rows 4 w .. 4 w + 3; [256][k]: as k_nt32
-    const int col = 64 * ((lane >> 2) ^ (w & 3)) + 16 * (lane & 3);
-    const int cj = (int)min<int64_t>(col, a.ldb - 16 - 4 * n0);
-    int vi[4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        if constexpr (A_T) vi[p] = (4 * w + p) * (int)a.lda + col;
-        else vi[p] = (32 * w + 8 * p + (lane >> 3)) * (int)a.lda + 16 * ((lane & 7) ^ ((4 * (p & 1) + fk) & 7));
-    }
-    const int64_t astep = A_T ? 32 * a.lda : KBY32, bstep = 32 * a.ldb;
-    const char *pa = a.A + (A_T ? 4 * m0 : m0 * a.lda) + s0 * astep;
-    const char *pb = a.B + 4 * n0 + s0 * bstep;
-    const uint32_t li = lds_addr(&rg.b[0][0][4096 * w]), lj = lds_addr(&rg.b[0][1][4096 * w]);
-    int staged = 0;
-    auto issue = [&]() __attribute__((always_inline)) {
-        if (staged >= nstep) return;
-        const int last = (int)min<int64_t>(31, a.k - 1 - (int64_t)(s0 + staged) * 32);
-        const uint32_t slot = (staged & 1) * 2 * HALF32;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            dma16(pa, vi[p], li + slot + 1024 * p);
-            dma16(pb, min(4 * w + p, last) * (int)a.ldb + cj, lj + slot + 1024 * p);
+    // pieces of i: as k_nt32, or column tid & 255, rows 8 (tid / 256) and 16
+    // more; of j: column tid % (32 NJ), rows 8 (tid / (32 NJ))
+    const int ri = A_T ? tid & 255 : tid >> 2, ki = A_T ? tid >> 8 : tid & 3;
+    const int rj = tid % (32 * NJ), kj = tid / (32 * NJ);
+    auto at = [](int r, int c) __attribute__((always_inline)) { return r * KBY + 16 * (c ^ quad_swizzle((r >> 2) & 3)); };
+    const int put[3] = {at(ri, ki), A_T ? at(ri, ki + 2) : at(ri + 128, ki), TILE * KBY + at(rj, kj & 3)};
+    const uint32_t vj = (uint32_t)min<int64_t>(4 * rj, a.ldb - 4 - 4 * n0);
+    const char *pa = a.A + (A_T ? 4 * m0 + (int64_t)s0 * 32 * a.lda : m0 * a.lda + (int64_t)s0 * 128);
+    const char *pb = a.B + 4 * n0 + (int64_t)s0 * 32 * a.ldb;
+    int sk = s0;
+    auto load = [&](float (&v)[3][8]) __attribute__((always_inline)) {
+        const int last = (int)min<int64_t>(31, a.k - 1 - (int64_t)sk * 32);
+        if constexpr (A_T) {  // whole tiles exist
+            load_col(v[0], pa, 4 * ri, 8 * ki, (uint32_t)a.lda, 31);
+            load_col(v[1], pa, 4 * ri, 8 * ki + 16, (uint32_t)a.lda, 31);
+        } else {
+            const uint32_t o = ri * (uint32_t)a.lda + 32 * ki;
+            load_row(v[0], pa, o, o + 16);
+            load_row(v[1], pa, o + 128 * (uint32_t)a.lda, o + 128 * (uint32_t)a.lda + 16);
         }
-        pa += astep;
-        pb += bstep;
-        ++staged;
+        if (NJ == 4 || tid < 128 * NJ) load_col(v[2], pb, vj, 8 * kj, (uint32_t)a.ldb, last);
+        ++sk;
+        pa += A_T ? 32 * a.lda : 128;
+        pb += 32 * a.ldb;
     };
-
-    f32x4 acc[4][NF];
+    f32x4 acc[4][NJ];
 #pragma unroll
     for (int f = 0; f < 4; ++f)
 #pragma unroll
-        for (int g = 0; g < NF; ++g) acc[f][g] = (f32x4)(0.f);
-    Split fi[4], fj[NJ];
-    const int pc = 16 * (fk ^ (fr >> 1));
-    const char *ri = &rg.b[0][0][(64 * wi + fr) * KBY32];
-    // columns: rows 4 fk .. + 3 and 16 on, 16-column slot s
-    auto cols = [&](const char *half, int s) __attribute__((always_inline)) {
-        const float *p = reinterpret_cast<const float *>(half + 4096 * fk + 64 * (s ^ fk)) + fr;
-        const f32x4 x = {p[0], p[256], p[512], p[768]}, y = {p[4096], p[4352], p[4608], p[4864]};
-        return split8(x, y);
-    };
-    auto read_j = [&](int so, int g0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int g = 0; g < NJ; ++g) fj[g] = cols(&rg.b[0][1][0] + so, NF * wj + g0 + g);
-    };
-    if (nstep > 0) {
-        issue();
-        vm_wait();
-        window_end();
-        if (wj) {
-            issue();
-            window_end();
-        }
-        for (int n = 0; n < nstep; ++n) {
-            if (!wj) issue();
-            const int so = (n & 1) * 2 * HALF32;
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-                if constexpr (A_T) fi[f] = cols(&rg.b[0][0][0] + so, 4 * wi + f);
-                else fi[f] = read_rows(ri + pc, ri + (pc ^ 64), so + 16 * f * KBY32);
-            }
-            read_j(so, 0);
-            here(fi);
-            here(fj);
-            read_ahead<4 + NJ, 4>();
-            lds_wait();
-            window_end();
-            products<NJ>(acc, 0, fi, fj);
-            window_end();
-            if constexpr (NF == 8) {
-                read_j(so, 4);
-                here(fj);
-                read_ahead<NJ, 4>();
-            }
-            lds_wait();
-            if (wj) vm_wait();
-            window_end();
-            if (wj) issue();
-            if constexpr (NF == 8) products<NJ>(acc, 4, fi, fj);
-            if (!wj) vm_wait();
-            window_end();
-        }
-        if (!wj) window_end();
-        vm_wait();
-    }
-    epi(acc, m0 + 64 * wi, n0 + 16 * NF * wj, lane, z);
+        for (int g = 0; g < NJ; ++g) acc[f][g] = (f32x4)(0.f);
+    auto start = [&](int n) __attribute__((always_inline)) { return n < nstep; };
+    const int q = 16 * (fk ^ quad_swizzle(fr >> 2));
+    steps32<NJ>(pl, acc, nstep, put, NJ == 4 || tid < 128 * NJ, (64 * wi + fr) * KBY + q,
+                (TILE + 16 * NJ * wj + fr) * KBY + q, 16 * KBY, 32 * KBY, load, start);
+    epi(acc, m0 + 64 * wi, n0 + 16 * NJ * wj, lane, z);
 }
 
-template <int NF, class E1, class E2>
+template <int NJ, class E1, class E2>
 __global__ __launch_bounds__(NT, 2) void k_kn2_32(KnArgs a1, E1 e1, KnGrid g1, KnArgs a2, E2 e2, KnGrid g2) {
-    __shared__ Ring32 rg;
+    __shared__ Planes pl;
     const int b = (int)blockIdx.x, n1 = g1.blocks();
     if (b < n1) {
         const int v = xcd_range(b, n1), r = v / g1.cols;
-        kn32_tile<NF, false>(rg, a1, e1, (int64_t)(r % g1.rows) * TILE, (int64_t)(v % g1.cols) * 32 * NF, r / g1.rows);
+        kn32_tile<NJ, false>(pl, a1, e1, (int64_t)(r % g1.rows) * TILE, (int64_t)(v % g1.cols) * 32 * NJ, r / g1.rows);
     } else {
         const int v = xcd_range(b - n1, g2.blocks()), r = v / g2.cols;
-        kn32_tile<NF, true>(rg, a2, e2, (int64_t)(r % g2.rows) * TILE, (int64_t)(v % g2.cols) * 32 * NF, r / g2.rows);
+        kn32_tile<NJ, true>(pl, a2, e2, (int64_t)(r % g2.rows) * TILE, (int64_t)(v % g2.cols) * 32 * NJ, r / g2.rows);
     }
 }
 

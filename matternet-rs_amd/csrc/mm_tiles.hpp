@@ -151,9 +151,9 @@ struct NtArgs {
 // How many runs the tiles of B are cut into for `panels` panels: the cut with
 // the least rounds of 256 blocks, a run costing its tiles and 0.3 for filling
 // the ring.
-inline void plan_runs(NtArgs &a) {
+inline void plan_runs(NtArgs &a, int cols = TILE) {  // cols: rows of B in a tile
     a.panels = (int)((a.m + TILE - 1) / TILE);
-    a.tiles = (int)((a.n + TILE - 1) / TILE);
+    a.tiles = (int)((a.n + cols - 1) / cols);
     double best = 1e300;
     for (int run = 1; run <= a.tiles; run = run < 32 ? run + 1 : run + run / 16) {
         const int64_t s = (a.tiles + run - 1) / run, blocks = s * a.panels;

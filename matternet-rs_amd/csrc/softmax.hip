@@ -230,12 +230,8 @@ __global__ __launch_bounds__(256) void k_prep(Pack q, Pack c, Rows r) {
 // target's left out; joined over the lanes and written per run of tiles and
 // half of the columns.  An element costs a max, an fma, an exp and an add: for
 // 768 columns of operands about a seventh of its time on the matrix pipe.
-template <bool F32>
 struct StatsEpi {
-    // f32's products leave no registers for the state: it lies in LDS
-    struct Shared {
-        float2 s[F32 ? 4 : 1][F32 ? mm::NT : 1];
-    };
+    struct Shared {};
     static constexpr bool FETCH = false;
     static constexpr int STORES = 0, STAGE = 0;
     static constexpr bool counted = false;
@@ -246,74 +242,59 @@ struct StatsEpi {
     float scale2;  // scale log2(e)
     int at[4];
     float m2[4], sum[4];
-    int64_t i0_;
-    __device__ __forceinline__ void targets_of(int (&a)[4], int lane) const {
+    int64_t row0;
+    __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
+        row0 = i0 + (lane & 15);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            const int64_t i = i0_ + (lane & 15) + 16 * f, x = i < t ? targets[i] : -1;
-            a[f] = x >= c_offset && x - c_offset < v ? (int)(x - c_offset) : -1;
-        }
-    }
-    __device__ __forceinline__ void init(Shared &sh, int64_t i0, int lane) {
-        i0_ = i0;
-        if constexpr (!F32) targets_of(at, lane);
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-            if constexpr (F32) sh.s[f][threadIdx.x] = make_float2(-__builtin_inff(), 0.f);
-            else m2[f] = -__builtin_inff(), sum[f] = 0.f;
+            const int64_t i = row0 + 16 * f, x = i < t ? targets[i] : -1;
+            at[f] = x >= c_offset && x - c_offset < v ? (int)(x - c_offset) : -1;
+            m2[f] = -__builtin_inff();
+            sum[f] = 0.f;
         }
     }
     __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
-    __device__ __forceinline__ void tile(Shared &sh, mm::f32x4 (&acc)[4][8], int64_t j0, int lane) {
+    template <int G>
+    __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][G], int64_t j0, int lane) {
         const int jw = (int)j0, jl = jw + 8 * (lane >> 4);
-        int a[4];
-        if constexpr (F32) targets_of(a, lane);
-        else
+        bool hit = jw + 16 * G > v;
 #pragma unroll
-            for (int f = 0; f < 4; ++f) a[f] = at[f];
-        bool hit = jw + 128 > v;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(a[f] - jw) < 128u;
+        for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 16u * G;
         if (__ballot(hit)) {
 #pragma unroll
-            for (int g = 0; g < 8; ++g)
+            for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int f = 0; f < 4; ++f) {
                         const int j = jl + 32 * (g >> 1) + 4 * (g & 1) + r;
-                        acc[f][g][r] = j >= v || j == a[f] ? -__builtin_inff() : acc[f][g][r];
+                        acc[f][g][r] = j >= v || j == at[f] ? -__builtin_inff() : acc[f][g][r];
                     }
         }
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            float2 old;
-            if constexpr (F32) old = sh.s[f][threadIdx.x];
-            else old = make_float2(m2[f], sum[f]);
             float top = acc[f][0][0];
 #pragma unroll
-            for (int g = 0; g < 8; ++g)
+            for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[f][g][r]);
-            const float m = fmaxf(old.x, top * scale2);
+            const float m = fmaxf(m2[f], top * scale2);
             const float mz = m == -__builtin_inff() ? 0.f : m;
             float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-            for (int g = 0; g < 8; g += 2)
+            for (int g = 0; g < G; g += 2)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     s0 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g][r], scale2, -mz));
                     s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][g + 1][r], scale2, -mz));
                 }
-            const float s = old.y * __builtin_amdgcn_exp2f(old.x - mz) + (s0 + s1);
-            if constexpr (F32) sh.s[f][threadIdx.x] = make_float2(m, s);
-            else m2[f] = m, sum[f] = s;
+            sum[f] = sum[f] * __builtin_amdgcn_exp2f(m2[f] - mz) + (s0 + s1);
+            m2[f] = m;
         }
     }
-    __device__ __forceinline__ void finish(Shared &sh, int64_t, int piece, int lane) {
+    __device__ __forceinline__ void finish(Shared &, int64_t, int piece, int lane) {
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            if constexpr (F32) m2[f] = sh.s[f][threadIdx.x].x, sum[f] = sh.s[f][threadIdx.x].y;
 #pragma unroll
             for (int o = 16; o <= 32; o <<= 1) {
                 const float mo = __shfl_xor(m2[f], o), so = __shfl_xor(sum[f], o);
@@ -321,7 +302,7 @@ struct StatsEpi {
                 sum[f] = sum[f] * __builtin_amdgcn_exp2f(m2[f] - mz) + so * __builtin_amdgcn_exp2f(mo - mz);
                 m2[f] = m;
             }
-            const int64_t i = i0_ + (lane & 15) + 16 * f;
+            const int64_t i = row0 + 16 * f;
             if (lane < 16 && i < t) part[piece * t + i] = make_float2(m2[f], sum[f]);
         }
     }
@@ -485,10 +466,6 @@ struct DlogitsEpi {
     int64_t i0_;
     __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
         i0_ = i0;
-        if constexpr (!F32) rows_of(lane);
-    }
-    // f32's products leave no registers for these: read again for every tile
-    __device__ __forceinline__ void rows_of(int lane) {
         any = false;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
@@ -504,20 +481,20 @@ struct DlogitsEpi {
         any = __ballot(any) != 0;
     }
     __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
-    __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][8], int64_t j0, int lane) {
+    template <int G>
+    __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][G], int64_t j0, int lane) {
         constexpr int SZ = F32 ? 4 : 2;
-        if constexpr (F32) rows_of(lane);
         const int jw = (int)j0, jl = 8 * (lane >> 4);
-        bool hit = jw + 128 > v || !any;
+        bool hit = jw + 16 * G > v || !any;
 #pragma unroll
-        for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 128u;
+        for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 16u * G;
         const bool slow = __ballot(hit) != 0;
         char *base = D + SZ * (i0_ * ldd + j0);
         const int to = SZ * ((lane & 15) * (int)ldd + jl);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
 #pragma unroll
-            for (int g = 0; g < 8; g += 2) {
+            for (int g = 0; g < G; g += 2) {
                 float x[8];
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
@@ -632,6 +609,7 @@ struct Plan {
     int size;           // bytes of a value
     bool pack_c;        // C's rows start off 16-byte borders
     int64_t ldc;        // bytes of a row of C as the products read it
+    int tile;           // items of a tile of logits
     mm::NtArgs nt;      // the whole table's logits
     mm::FewArgs few;    // the same for few queries; blocks 0: not so
     bool few_q;         // on the queries as they are
@@ -655,6 +633,7 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
     p.pack_c = (d * p.size) % 16 != 0;
     p.ldc = (int64_t)(p.pack_c ? p.kp : d) * p.size;
     p.tp = (t + mm::TILE - 1) / mm::TILE * mm::TILE;
+    p.tile = f32 ? mm::COLS32 : mm::TILE;
     p.nt.lda = (int64_t)p.kp * p.size;
     p.nt.ldb = p.ldc;
     p.nt.m = t;
@@ -673,7 +652,7 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         p.few.ldq = p.few.ldb = p.ldc;
         p.few.qbytes = (int)p.ldc;
         if (t > (f32 ? 32 : 64) || !mm::plan_few(p.few)) p.few.blocks = 0;
-        mm::plan_runs(p.nt);
+        mm::plan_runs(p.nt, p.tile);
         p.part = take((size_t)std::max(p.nt.slices * 2, p.few.blocks) * t * 8);
     } else {
         // Pieces whose D stays below 256 MB (the last-level cache; 128, 512 and
@@ -692,14 +671,14 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         // dQ's runs of k: the cut with the least time for the blocks of both
         // products on 256 processors, dQ's first, in steps: a block of dQ
         // costs its run and 20 for its part of the sum (256 KB to memory), one
-        // of dC t / 32 and 10 (f32, whose steps take four times as long: 5 and 3).  Free processors take the next block: dC's done
+        // of dC t / 32 and 10 (f32, whose steps take twice as long: 6 and 4).  Free processors take the next block: dC's done
         // by a time are counted from the two times at which dQ's blocks end.
-        p.nf = d > 128 ? 8 : d > 64 ? 4 : 2;
+        p.nf = f32 ? (d > 64 ? 4 : 2) : d > 128 ? 8 : d > 64 ? 4 : 2;
         const int64_t cols = (d + 32 * p.nf - 1) / (32 * p.nf), tiles = panels * cols;
-        const int64_t steps = p.vc / 32, nc = p.vc / mm::TILE * cols, b = t / 32 + (f32 ? 3 : 10);
+        const int64_t steps = p.vc / 32, nc = p.vc / mm::TILE * cols, b = t / 32 + (f32 ? 4 : 10);
         int64_t best = INT64_MAX;
         for (int64_t s = 1; s <= std::min<int64_t>(steps / 4 + 1, std::max<int64_t>(1, 512 / tiles)); ++s) {
-            const int64_t a = (steps + s - 1) / s + (f32 ? 5 : 20), nq = tiles * s, full = nq / 256 * a, more = nq % 256;
+            const int64_t a = (steps + s - 1) / s + (f32 ? 6 : 20), nq = tiles * s, full = nq / 256 * a, more = nq % 256;
             int64_t end = full + (more ? a : 0);
             for (int64_t k = (nc + 255) / 256;; ++k) {
                 const int64_t e1 = full + k * b, e2 = std::max<int64_t>(0, e1 - full - a) / b;
@@ -801,7 +780,7 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
     } else {
         const mm::NtArgs a = nt_args(p, C, w);
         pieces = (int64_t)a.slices * 2;
-        StatsEpi<F32> epi = {};
+        StatsEpi epi = {};
         epi.part = part;
         epi.targets = targets;
         epi.c_offset = c_offset;
@@ -866,7 +845,7 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         mm::NtArgs a = nt_args(p, C, w);
         a.B += j0 * a.ldb;
         a.n = vn;
-        mm::plan_runs(a);
+        mm::plan_runs(a, p.tile);
         DlogitsEpi<F32> epi = {};
         epi.D = w + p.D;
         epi.ldd = p.ldd;
@@ -903,9 +882,9 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
             else
                 hipLaunchKernelGGL((mm::k_kn2<n, PartEpi, GradEpi<F32>>), grid, dim3(mm::NT), 0, s, gq, pe, nq, gc, ge, nc);
         };
-        if (p.nf == 8) go(std::integral_constant<int, 8>());
-        else if (p.nf == 4) go(std::integral_constant<int, 4>());
-        else go(std::integral_constant<int, 2>());
+        if (p.nf == 4) go(std::integral_constant<int, 4>());
+        else if (p.nf == 2) go(std::integral_constant<int, 2>());
+        else if constexpr (!F32) go(std::integral_constant<int, 8>());
         MN_KCHECK(s, "k_kn2");
     }
     if (dQ) {
