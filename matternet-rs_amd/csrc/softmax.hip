@@ -195,7 +195,9 @@ __device__ __forceinline__ void rows(const Rows &p, int block) {
     if (i >= p.tp) return;
     const float top = p.grad_n == 1 ? fabsf(p.grad[0]) : p.gs[1];
     if (i == 0) p.gs[0] = (p.grad_scale ? top * p.grad_scale[0] : top) * p.scale;
-    Row r = {0.f, 0.f, 0.f, 0.f};
+    // no part (or only there to fill a tile, where the last query's logits of any
+    // size are computed again): exp(z - inf) = 0
+    Row r = {0.f, __builtin_inff(), 0.f, 0.f};
     int32_t a = -1;
     if (i < p.t && p.targets[i] >= 0) {
         const int64_t tl = p.targets[i] - p.c_offset;
@@ -451,7 +453,7 @@ template <bool F32>
 struct DlogitsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;
-    static constexpr int STORES = F32 ? 32 : 16, STAGE = 0;
+    static constexpr int STORES = 16, STAGE = 0;  // (k_nt; k_nt32 counts nothing)
     static constexpr bool counted = true;
     char *D;
     int64_t ldd;
@@ -462,11 +464,9 @@ struct DlogitsEpi {
     float scale2;
     int at[4];
     float rel[4], lse2[4], dt[4];
-    bool any;
     int64_t i0_;
     __device__ __forceinline__ void init(Shared &, int64_t i0, int lane) {
         i0_ = i0;
-        any = false;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             const int64_t i = i0_ + 16 * f + (lane & 15);
@@ -476,16 +476,14 @@ struct DlogitsEpi {
             dt[f] = r.dt;
             const int64_t a = at_[i] - j_first;
             at[f] = at_[i] >= 0 && a >= 0 && a < v ? (int)a : -1;
-            any = any || r.rel != 0.f;
         }
-        any = __ballot(any) != 0;
     }
     __device__ __forceinline__ void fetch(Shared &, int64_t, int, int) {}
     template <int G>
     __device__ __forceinline__ void tile(Shared &, mm::f32x4 (&acc)[4][G], int64_t j0, int lane) {
         constexpr int SZ = F32 ? 4 : 2;
         const int jw = (int)j0, jl = 8 * (lane >> 4);
-        bool hit = jw + 16 * G > v || !any;
+        bool hit = jw + 16 * G > v;
 #pragma unroll
         for (int f = 0; f < 4; ++f) hit = hit || (unsigned)(at[f] - jw) < 16u * G;
         const bool slow = __ballot(hit) != 0;
@@ -504,7 +502,7 @@ struct DlogitsEpi {
                     for (int q = 0; q < 8; ++q) {
                         const int j = jw + jl + 16 * g + q;
                         const float y = j == at[f] ? dt[f] : x[q];
-                        x[q] = j >= v || !any ? 0.f : y;
+                        x[q] = j >= v ? 0.f : y;
                     }
                 }
                 const int off = to + SZ * (16 * f * (int)ldd + 16 * g);

@@ -136,6 +136,30 @@ def test_gradient_against_differences():
         assert abs(float(diff) - float((dc * p).sum())) <= h * h / 6 * (2 * 1 * 3) ** 3 + 2e-5 / h
 
 
+@pytest.mark.parametrize("t,v,d", [(37, 300, 40), (100, 700, 64), (261, 1030, 20)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_logits(t, v, d, dtype):
+    """Logits of several hundred, the last query's largest: exp of them, unlike
+    exp of their distance to the log-sum-exp, is infinite.  (Terms below 2^-126
+    may be flushed: n of them, times at most scale and 4.)"""
+    import surfface_hip as S
+    q, c, at = data(t, v, d, torch.float32, 31)
+    q, at[-1] = q.abs() + 0.2, v - 1
+    c[: v // 2] = c[: v // 2].abs()
+    q[-1] *= 4
+    q, c = q.to(dtype), c.to(dtype)
+    qg, cg = q.cuda().requires_grad_(), c.cuda().requires_grad_()
+    loss = S.softmax_loss(qg, cg, at.cuda(), scale=60.0)
+    dq, dc = torch.autograd.grad(loss, (qg, cg))
+    w_loss, w_dq, w_dc, s_dq, s_dc, delta = formula(q, c, at, 60.0)
+    assert float((60 * q[-1].double() @ c.double().T).max()) > 300
+    n = int((at >= 0).sum())
+    close(loss.detach(), w_loss.sum() / n, torch.tensor(2 * delta + (t + 4) * U * float(w_loss.sum()) / n), "loss")
+    b = B if dtype == torch.bfloat16 else 0.0
+    for got, want, mag, k in ((dq, w_dq, s_dq, v), (dc, w_dc, s_dc, t)):
+        close(got, want, (2 * delta + (6 * k + 64) * U + b) * mag + (b or U) * want.abs() + k * 240 * 2.0 ** -126, "gradient")
+
+
 def test_small_losses_keep_their_precision():
     """Targets whose probability is nearly 1: loss and gradients relative to
     themselves, not to the logits: 1 - p = sum exp(z_j - z_t) is off by the
