@@ -312,9 +312,13 @@ struct StatsEpi {
 
 // loss of a row from (rest, zt); -inf for zt: no target in any range (loss +inf)
 __device__ __forceinline__ float row_loss(float rest, float zt) {
+    if (zt != zt) return zt;
     if (rest == -__builtin_inff()) return zt == rest ? __builtin_inff() : 0.f;
     return zt == -__builtin_inff() ? __builtin_inff() : softplus(rest - zt);
 }
+
+// maximum, NaN if either is
+__device__ __forceinline__ float fmax_nan(float x, float y) { return x != x || x > y ? x : y; }
 
 template <class F>
 __device__ __forceinline__ float block_fold(float x, float *sh, F f) {
@@ -374,7 +378,7 @@ __global__ __launch_bounds__(256) void k_join(const float2 *__restrict__ part, c
         else
             sum += p.y;  // nothing yet, or a NaN
         top = m;
-        if (zts) z = fmaxf(z, zts[k * t + i]);
+        if (zts) z = fmax_nan(z, zts[k * t + i]);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(256) void k_join(const float2 *__restrict__ part, c
         else
             sum += s2;
         top = m;
-        z = fmaxf(z, __shfl_xor(z, o));
+        z = fmax_nan(z, __shfl_xor(z, o));
     }
     if (lane == 0) {
         const float r = sum == 0.f ? -__builtin_inff() : (top == -__builtin_inff() ? sum : (top + log2f(sum)) * kLn2);

@@ -250,6 +250,23 @@ def test_row_ranges_of_a_table_join(dtype):
         qd, cd, ad, st.rest, st.target, one, 6.0, grad_scale=st.share)[1])
 
 
+def test_nan_in_the_target_s_row_survives_the_join():
+    """A NaN in an item is in no other item's logit: the row's rest is finite, its loss NaN."""
+    import surfface_hip as S
+    q, c, at = data(9, 80, 12, torch.float32, 21, ignore=False)
+    at[:] = torch.arange(9) * 8
+    c[at[4], 5] = float("nan")
+    qd, cd, ad = q.cuda(), c.cuda(), at.cuda()
+    parts = [S.softmax_stats(qd, cd[a:b], ad, 2.0, c_offset=a) for a, b in ((0, 40), (40, 80))]
+    st = S.softmax_merge(torch.stack([p.rest for p in parts]), torch.stack([p.target for p in parts]), ad)
+    for x in (st, S.softmax_stats(qd, cd, ad, 2.0)):
+        assert torch.isfinite(x.rest[4]) and torch.isnan(x.target[4]) and torch.isnan(x.loss).all() and torch.isnan(x.mean)
+    one = qd.clone()
+    one[3] = float("nan")
+    alone = S.softmax_stats(one, cd[:1], torch.zeros(9, dtype=torch.int64).cuda())
+    assert torch.isnan(alone.loss[3]) and not alone.loss[:3].any()
+
+
 def test_same_target_many_times_and_int32_targets():
     import surfface_hip as S
     q, c, at = data(200, 90, 24, torch.float32, 13, ignore=False)
