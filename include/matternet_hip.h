@@ -656,7 +656,7 @@ int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const float *scale, i
                           int32_t d, void *X, int32_t x_type, void *stream);
 /* Y [m][n] (MN_F32, or rounded to MN_BF16) = (sum_k q_ik c_jk) q_scale[i]
  * c_scale[j]: the sum exact, then rounded to f32 and multiplied in that order.
- * d <= 131071.  What lies behind column d of a row of codes has no effect. */
+ * d <= 131071, strides <= 2^23.  What lies behind column d of a row of codes has no effect. */
 int mn_scores_i8_workspace(int64_t m, int32_t d, size_t *bytes);
 int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, const int8_t *C,
                  int64_t ldc, const float *c_scale, int64_t n, int32_t d, void *Y, int32_t y_type,

@@ -318,8 +318,8 @@ extern "C" int mn_quantize_rows_i8(const void *X, int32_t x_type, int64_t n, int
                                    int8_t *codes, int64_t ld, float *scale, void *stream) {
     using namespace mn::i8;
     mn::clear_error();
-    MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX, MN_EINVAL,
-               "mn_quantize_rows_i8: n >= 0, d >= 1, ld >= d and a multiple of 16 needed");
+    MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX - 4096, MN_EINVAL,
+               "mn_quantize_rows_i8: n >= 0, d >= 1, ld >= d, a multiple of 16 and < 2^31 - 4096 needed");
     MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 256 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
                "mn_quantize_rows_i8: n < 2^31 - 1 rows and n d < 2^40 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_quantize_rows_i8: MN_F32 or MN_BF16");
@@ -337,8 +337,8 @@ extern "C" int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const floa
                                      int32_t d, void *X, int32_t x_type, void *stream) {
     using namespace mn::i8;
     mn::clear_error();
-    MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX, MN_EINVAL,
-               "mn_dequantize_rows_i8: n >= 0, d >= 1, ld >= d and a multiple of 16 needed");
+    MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX - 4096, MN_EINVAL,
+               "mn_dequantize_rows_i8: n >= 0, d >= 1, ld >= d, a multiple of 16 and < 2^31 - 4096 needed");
     MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 256 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
                "mn_dequantize_rows_i8: n < 2^31 - 1 rows and n d < 2^40 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_dequantize_rows_i8: MN_F32 or MN_BF16");
@@ -382,6 +382,8 @@ extern "C" int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, 
     MN_REQUIRE(d <= 131071, MN_ENOTSUP, "mn_scores_i8: d > 131071 (an int32 sum could overflow)");
     MN_REQUIRE(ldq >= d && ldc >= d && ldq % 16 == 0 && ldc % 16 == 0, MN_EINVAL,
                "mn_scores_i8: row strides need to be >= d and multiples of 16");
+    MN_REQUIRE(ldq <= 1 << 23 && ldc <= 1 << 23, MN_ENOTSUP,  // offsets in a tile of 256 rows are 32 bits
+               "mn_scores_i8: row strides above 2^23 bytes");
     MN_REQUIRE(y_type == MN_F32 || y_type == MN_BF16, MN_ENOTSUP, "mn_scores_i8: MN_F32 or MN_BF16 scores");
     if (m == 0 || n == 0) return MN_OK;
     MN_REQUIRE(Q && q_scale && C && c_scale && Y, MN_EINVAL, "mn_scores_i8: NULL pointer");

@@ -19,7 +19,7 @@ def test_quantize_and_dequantize_refusals():
     dq = lambda codes=A, ld=32, s=A, n=4, d=20, X=A, ty=0: L.mn_dequantize_rows_i8(codes, ld, s, n, d, X, ty, None)
     for f in (q, dq):
         assert f(n=-1) == E.MN_EINVAL and f(d=0) == E.MN_EINVAL and f(ld=16) == E.MN_EINVAL
-        assert f(ld=40) == E.MN_EINVAL and f(ld=1 << 32) == E.MN_EINVAL
+        assert f(ld=40) == E.MN_EINVAL and f(ld=1 << 32) == E.MN_EINVAL and f(ld=2 ** 31 - 16) == E.MN_EINVAL
         assert f(ty=1) == E.MN_ENOTSUP and f(ty=7) == E.MN_ENOTSUP
         assert f(X=None) == E.MN_EINVAL and f(codes=None) == E.MN_EINVAL and f(s=None) == E.MN_EINVAL
         assert f(codes=ODD) == E.MN_EINVAL
@@ -36,7 +36,7 @@ def test_scores_refusals():
     assert f(m=-1) == f(n=-1) == f(d=0) == E.MN_EINVAL
     assert f(d=131072, ldq=131072, ldc=131072) == E.MN_ENOTSUP
     assert f(ldq=16) == f(ldc=16) == f(ldq=24) == f(ldc=40) == E.MN_EINVAL
-    assert f(ty=1) == E.MN_ENOTSUP
+    assert f(ty=1) == f(ldq=(1 << 23) + 16) == f(ldc=1 << 40) == E.MN_ENOTSUP
     assert f(Q=None) == f(c=None) == f(qs=None) == f(cs=None) == f(Y=None) == E.MN_EINVAL
     assert f(Q=ODD) == f(c=ODD) == E.MN_EINVAL
     assert f(m=65, ws=None) == f(m=65, wb=65 * 64 - 1) == f(m=65, ws=ODD) == E.MN_ECAP
