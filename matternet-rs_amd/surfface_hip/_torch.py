@@ -39,13 +39,15 @@ def enqueues(fn):
 
     @functools.wraps(fn)
     def wrapped(*args, stream=None, **kwargs):
+        t = args[0] if args else next(iter(kwargs.values()), None)
+        t = getattr(t, "codes", t)
         if stream is None:
-            t = args[0] if args else None
-            t = getattr(t, "codes", t)
             if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() == torch.cuda.current_device():
                 return fn(*args, **kwargs)
             with torch.cuda.device(t.device):
                 return fn(*args, **kwargs)
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device != stream.device:
+            raise ValueError(f"stream is on {stream.device}, the call's tensors on {t.device}")
         with torch.cuda.stream(stream):
             for a in (*args, *kwargs.values()):
                 for t in (a, getattr(a, "codes", None), getattr(a, "scale", None)):

@@ -267,6 +267,23 @@ def test_nan_in_the_target_s_row_survives_the_join():
     assert torch.isnan(alone.loss[3]) and not alone.loss[:3].any()
 
 
+def test_calls_by_name_and_streams_of_another_device():
+    import surfface_hip as S
+    q, c, at = (x.cuda() for x in data(20, 60, 16, torch.float32, 27))
+    a = S.softmax_stats(queries=q, items=c, targets=at, scale=2.0)
+    b = S.softmax_stats(q, c, at, 2.0)
+    assert torch.equal(a.loss, b.loss)
+    rows = S.quantize_rows(X=q)
+    assert torch.equal(S.scores_i8(queries=rows, items=rows), S.scores_i8(rows, rows))
+
+    class Elsewhere:
+        device = torch.device("cuda", 1)
+    for bad in (lambda: S.softmax_loss(q, c, at, stream=Elsewhere()), lambda: S.quantize_rows(X=q, stream=Elsewhere()),
+                lambda: S.scores_i8(rows, rows, stream=Elsewhere())):
+        with pytest.raises(ValueError, match="stream is on"):
+            bad()
+
+
 def test_same_target_many_times_and_int32_targets():
     import surfface_hip as S
     q, c, at = data(200, 90, 24, torch.float32, 13, ignore=False)
