@@ -6,8 +6,9 @@ no [t, v] matrix of logits is kept.  Has no counterpart in the reference.
 softmax_loss is the whole of it with autograd.  softmax_stats, softmax_merge
 and softmax_backward are its parts, for tables whose rows are spread over
 processes (c_offset, as in knn_l2sq_qc) and for steps captured into a graph.
-Capture those: a backward pass of autograd that is captured while an eager
-graph of the same leaves lives ends the process (torch's own rule).
+softmax_loss with gradients is refused in a capture: a backward pass of autograd
+that is captured while an eager graph of the same leaves lives ends the process,
+which no check here could see coming.
 
 The calls only enqueue on the stream (default: the current one).  With `stream`
 given the caller orders it after the work that made the inputs, as with
@@ -160,7 +161,9 @@ class _SoftmaxLoss(torch.autograd.Function):
         # a dense copy of an input
         same = inputs[0] is queries and inputs[1] is items and inputs[2] is targets
         ctx.of = (inputs[3:] if same else None, st.rest, st.target, st.share if reduction == "mean" else None, scale)
-        return st.mean if reduction == "mean" else st.loss if reduction == "none" else st.loss.sum()
+        if reduction == "sum":  # (torch's sum over many blocks cannot be captured)
+            return st.mean / st.share[0]
+        return st.mean if reduction == "mean" else st.loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -180,7 +183,11 @@ def softmax_loss(queries: torch.Tensor, items: torch.Tensor, targets: torch.Tens
     (f32 or bf16) with logits scale q.c, f32; differentiable once in queries
     and items.  targets [t]: row ids, negative: the query has no part (loss 0,
     gradient 0).  reduction: "mean" over the queries that take part (0 when
-    there is none), "sum" or "none"."""
+    there is none), "sum" or "none".  In a graph capture only without gradients
+    (else RuntimeError): capture softmax_stats and softmax_backward."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("reduction must be 'mean', 'sum' or 'none'")
+    if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad and x.is_cuda
+                                       for x in (queries, items)) and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("softmax_loss with gradients in a graph capture: capture softmax_stats and softmax_backward")
     return _SoftmaxLoss.apply(queries, items, targets, float(scale), reduction)

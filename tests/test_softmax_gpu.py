@@ -350,6 +350,31 @@ def test_captured_steps(dtype):
                 assert torch.equal(got, want)
 
 
+def test_capture_of_the_loss():
+    """Without gradients: replays equal the eager call, each reduction; with: refused."""
+    import surfface_hip as S
+    q, c, at = data(300, 500, 32, torch.float32, 29)
+    x, cd, a = q.cuda(), c.cuda(), at.cuda()
+    kinds = ("mean", "sum", "none")
+    want = [S.softmax_loss(x, cd, a, 5.0, k) for k in kinds]
+    # a sum over t f32 losses, a product and a quotient
+    close(want[1], want[2].double().sum().cpu(), (len(at) + 4) * U * want[2].double().sum().cpu(), "sum")
+    cg = cd.clone().requires_grad_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="graph capture"):
+            S.softmax_loss(x, cg, a)
+        with torch.no_grad():
+            out = [S.softmax_loss(x, cg, a, 5.0, k) for k in kinds]
+    for k in range(3):
+        x.copy_((q * (1 + k)).cuda())
+        want = [S.softmax_loss(x, cd, a, 5.0, k) for k in kinds]
+        g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(out, want):
+            assert torch.equal(o, w)
+
+
 def test_empty_batch_and_refusals():
     import surfface_hip as S
     q, c, at = (x.cuda() for x in data(8, 30, 16, torch.float32, 1))
