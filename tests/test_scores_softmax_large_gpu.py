@@ -1,0 +1,223 @@
+"""Item scores and softmax loss where the sizes decide: tables in several pieces,
+partial sums added up, every class of the kernels for few queries, offsets past
+2^31 and 2^32, several threads at once.  References in 64 bits, in chunks on the
+GPU; tolerances as in test_softmax_gpu.py."""
+import math
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U, B = 2.0 ** -24, 2.0 ** -8
+CHUNK = 65536
+
+
+def make(t, v, d, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c = torch.empty(v, d, dtype=dtype, device="cuda")
+    for j in range(0, v, CHUNK):
+        x = torch.randn(min(CHUNK, v - j), d, generator=g, device="cuda")
+        c[j:j + CHUNK] = (x / x.norm(dim=1, keepdim=True)).to(dtype)
+    at = torch.randint(0, v, (t,), generator=g, device="cuda")
+    q = (c[at].float() + 0.7 * torch.randn(t, d, generator=g, device="cuda") / math.sqrt(d)).to(dtype)
+    at[0] = v - 1
+    at[1::5] = -1
+    return q, c, at
+
+
+def worst(got, want, tol):
+    return float(((got.double() - want).abs() / tol).nan_to_num(nan=math.inf).max())
+
+
+def check(t, v, d, dtype, seed, scale=8.0):
+    import surfface_hip as S
+    q, c, at = make(t, v, d, dtype, seed)
+    qg, cg = q.clone().requires_grad_(), c.requires_grad_()
+    loss = S.softmax_loss(qg, cg, at, scale=scale, reduction="none")
+    n = int((at >= 0).sum())
+    dq, dc = torch.autograd.grad(loss, (qg, cg), torch.full((t,), 1.0 / n, device="cuda"))
+    c = c.detach()
+    has = at >= 0
+    x = torch.where(has[:, None], q.double(), 0.0)
+    zt = scale * (x * c[at.clamp(min=0)].double()).sum(1)
+    rest, A = torch.full((t,), -math.inf, dtype=torch.float64, device="cuda"), 0.0
+    rows = torch.arange(t, device="cuda")
+
+    def logits(j):
+        y = c[j:j + CHUNK].double()
+        here = (at >= j) & (at < j + y.shape[0])
+        return y, scale * (x @ y.T), rows[here], at[here] - j
+
+    for j in range(0, v, CHUNK):
+        y, z, r, k = logits(j)
+        z[r, k] = -math.inf
+        rest = torch.logaddexp(rest, torch.logsumexp(z, 1))
+        A = max(A, scale * float((x.abs() @ y.abs().T).max()))
+    lse = torch.logaddexp(rest, zt)
+    want = torch.where(has, lse - zt, 0.0)
+    delta = 2 * (6 * d + 8) * U * A + 16 * U * (1 + float(lse.abs().max()) + math.log2(v + 1))
+    b = B if dtype == torch.bfloat16 else 0.0
+    assert worst(loss.detach(), want, 2 * delta + 4 * U * want) <= 1
+    w_dq, s_dq = torch.zeros(t, d, dtype=torch.float64, device="cuda"), 0
+    for j in range(0, v, CHUNK):
+        y, z, r, k = logits(j)
+        D = torch.exp(z - lse[:, None])
+        D[r, k] -= 1
+        D *= torch.where(has, 1.0 / n, 0.0)[:, None]
+        w_dq += scale * (D @ y)
+        s_dq = s_dq + scale * (D.abs() @ y.abs())
+        w, mag = scale * (D.T @ x), scale * (D.abs().T @ x.abs())
+        tol = (2 * delta + (6 * t + 64) * U + b) * mag + (b or U) * w.abs() + t * 4 * scale * 2.0 ** -126
+        assert worst(dc[j:j + CHUNK], w, tol) <= 1, f"items from {j}"
+    tol = (2 * delta + (6 * v + 64) * U + b) * s_dq + (b or U) * w_dq.abs() + 1e-30
+    assert worst(dq, w_dq, tol) <= 1
+    assert not dq[~has].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pieces_of_a_table(dtype):
+    """Three (bf16) and five (f32) pieces, the last one short and odd, many partial sums of dQ."""
+    check(300, 530001, 16, dtype, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_partial_sums_added_up(dtype):
+    """Partial sums of dQ above 256 MB in all: each piece adds to those before."""
+    check(4096, 150001, 2048, dtype, 2)
+
+
+@pytest.mark.parametrize("dtype,v", [(torch.float32, 1500001), (torch.bfloat16, 3000001)])
+def test_tables_past_32_bits(dtype, v):
+    """4.6 GB of items: targets and gradients at the far end among them."""
+    check(70, v, 768, dtype, 3)
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,t,d", [
+    (torch.bfloat16, t, d) for t, d in ((1, 1288), (16, 4600), (16, 4616), (1, 65536), (17, 640), (32, 648), (33, 320), (64, 328),
+                                        (64, 1152), (64, 1160), (50, 331))] + [
+    (torch.float32, t, d) for t, d in ((1, 640), (16, 644), (16, 2304), (5, 2308), (17, 320), (32, 324), (31, 1152), (32, 1156),
+                                       (33, 40), (20, 323))])
+def test_stats_of_few_queries(dtype, t, d):
+    """Both sides of every border between the kernels for few queries, loss against the formula."""
+    check(t, 701, d, dtype, t + d, scale=4.0)
+
+
+@pytest.mark.parametrize("m,d", [(1, 2560), (16, 2561), (16, 9216), (3, 9217), (17, 1280), (32, 1281), (32, 4608), (20, 4609),
+                                 (33, 640), (64, 641), (64, 2304), (64, 2305)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_of_few_queries(dtype, m, d):
+    import surfface_hip as S
+    g = torch.Generator(device="cuda").manual_seed(m + d)
+    q, c = S.quantize_rows(torch.randn(m, d, generator=g, device="cuda")), S.quantize_rows(torch.randn(333, d, generator=g, device="cuda"))
+    exact = (q.codes[:, :d].double() @ c.codes[:, :d].double().T) * q.scale.double()[:, None] * c.scale.double()
+    tol = exact.abs() * (3.01 * U + (B if dtype == torch.bfloat16 else 0)) + 1e-44
+    assert worst(S.scores_i8(q, c, dtype), exact, tol) <= 1
+
+
+@pytest.mark.parametrize("m", [2, 70])
+def test_scores_of_a_table_past_32_bits(m):
+    """6M rows of 768 codes (4.6 GB) from bf16 rows of 9.2 GB; scores of 1.7 GB."""
+    import surfface_hip as S
+    n, d = 6_000_001, 768
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.empty(n, d, dtype=torch.bfloat16, device="cuda")
+    for j in range(0, n, 1 << 20):
+        x[j:j + (1 << 20)] = torch.randn(min(1 << 20, n - j), d, generator=g, device="cuda").bfloat16()
+    c, q = S.quantize_rows(x), S.quantize_rows(x[-m:])
+    y = S.scores_i8(q, c)
+    back = S.dequantize_rows(c, torch.bfloat16)
+    for j in (0, (1 << 31) // d - 500, (1 << 32) // d - 500, n - 1000):
+        part = S.quantize_rows(x[j:j + 1000])
+        assert torch.equal(part.codes, c.codes[j:j + 1000]) and torch.equal(part.scale, c.scale[j:j + 1000])
+        assert torch.equal(back[j:j + 1000], S.dequantize_rows(part, torch.bfloat16))
+        exact = (q.codes.double() @ part.codes.double().T) * q.scale.double()[:, None] * part.scale.double()
+        assert worst(y[:, j:j + 1000], exact, exact.abs() * 3.01 * U + 1e-44) <= 1
+    del x, c, y, back
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_past_32_bits_of_output(dtype):
+    """2100 x 1.1M scores: 2.3e9 of them."""
+    import surfface_hip as S
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = S.quantize_rows(torch.randn(2100, 40, generator=g, device="cuda"))
+    c = S.quantize_rows(torch.randn(1_100_003, 40, generator=g, device="cuda"))
+    y = S.scores_i8(q, c, dtype)
+    rows = torch.tensor([0, 1951, 1952, 1953, 2047, 2048, 2099], device="cuda")  # 1952 n: 2^31
+    for j in (0, 500_000, 1_100_003 - 70_000):
+        exact = (q.codes[rows].double() @ c.codes[j:j + 70_000].double().T) * q.scale[rows].double()[:, None] * \
+            c.scale[j:j + 70_000].double()
+        tol = exact.abs() * (3.01 * U + (B if dtype == torch.bfloat16 else 0)) + 1e-44
+        assert worst(y[rows, j:j + 70_000], exact, tol) <= 1
+    del y
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [20, 130])
+def test_items_masked_with_the_lowest_value(dtype, t):
+    """A column that gives masked items the type's lowest value: no loss, no gradient, no NaN from them."""
+    import surfface_hip as S
+    q, c, at = make(t, 900, 24, dtype, 8)
+    q[:, 0] = 1.0
+    c[:, 0] = 0.0
+    keep = torch.ones(900, dtype=torch.bool, device="cuda")
+    keep[at.clamp(min=0)] = False
+    masked = keep & (torch.arange(900, device="cuda") % 3 == 0)
+    full = c.clone()
+    full[masked, 0] = torch.finfo(dtype).min
+    new = torch.cumsum(~masked, 0) - 1  # an item's place in the table without the masked ones
+    out = []
+    for table, goal in ((full, at), (c[~masked].contiguous(), torch.where(at >= 0, new[at.clamp(min=0)], -1))):
+        qg, cg = q.clone().requires_grad_(), table.requires_grad_()
+        loss = S.softmax_loss(qg, cg, goal, 6.0, "none")
+        out.append([loss.detach(), *torch.autograd.grad(loss.mean(), (qg, cg))])
+    (l0, q0, c0), (l1, q1, c1) = out
+    assert torch.isfinite(q0).all() and torch.isfinite(c0).all() and not c0[masked].any()
+    # both within their bounds of the same formula; see test_softmax_gpu.py for the terms
+    A = 6.0 * float((q.double().abs() @ c.double().abs().T).max())
+    delta = 2 * (6 * 24 + 8) * U * A + 16 * U * (1 + A + 10)
+    assert ((l0 - l1).abs().double() <= 4 * delta + 8 * U * l1).all()
+    b = B if dtype == torch.bfloat16 else U
+    for a, w, mag in ((q0, q1, 12.0 / t * c.double().abs().max(0).values), (c0[~masked], c1, 12.0 / t * q.double().abs().sum(0))):
+        assert ((a.double() - w.double()).abs() <= 2 * (2 * delta + 6000 * U + 2 * b) * mag).all()
+
+
+def test_threads_on_streams_of_their_own():
+    """Two threads, a stream each, steps and scores at the same time: the results of one after the other."""
+    import surfface_hip as S
+    jobs = [make(200 + 300 * k, 5000 + 999 * k, 48, torch.bfloat16, 20 + k) for k in range(2)]
+
+    def run(q, c, at):
+        qg, cg = q.clone().requires_grad_(), c.clone().requires_grad_()
+        loss = S.softmax_loss(qg, cg, at, 5.0)
+        return [loss.detach(), *torch.autograd.grad(loss, (qg, cg)), S.scores_i8(S.quantize_rows(q), S.quantize_rows(c))]
+
+    want = [run(*j) for j in jobs]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(k):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    got[k].append(run(*jobs[k]))
+            s.synchronize()
+        except Exception as e:  # shown by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors
+    for k in range(2):
+        for r in got[k]:
+            for a, b in zip(r, want[k]):
+                assert torch.equal(a, b)
