@@ -667,7 +667,9 @@ int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, 
  * matrix is kept.  targets [t] (int64) hold global row ids, C's rows are the
  * ids c_offset .. c_offset + v - 1 (c_offset 0: the whole table).  A row with a
  * negative target has no part: loss 0, gradient 0, and what it holds (a NaN)
- * reaches no other row.
+ * reaches no other row.  All other values have to be finite: an infinity or a
+ * NaN makes the results that it meets NaN.  The type's lowest value in an item
+ * (a mask) is finite; a logit below -2^127 counts as -infinity.
  * mn_softmax_stats writes per row rest = log sum exp z over the items but the
  * target, zt = the target's logit (-inf where it is not among the rows here),
  * loss = log(1 + exp(rest - zt)) (+inf where zt is -inf), and where mean is not

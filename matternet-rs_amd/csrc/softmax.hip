@@ -230,8 +230,8 @@ __global__ __launch_bounds__(256) void k_prep(Pack q, Pack c, Rows r) {
 // Per lane and row the largest logit so far (m2, base 2, rounded: the number
 // that every exponent is taken from) and the sum of exp of the rest, the
 // target's left out; joined over the lanes and written per run of tiles and
-// half of the columns.  An element costs a max, an fma, an exp and an add: for
-// 768 columns of operands about a seventh of its time on the matrix pipe.
+// half of the columns.  An element costs a max, an fma, an exp and an add: 701 us
+// for 4096 x 131072 x 768 in bf16, 618 without.
 struct StatsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;
@@ -452,7 +452,8 @@ __global__ __launch_bounds__(1024) void k_grad_max(const float *__restrict__ gra
 }
 
 // D of a piece of the table, [tp][ldd], f32 or rounded to bf16; zeros in the
-// rows and columns that only fill tiles.
+// rows and columns that only fill tiles.  4096 x 32768 x 768 in bf16 220 us, 158
+// without this (the exp, and 268 MB to the last-level cache).
 template <bool F32>
 struct DlogitsEpi {
     struct Shared {};
@@ -673,8 +674,9 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         // dQ's runs of k: the cut with the least time for the blocks of both
         // products on 256 processors, dQ's first, in steps: a block of dQ
         // costs its run and 20 for its part of the sum (256 KB to memory), one
-        // of dC t / 32 and 10 (f32, whose steps take twice as long: 6 and 4).  Free processors take the next block: dC's done
-        // by a time are counted from the two times at which dQ's blocks end.
+        // of dC t / 32 and 10 (f32, whose steps take longer: 6 and 4).  Free
+        // processors take the next block: dC's done by a time are counted from
+        // the two times at which dQ's blocks end.
         p.nf = f32 ? (d > 64 ? 4 : 2) : d > 128 ? 8 : d > 64 ? 4 : 2;
         const int64_t cols = (d + 32 * p.nf - 1) / (32 * p.nf), tiles = panels * cols;
         const int64_t steps = p.vc / 32, nc = p.vc / mm::TILE * cols, b = t / 32 + (f32 ? 4 : 10);

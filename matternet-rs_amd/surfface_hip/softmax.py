@@ -13,6 +13,10 @@ which no check here could see coming.
 The calls only enqueue on the stream (default: the current one).  With `stream`
 given the caller orders it after the work that made the inputs, as with
 torch.cuda.stream(stream).
+
+Values of items and of queries that take part have to be finite (else what they
+meet is NaN); an item that holds the type's lowest value where the queries are
+positive is masked out: its logit is far below all others.
 """
 from __future__ import annotations
 
