@@ -21,13 +21,14 @@
 // the step read after the next barrier has landed.  Past the last step the
 // loads repeat it into the slot that nobody reads any more: the count stays.
 //
-// What bounds it: the matrix pipe and LDS together.  A step's 32 matrix
+// What bounds it: the chip's power, then LDS.  4096 x 131072 x 768 in bf16
+// without the epilogue takes 618 us, 1.33 PFLOP/s: 65% of the matrix pipe at the
+// 1.95 GHz that the chip then holds.  A large library product (8192^3, 1.33 to
+// 1.40) fills 87% of the pipe and gets 1.5 GHz for it.  A step's 32 matrix
 // instructions a wave take a SIMD 512 cycles for each of its two waves; its
 // fragments (96 KB a block) and the loads that land (32 KB) take LDS the same
-// 1024 at 128 bytes a cycle.  4096 x 131072 x 768 in bf16 without the epilogue:
-// 618 us, 1.33 PFLOP/s, at the 1.95 GHz that the chip holds under this load 65%
-// of the matrix pipe; a large library product (8192^3) reaches 1.40 here.  An
-// epilogue is not hidden: the other wave of the SIMD has one window to give.
+// 1024 at 128 bytes a cycle.  An epilogue is not hidden: the other wave of the
+// SIMD has one window to give.
 //
 // LDS layouts, free of bank conflicts.  Rows of k: a row's k-step is 64 bytes,
 // piece c (16 bytes) of row r at c ^ 2 ((r >> s) & 1), s = 3 where a fragment's
