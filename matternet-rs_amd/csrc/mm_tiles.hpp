@@ -61,6 +61,9 @@ constexpr int GP = 8;
 
 struct Bf16 {
     typedef f32x4 acc_t;
+    // of k_few: matrix instructions for 16 bytes of k; k-steps of a turn
+    static constexpr int PARTS = 1, AHEAD = 2;
+    static __device__ __forceinline__ acc_t part(u32x4 a, u32x4 b, acc_t c, int) { return mma(a, b, c); }
     static __device__ __forceinline__ acc_t mma(u32x4 a, u32x4 b, acc_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                        __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -68,6 +71,9 @@ struct Bf16 {
 };
 struct Int8 {
     typedef i32x4 acc_t;
+    // of k_few: matrix instructions for 16 bytes of k; k-steps of a turn
+    static constexpr int PARTS = 1, AHEAD = 2;
+    static __device__ __forceinline__ acc_t part(u32x4 a, u32x4 b, acc_t c, int) { return mma(a, b, c); }
     static __device__ __forceinline__ acc_t mma(u32x4 a, u32x4 b, acc_t c) {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
                                                      __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
@@ -77,11 +83,9 @@ struct Int8 {
 // f32 operands as they are: 16 bytes are four k's of one product each
 struct F32 {
     typedef f32x4 acc_t;
-    static __device__ __forceinline__ acc_t mma(u32x4 a, u32x4 b, acc_t c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
-        return c;
+    static constexpr int PARTS = 4, AHEAD = 4;
+    static __device__ __forceinline__ acc_t part(u32x4 a, u32x4 b, acc_t c, int e) {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
     }
 };
 
@@ -316,34 +320,42 @@ struct FewArgs {
     int64_t n;         // rows of B
     int m;             // queries
     int qbytes;        // bytes of a query's row that count (zeros behind)
-    int nk, bmax, blocks;
+    int nk, bmax;
+    int mf;            // a block has 16 mf queries in LDS
+    int groups;        // of so many queries; the groups' blocks of the same rows lie side by side on an XCD
+    int slices;        // blocks of a group
     bool small;        // queries take at most FEW_SMALL bytes of LDS
 };
 constexpr int FEW_SMALL = 40 << 10, FEW_LARGE = 144 << 10;
 
-// false: the queries do not fit LDS
-inline bool plan_few(FewArgs &a) {
+// false: the queries do not fit LDS (split: not even 16 of them)
+inline bool plan_few(FewArgs &a, bool split) {
     a.nk = (a.qbytes + KBY - 1) / KBY;
     a.bmax = (a.qbytes + 15) / 16 * 16 - 16;
-    const int64_t mf = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4, bytes = mf * 16 * a.nk * KBY;
-    a.small = bytes <= FEW_SMALL;
-    if (bytes > FEW_LARGE) return false;
-    const int64_t groups = (a.n + 15) / 16;
-    a.blocks = (int)std::min<int64_t>((groups + 7) / 8, a.small ? 512 : 256);
+    a.mf = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
+    auto bytes = [&]() { return (int64_t)a.mf * 16 * a.nk * KBY; };
+    while (split && a.mf > 1 && bytes() > FEW_LARGE) a.mf /= 2;
+    a.small = bytes() <= FEW_SMALL;
+    if (bytes() > FEW_LARGE) return false;
+    a.groups = (a.m + 16 * a.mf - 1) / (16 * a.mf);
+    a.slices = (int)std::min<int64_t>((a.n + 127) / 128, (a.small ? 512 : 256) / a.groups);
+    if (a.groups > 1) a.slices = (a.slices + 7) / 8 * 8;
     return true;
 }
 
 template <class OP, int MF, int LDSB, class EPI>
 __global__ __launch_bounds__(NT) void k_few(FewArgs a, EPI epi) {
     __shared__ alignas(16) char qs[LDSB];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fr = lane & 15, fk = lane >> 4;
+    const int unit = (int)blockIdx.x >> 3, slice = ((int)blockIdx.x & 7) + 8 * (unit / a.groups);
+    const int q0 = 16 * MF * (unit % a.groups);
     for (int p = tid; p < 64 * MF * a.nk; p += NT) {
         const int c = p & 3, r = (p >> 2) % (16 * MF), kc = (p >> 2) / (16 * MF);
         const int byte = kc * KBY + 16 * c;
         uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < a.m && byte < a.qbytes && epi.takes(r)) {
-            x = *reinterpret_cast<const uint4 *>(a.Q + r * a.ldq + byte);
+        if (q0 + r < a.m && byte < a.qbytes && epi.takes(q0 + r)) {
+            x = *reinterpret_cast<const uint4 *>(a.Q + (q0 + r) * a.ldq + byte);
             const int left = a.qbytes - byte;  // bytes of the piece that count
             if (left < 16) {
                 uint32_t *q = &x.x;
@@ -356,48 +368,71 @@ __global__ __launch_bounds__(NT) void k_few(FewArgs a, EPI epi) {
         }
         *reinterpret_cast<uint4 *>(qs + (p >> 2) * KBY + 16 * (c ^ (((r >> 3) & 1) << 1))) = x;
     }
-    epi.init(lane);
+    epi.init(q0, lane);
     __syncthreads();
     const char *qr = qs + fr * KBY + 16 * (fk ^ (((fr >> 3) & 1) << 1));
     const int64_t groups = (a.n + 15) / 16;
-    for (int64_t g = (int64_t)blockIdx.x * (NT / 64) + w; g < groups; g += (int64_t)gridDim.x * (NT / 64)) {
-        const char *row = a.B + min(16 * g + fr, a.n - 1) * a.ldb;
-        typename OP::acc_t acc[MF];
+    const int64_t stride = (int64_t)a.slices * (NT / 64);
+    int64_t g = (int64_t)slice * (NT / 64) + w;
+    typename OP::acc_t acc[MF];
+    constexpr int U = OP::AHEAD;
+    u32x4 b[2][U];
+    auto row_of = [&](int64_t x) __attribute__((always_inline)) { return a.B + min(16 * x + fr, a.n - 1) * a.ldb; };
+    auto load = [&](u32x4 (&x)[U], const char *row, int kc) __attribute__((always_inline)) {
 #pragma unroll
-        for (int f = 0; f < MF; ++f) acc[f] = (typename OP::acc_t)(0);
-        constexpr int U = 4;
-        u32x4 b[2][U];
-        auto load = [&](u32x4 (&x)[U], int kc) __attribute__((always_inline)) {
+        for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const u32x4 *>(row + min((kc + u) * KBY + 16 * fk, a.bmax));
+    };
+    const char *row = nullptr;
+    int kc = 0;
+    // four k-steps: those after them on their way first, of the next rows too
+    auto turn = [&](u32x4 (&x)[U], u32x4 (&next)[U]) __attribute__((always_inline)) {
+        const bool last = kc + U >= a.nk;
+        const int64_t gn = last ? g + stride : g;
+        const int kn = last ? 0 : kc + U;
+        if (kc == 0) {
+            epi.fetch(16 * g, lane);
+#pragma unroll
+            for (int f = 0; f < MF; ++f) acc[f] = (typename OP::acc_t)(0);
+        }
+        if (gn < groups) {
+            if (last) row = row_of(gn);
+            load(next, row, kn);
+        }
+        auto use = [&](int u) __attribute__((always_inline)) {
+            u32x4 q[MF];
+#pragma unroll
+            for (int f = 0; f < MF; ++f) q[f] = *reinterpret_cast<const u32x4 *>(qr + ((kc + u) * MF + f) * 16 * KBY);
+#pragma unroll
+            for (int e = 0; e < OP::PARTS; ++e)
+#pragma unroll
+                for (int f = 0; f < MF; ++f) acc[f] = OP::part(x[u], q[f], acc[f], e);
+        };
+        if (kc + U <= a.nk) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) use(u);
+        } else {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                x[u] = *reinterpret_cast<const u32x4 *>(row + min((kc + u) * KBY + 16 * fk, a.bmax));
-        };
-        auto use = [&](u32x4 (&x)[U], int kc) __attribute__((always_inline)) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (kc + u >= a.nk) break;
-#pragma unroll
-                for (int f = 0; f < MF; ++f)
-                    acc[f] = OP::mma(x[u], *reinterpret_cast<const u32x4 *>(qr + ((kc + u) * MF + f) * 16 * KBY), acc[f]);
-            }
-        };
-        load(b[0], 0);
-        for (int kc = 0; kc < a.nk; kc += 2 * U) {
-            if (kc + U < a.nk) load(b[1], kc + U);
-            use(b[0], kc);
-            if (kc + U >= a.nk) break;
-            if (kc + 2 * U < a.nk) load(b[0], kc + 2 * U);
-            use(b[1], kc + U);
+                if (kc + u < a.nk) use(u);
         }
-        epi.group(acc, 16 * g, lane);
+        if (last) epi.group(acc, 16 * g, lane);
+        g = gn;
+        kc = kn;
+        return g < groups;
+    };
+    if (g < groups) {
+        row = row_of(g);
+        load(b[0], row, 0);
+        while (turn(b[0], b[1]) && turn(b[1], b[0])) {
+        }
     }
-    epi.finish(qs, tid);
+    epi.finish(qs, slice, tid);
 }
 
 template <class OP, int MF, class EPI>
 void launch_few(const FewArgs &a, const EPI &epi, hipStream_t s) {
-    if (a.small) hipLaunchKernelGGL((k_few<OP, MF, FEW_SMALL, EPI>), dim3(a.blocks), dim3(NT), 0, s, a, epi);
-    else hipLaunchKernelGGL((k_few<OP, MF, FEW_LARGE, EPI>), dim3(a.blocks), dim3(NT), 0, s, a, epi);
+    if (a.small) hipLaunchKernelGGL((k_few<OP, MF, FEW_SMALL, EPI>), dim3(a.slices * a.groups), dim3(NT), 0, s, a, epi);
+    else hipLaunchKernelGGL((k_few<OP, MF, FEW_LARGE, EPI>), dim3(a.slices * a.groups), dim3(NT), 0, s, a, epi);
 }
 
 struct KnArgs {

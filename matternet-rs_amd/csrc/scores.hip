@@ -254,21 +254,24 @@ struct FewScoreEpi {
     const float *qs, *cs;
     T *Y;
     int64_t n;
-    int m;
-    float q[MF];
+    int m, q0_;
+    float q[MF], c[4];
     __device__ __forceinline__ bool takes(int) const { return true; }
-    __device__ __forceinline__ void init(int lane) {
+    __device__ __forceinline__ void init(int q0, int lane) {
+        q0_ = q0;
 #pragma unroll
-        for (int f = 0; f < MF; ++f) q[f] = qs[min(16 * f + (lane & 15), m - 1)];
+        for (int f = 0; f < MF; ++f) q[f] = qs[min(q0 + 16 * f + (lane & 15), m - 1)];
+    }
+    __device__ __forceinline__ void fetch(int64_t j0, int lane) {
+        const int64_t j = j0 + 4 * (lane >> 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] = cs[min(j + r, n - 1)];
     }
     __device__ __forceinline__ void group(mm::i32x4 (&acc)[MF], int64_t j0, int lane) {
         const int64_t j = j0 + 4 * (lane >> 4);
-        float c[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) c[r] = cs[min(j + r, n - 1)];
 #pragma unroll
         for (int f = 0; f < MF; ++f) {
-            const int i = 16 * f + (lane & 15);
+            const int i = q0_ + 16 * f + (lane & 15);
             if (i >= m || j >= n) continue;
             mm::f32x4 x;
 #pragma unroll
@@ -276,7 +279,7 @@ struct FewScoreEpi {
             mm::store4<sizeof(T) == 4>(Y, i * n + j, (int)min<int64_t>(4, n - j), x);
         }
     }
-    __device__ __forceinline__ void finish(char *, int) {}
+    __device__ __forceinline__ void finish(char *, int, int) {}
 };
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -304,7 +307,7 @@ inline int padded(int d) { return (d + mm::KBY - 1) / mm::KBY * mm::KBY; }
 inline bool few_args(mm::FewArgs &a, int64_t m, int d) {
     a.m = (int)std::min<int64_t>(m, 65);
     a.qbytes = d;
-    return m <= 64 && mm::plan_few(a);
+    return m <= 64 && mm::plan_few(a, false);
 }
 inline size_t workspace(int64_t m, int d) {
     mm::FewArgs few = {};
@@ -408,8 +411,8 @@ extern "C" int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, 
             mm::launch_few<mm::Int8, decltype(MF)::value>(few, epi, s);
         };
         auto size = [&](auto out) {
-            if (m <= 16) go(out, std::integral_constant<int, 1>());
-            else if (m <= 32) go(out, std::integral_constant<int, 2>());
+            if (few.mf == 1) go(out, std::integral_constant<int, 1>());
+            else if (few.mf == 2) go(out, std::integral_constant<int, 2>());
             else go(out, std::integral_constant<int, 4>());
         };
         if (y_type == MN_F32) size(float());

@@ -84,24 +84,26 @@ __device__ __forceinline__ void pack(const Pack &p, int block) {
 // As StatsEpi, for k_few: 16 items at a time, MF groups of 16 queries.
 template <int MF>
 struct FewStatsEpi {
-    float2 *part;  // [blocks][t]
+    float2 *part;  // [slices][t]
     const int64_t *targets;
     int64_t c_offset, v;
-    int t;
+    int t, q0_;
     float scale2;
     int at[MF];
     float m2[MF], sum[MF];
     __device__ __forceinline__ bool takes(int i) const { return targets[i] >= 0; }
-    __device__ __forceinline__ void init(int lane) {
+    __device__ __forceinline__ void init(int q0, int lane) {
+        q0_ = q0;
 #pragma unroll
         for (int f = 0; f < MF; ++f) {
-            const int i = 16 * f + (lane & 15);
+            const int i = q0 + 16 * f + (lane & 15);
             const int64_t x = i < t ? targets[i] : -1;
             at[f] = x >= c_offset && x - c_offset < v ? (int)(x - c_offset) : -1;
             m2[f] = -__builtin_inff();
             sum[f] = 0.f;
         }
     }
+    __device__ __forceinline__ void fetch(int64_t, int) {}
     __device__ __forceinline__ void group(mm::f32x4 (&acc)[MF], int64_t j0, int lane) {
         const int j = (int)j0 + 4 * (lane >> 4);
 #pragma unroll
@@ -119,7 +121,7 @@ struct FewStatsEpi {
         }
     }
     // joined over the lanes, then over the block's waves
-    __device__ __forceinline__ void finish(char *lds, int tid) {
+    __device__ __forceinline__ void finish(char *lds, int slice, int tid) {
         float2 *sh = reinterpret_cast<float2 *>(lds);
         const int lane = tid & 63, w = tid >> 6;
         auto join = [](float &m, float &s, float mo, float so) {
@@ -138,11 +140,11 @@ struct FewStatsEpi {
             if (lane < 16) sh[w * 16 * MF + 16 * f + lane] = make_float2(m2[f], sum[f]);
         }
         __syncthreads();
-        if (tid < t) {
+        if (tid < 16 * MF && q0_ + tid < t) {
             float2 x = sh[tid];
 #pragma unroll
             for (int k = 1; k < mm::NT / 64; ++k) join(x.x, x.y, sh[k * 16 * MF + tid].x, sh[k * 16 * MF + tid].y);
-            part[(int64_t)blockIdx.x * t + tid] = x;
+            part[(int64_t)slice * t + q0_ + tid] = x;
         }
     }
 };
@@ -614,7 +616,7 @@ struct Plan {
     int64_t ldc;        // bytes of a row of C as the products read it
     int tile;           // items of a tile of logits
     mm::NtArgs nt;      // the whole table's logits
-    mm::FewArgs few;    // the same for few queries; blocks 0: not so
+    mm::FewArgs few;    // the same for few queries; slices 0: not so
     bool few_q;         // on the queries as they are
     int64_t ldd;        // row stride of D
     int64_t vc, vmax;   // items per piece (backward), of the longest piece, in whole tiles
@@ -654,9 +656,9 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         p.few_q = !p.pack_c;
         p.few.ldq = p.few.ldb = p.ldc;
         p.few.qbytes = (int)p.ldc;
-        if (t > (f32 ? 32 : 64) || !mm::plan_few(p.few)) p.few.blocks = 0;
+        if (t > 64 || !mm::plan_few(p.few, f32)) p.few.slices = 0;
         mm::plan_runs(p.nt, p.tile);
-        p.part = take((size_t)std::max(p.nt.slices * 2, p.few.blocks) * t * 8);
+        p.part = take((size_t)std::max(p.nt.slices * 2, p.few.slices) * t * 8);
     } else {
         // Pieces whose D stays below 256 MB (the last-level cache; 128, 512 and
         // 1024 MB take 3.22, 3.05 and 3.06 ms for 4096 x 131072 x 768, 256 MB
@@ -722,7 +724,7 @@ int prep(const Plan &p, const void *Q, const void *C, const int64_t *targets, ch
         const int blocks = (int)((pieces + 256 * per - 1) / (256 * per));
         return Pack{X, w + out, tg, n, p.d, p.kp, per, blocks, !p.pack_c};
     };
-    const Pack q = p.few.blocks && p.few_q ? Pack{} : one(Q, p.q, p.t, targets);
+    const Pack q = p.few.slices && p.few_q ? Pack{} : one(Q, p.q, p.t, targets);
     const Pack c = p.pack_c ? one(C, p.c, p.v, nullptr) : Pack{};
     hipLaunchKernelGGL(k_prep<F32>, dim3((unsigned)(q.blocks + c.blocks + row_blocks)), dim3(256), 0, s, q, c, r);
     MN_KCHECK(s, "k_prep");
@@ -762,11 +764,11 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
     if (rc != MN_OK) return rc;
     float2 *part = (float2 *)(w + p.part);
     int64_t pieces;
-    if (p.few.blocks) {
+    if (p.few.slices) {
         mm::FewArgs a = p.few;
         a.Q = p.few_q ? (const char *)Q : w + p.q;
         a.B = p.pack_c ? w + p.c : (const char *)C;
-        pieces = a.blocks;
+        pieces = a.slices;
         auto go = [&](auto MF) {
             FewStatsEpi<decltype(MF)::value> epi = {};
             epi.part = part;
@@ -777,9 +779,9 @@ int stats_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d, co
             epi.scale2 = scale * kLog2e;
             mm::launch_few<std::conditional_t<F32, mm::F32, mm::Bf16>, decltype(MF)::value>(a, epi, s);
         };
-        if (t <= 16) go(std::integral_constant<int, 1>());
-        else if (t <= 32) go(std::integral_constant<int, 2>());
-        else if constexpr (!F32) go(std::integral_constant<int, 4>());
+        if (a.mf == 1) go(std::integral_constant<int, 1>());
+        else if (a.mf == 2) go(std::integral_constant<int, 2>());
+        else go(std::integral_constant<int, 4>());
         MN_KCHECK(s, "k_few");
     } else {
         const mm::NtArgs a = nt_args(p, C, w);
