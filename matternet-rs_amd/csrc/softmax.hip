@@ -37,7 +37,8 @@ struct Row {
 // reaches no sum.  A thread takes 16 bytes at a time, all loads first.
 struct Pack {
     const void *X;
-    char *out;
+    char *out;               // or NULL
+    char *planes;            // or NULL: f32 as three planes of bf16 of rows * kp values
     const int64_t *targets;  // or NULL
     int64_t rows;
     int d, kp, per, blocks;  // per: pieces a thread, 1 or kPackPer
@@ -77,7 +78,14 @@ __device__ __forceinline__ void pack(const Pack &p, int block) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t l = 256 * u + threadIdx.x;
-        if (l < left) *reinterpret_cast<mm::u32x4 *>(p.out + 16 * (base + l)) = v[u];
+        if (l >= left) return;
+        if (p.out) *reinterpret_cast<mm::u32x4 *>(p.out + 16 * (base + l)) = v[u];
+        if (F32 && p.planes) {
+            uint2 s[3];
+            mm::split4(v[u], s);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2 *>(p.planes + k * p.rows * p.kp * 2 + 8 * (base + l)) = s[k];
+        }
     }
 }
 
@@ -624,7 +632,7 @@ struct Plan {
     int splits;         // of dQ's sum over a piece
     int pieces, parts;  // of the table; partial sums of dQ in all
     bool apart;         // a piece's partial sums are its own
-    size_t q, c, part, row, at, gs, D, dq, bytes;
+    size_t q, planes, c, part, row, at, gs, D, dq, bytes;
 };
 
 inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
@@ -639,7 +647,7 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
     p.ldc = (int64_t)(p.pack_c ? p.kp : d) * p.size;
     p.tp = (t + mm::TILE - 1) / mm::TILE * mm::TILE;
     p.tile = f32 ? mm::COLS32 : mm::TILE;
-    p.nt.lda = (int64_t)p.kp * p.size;
+    p.nt.lda = (int64_t)p.kp * 2;
     p.nt.ldb = p.ldc;
     p.nt.m = t;
     p.nt.n = v;
@@ -647,7 +655,6 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
     p.nt.bmax = (int)p.ldc - 16;
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += up(b); return at; };
-    p.q = take((size_t)t * p.kp * p.size);
     p.c = take(p.pack_c ? (size_t)v * p.kp * p.size : 0);
     if (!backward) {
         // few queries: items straight to registers
@@ -657,9 +664,14 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         p.few.ldq = p.few.ldb = p.ldc;
         p.few.qbytes = (int)p.ldc;
         if (t > 64 || !mm::plan_few(p.few, f32)) p.few.slices = 0;
+        const bool few = p.few.slices > 0;
+        p.q = take(few ? (p.few_q ? 0 : (size_t)t * p.kp * p.size) : f32 ? 0 : (size_t)t * p.kp * 2);
+        p.planes = take(f32 && !few ? (size_t)t * p.kp * 6 : 0);
         mm::plan_runs(p.nt, p.tile);
         p.part = take((size_t)std::max(p.nt.slices * 2, p.few.slices) * t * 8);
     } else {
+        p.q = take((size_t)t * p.kp * p.size);
+        p.planes = take(f32 ? (size_t)t * p.kp * 6 : 0);
         // Pieces whose D stays below 256 MB (the last-level cache; 128, 512 and
         // 1024 MB take 3.22, 3.05 and 3.06 ms for 4096 x 131072 x 768, 256 MB
         // 3.05) and whose tiles fill whole rounds of 256 blocks; a short
@@ -718,14 +730,16 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
 template <bool F32>
 int prep(const Plan &p, const void *Q, const void *C, const int64_t *targets, char *w, const Rows &r, int64_t row_blocks,
          hipStream_t s) {
-    auto one = [&](const void *X, size_t out, int64_t n, const int64_t *tg) {
+    // f32 queries: planes for the logits, as they are for k_few and for dC
+    const bool few = p.few.slices > 0, planes = F32 && !few;
+    auto one = [&](const void *X, char *out, char *pl, int64_t n, const int64_t *tg) {
         const int64_t pieces = n * (p.kp * p.size / 16);
         const int per = pieces >= kPackPer * 256 * 1024 ? kPackPer : 1;
         const int blocks = (int)((pieces + 256 * per - 1) / (256 * per));
-        return Pack{X, w + out, tg, n, p.d, p.kp, per, blocks, !p.pack_c};
+        return Pack{X, out, pl, tg, n, p.d, p.kp, per, blocks, !p.pack_c};
     };
-    const Pack q = p.few.slices && p.few_q ? Pack{} : one(Q, p.q, p.t, targets);
-    const Pack c = p.pack_c ? one(C, p.c, p.v, nullptr) : Pack{};
+    const Pack q = few && p.few_q ? Pack{} : one(Q, planes && !r.rest ? nullptr : w + p.q, planes ? w + p.planes : nullptr, p.t, targets);
+    const Pack c = p.pack_c ? one(C, w + p.c, nullptr, p.v, nullptr) : Pack{};
     hipLaunchKernelGGL(k_prep<F32>, dim3((unsigned)(q.blocks + c.blocks + row_blocks)), dim3(256), 0, s, q, c, r);
     MN_KCHECK(s, "k_prep");
     return MN_OK;
@@ -733,7 +747,7 @@ int prep(const Plan &p, const void *Q, const void *C, const int64_t *targets, ch
 
 static mm::NtArgs nt_args(const Plan &p, const void *C, char *ws) {
     mm::NtArgs a = p.nt;
-    a.A = ws + p.q;
+    a.A = ws + (p.size == 4 ? p.planes : p.q);
     a.B = p.pack_c ? ws + p.c : (const char *)C;
     return a;
 }
@@ -741,7 +755,7 @@ static mm::NtArgs nt_args(const Plan &p, const void *C, char *ws) {
 template <bool F32, class EPI>
 void launch_nt(const mm::NtArgs &a, const EPI &epi, hipStream_t s) {
     const dim3 grid((unsigned)(a.panels * a.slices));
-    if constexpr (F32) hipLaunchKernelGGL((mm::k_nt32<EPI>), grid, dim3(mm::NT), 0, s, a, epi);
+    if constexpr (F32) hipLaunchKernelGGL((mm::k_nt32<EPI>), grid, dim3(mm::NT), 0, s, a, a.m * a.lda, epi);
     else hipLaunchKernelGGL((mm::k_nt<mm::Bf16, EPI>), grid, dim3(mm::NT), 0, s, a, epi);
 }
 
