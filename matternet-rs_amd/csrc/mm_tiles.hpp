@@ -3,7 +3,7 @@
 //
 //   k_nt   Y[i][j] = sum_k A[i][k] B[j][k]   (rows against rows): a block keeps
 //          256 rows of A and goes through a run of 256-row tiles of B
-//   k_few  the same for up to 64 rows of A
+//   k_few  the same for few rows of A, B straight to registers
 //   k_kn2  Y[m][n] = sum_k A(m,k) B[k][n]    (A [m][k] or [k][m]): one 256 x 256
 //          tile and run of k a block, two such products in a launch
 // with f32 (bf16 operands) or int32 (int8 operands) sums; an epilogue object
@@ -306,14 +306,16 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     epi.finish(sh, i0 + 64 * wi, slice * 2 + wj, lane);
 }
 
-// Up to 64 queries against many rows: as many bytes of B as possible in flight
-// is all that counts.  The queries lie in LDS ([k-step][query][64 bytes], pieces
-// at c ^ 2 ((query >> 3) & 1): no bank conflicts), a wave takes 16 rows of B at
-// a time from memory to registers, four k-steps of loads ahead of their
-// products, and the block's waves go through B side by side.  One query on 1M
-// rows of 768 codes (768 MB): 135 us, 5.7 TB/s; 512 blocks, not 768 (145), 384
-// (146) or 256 (144), loads of 4 steps, not 3 (139) or 6 (143), and through the
-// caches (past them: 150).
+// Up to 64 queries against many rows: that the bytes of B are in flight is all
+// that counts.  The queries lie in LDS ([k-step][query][64 bytes], pieces at c ^
+// 2 ((query >> 3) & 1): no bank conflicts), a wave takes 16 rows of B at a time
+// from memory to registers, a turn of k-steps ahead of their products (the next
+// 16 rows' first turn too), and the block's waves go through B side by side.
+// One query on 1M rows of 768 codes (768 MB): 132 us, 5.8 TB/s; 512 blocks (768:
+// 134, 1024: 145, 256: 181), turns of two k-steps (one: 162, three: 138, four:
+// 137), through the caches (past them: 150).  f32, whose products take longer
+// than the bytes: turns of four (64 queries x 200000 x 512: 162 us, two: 192);
+// more queries than LDS holds go in groups.
 struct FewArgs {
     const char *Q, *B;
     int64_t ldq, ldb;  // bytes, multiples of 16
@@ -338,7 +340,7 @@ inline bool plan_few(FewArgs &a, bool split) {
     a.small = bytes() <= FEW_SMALL;
     if (bytes() > FEW_LARGE) return false;
     a.groups = (a.m + 16 * a.mf - 1) / (16 * a.mf);
-    a.slices = (int)std::min<int64_t>((a.n + 127) / 128, (a.small ? 512 : 256) / a.groups);
+    a.slices = (int)std::min<int64_t>((a.n + 127) / 128, std::max(1, (a.small ? 512 : 256) / a.groups));
     if (a.groups > 1) a.slices = (a.slices + 7) / 8 * 8;
     return true;
 }

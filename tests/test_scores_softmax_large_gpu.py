@@ -105,6 +105,13 @@ def test_stats_of_few_queries(dtype, t, d):
     check(t, 701, d, dtype, t + d, scale=4.0)
 
 
+@pytest.mark.parametrize("t,v,d", [(33, 700, 580), (64, 300, 1160), (40, 901, 2304), (31, 129, 1200), (65, 500, 768),
+                                   (130, 1003, 772), (500, 1500, 130), (700, 300, 1000), (1024, 500, 768), (1030, 40, 2048)])
+def test_groups_of_queries_in_f32(t, v, d):
+    """Queries that LDS does not hold at once, with both sides of the rules that choose the kernel."""
+    check(t, v, d, torch.float32, t + v, scale=4.0)
+
+
 @pytest.mark.parametrize("m,d", [(1, 2560), (16, 2561), (16, 9216), (3, 9217), (17, 1280), (32, 1281), (32, 4608), (20, 4609),
                                  (33, 640), (64, 641), (64, 2304), (64, 2305)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
