@@ -533,12 +533,18 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
             }
 #pragma unroll
             for (int g = 0; g < NF; ++g) fj[g] = tr(&rg.b[0][1][0] + so, NF * wj + g);
-            issue();
-            read_window_end<8>();
+            read_window_end<4>();
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int g = 0; g < NF; ++g) acc[f][g] = Bf16::mma(fj[g], fi[f], acc[f][g]);
+                for (int g = 0; g < NF; ++g) {
+                    acc[f][g] = Bf16::mma(fj[g], fi[f], acc[f][g]);
+                    if (NF * f + g == 4) {  // the loads among the products: what is read next is two steps old
+                        __builtin_amdgcn_sched_barrier(0);
+                        issue();
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
             window_end();
         }
         if (!wj) window_end();
@@ -557,7 +563,9 @@ struct KnGrid {
 // Two products in one launch, so that the tiles of the second fill the
 // processors that the last round of the first leaves idle: A [m][k] first, then
 // A [k][m].  Bound as k_nt, with twice the read instructions for a transposed
-// fragment: 4096 x 32768 x 768 and its transpose 374 us, 1.10 PFLOP/s.
+// fragment; the loads are issued among the products (in the reading window: 379
+// us; k_nt is the faster that way): 4096 x 32768 x 768 and its transpose 365 us,
+// 1.13 PFLOP/s.
 template <int NF, class E1, class E2>
 __global__ __launch_bounds__(NT, 2) void k_kn2(KnArgs a1, E1 e1, KnGrid g1, KnArgs a2, E2 e2, KnGrid g2) {
     __shared__ Ring rg;
