@@ -194,6 +194,89 @@ def test_items_masked_with_the_lowest_value(dtype, t):
         assert ((a.double() - w.double()).abs() <= 2 * (2 * delta + 6000 * U + 2 * b) * mag).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,v,d", [(70001, 50, 16), (20000, 3, 9), (3, 70001, 1), (9, 2, 4100), (4100, 700, 8), (1, 300, 65536)])
+def test_lopsided_shapes(t, v, d, dtype):
+    check(t, v, d, dtype, t + 3 * v + d, scale=3.0)
+
+
+GUARD = 1 << 16
+
+
+def guarded(n, dtype):
+    """n values between two guards, 16 bytes past a larger border; and the whole buffer."""
+    size = torch.empty(0, dtype=dtype).element_size()
+    whole = torch.full((2 * GUARD + 16 + n * size,), 0x5a, dtype=torch.uint8, device="cuda")
+    at = GUARD + 16
+    return whole[at:at + n * size].view(dtype), whole, at, n * size
+
+
+def untouched(*buffers):
+    for _, whole, at, n in buffers:
+        assert (whole[:at] == 0x5a).all() and (whole[at + n:] == 0x5a).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,v,d", [(1, 1, 1), (5, 130, 7), (33, 700, 100), (70, 513, 65), (130, 1000, 260), (300, 40, 33)])
+def test_nothing_but_the_outputs_and_the_workspace_is_written(t, v, d, dtype):
+    """The C entries with a workspace of exactly the size asked for, 16-byte aligned and no more."""
+    import ctypes as C
+
+    from surfface_hip import _lib
+    L, kind = _lib.lib(), {torch.float32: _lib.MN_F32, torch.bfloat16: _lib.MN_BF16}[dtype]
+    q, c, at = make(t, v, d, dtype, 40)
+    n = C.c_size_t()
+    P = lambda g: C.c_void_p(g[0].data_ptr())
+    D = lambda x: C.c_void_p(x.data_ptr())
+    st = torch.cuda.current_stream().cuda_stream
+    f = lambda k: guarded(k, torch.float32)
+    rest, zt, loss, mean, share = f(t), f(t), f(t), f(1), f(1)
+    _lib.check(L.mn_softmax_workspace(t, v, d, kind, 0, C.byref(n)))
+    ws = guarded(n.value, torch.uint8)
+    _lib.check(L.mn_softmax_stats(D(q), D(c), kind, t, v, d, D(at), 0, 2.0, P(rest), P(zt), P(loss), P(mean), P(share),
+                                  P(ws), n.value, st))
+    _lib.check(L.mn_softmax_workspace(t, v, d, kind, 1, C.byref(n)))
+    wb = guarded(n.value, torch.uint8)
+    dq, dc = guarded(t * d, dtype), guarded(v * d, dtype)
+    one = torch.ones(1, device="cuda")
+    _lib.check(L.mn_softmax_backward(D(q), D(c), kind, t, v, d, D(at), 0, 2.0, P(rest), P(zt), D(one), 1, P(share), P(dq),
+                                     P(dc), P(wb), n.value, st))
+    untouched(rest, zt, loss, mean, share, ws, wb, dq, dc)
+    ld = (d + 15) // 16 * 16
+    qc, qs, cc, cs = guarded(t * ld, torch.int8), f(t), guarded(v * ld, torch.int8), f(v)
+    _lib.check(L.mn_quantize_rows_i8(D(q), kind, t, d, P(qc), ld, P(qs), st))
+    _lib.check(L.mn_quantize_rows_i8(D(c), kind, v, d, P(cc), ld, P(cs), st))
+    _lib.check(L.mn_scores_i8_workspace(t, d, C.byref(n)))
+    wi, y, back = guarded(n.value, torch.uint8), guarded(t * v, dtype), guarded(v * d, dtype)
+    _lib.check(L.mn_scores_i8(P(qc), ld, P(qs), t, P(cc), ld, P(cs), v, d, P(y), kind, P(wi), n.value, st))
+    _lib.check(L.mn_dequantize_rows_i8(P(cc), ld, P(cs), v, d, P(back), kind, st))
+    untouched(qc, qs, cc, cs, wi, y, back)
+
+
+def test_merge_of_many_ranges():
+    """200 ranges, one of them without any item but the target, against the sum in 64 bits."""
+    import surfface_hip as S
+    g = torch.Generator().manual_seed(50)
+    rests = torch.randn(200, 77, generator=g) * 30
+    rests[3] = -math.inf
+    zts = torch.full((200, 77), -math.inf)
+    zts[torch.randint(0, 200, (77,), generator=g), torch.arange(77)] = torch.randn(77, generator=g) * 30
+    at = torch.arange(77)
+    at[5], zts[:, 6] = -1, -math.inf
+    st = S.softmax_merge(rests.cuda(), zts.cuda(), at.cuda())
+    rest, zt = torch.logsumexp(rests.double(), 0), zts.max(0).values
+    want = torch.nn.functional.softplus(rest - zt.double(), threshold=1000)
+    want[5] = 0
+    # rest: 200 exponents and sums, off by 2^-24 of up to 200 / ln 2 and of their sum
+    tol = 2.0 ** -24 * (4 * rest.abs() + 800)
+    assert ((st.rest.double().cpu() - rest).abs() <= tol).all()
+    assert torch.equal(st.target.cpu(), zt) and torch.isinf(st.loss[6]) and st.loss[5] == 0 and torch.isinf(st.mean)
+    ok = torch.ones(77, dtype=torch.bool)
+    ok[6] = False
+    assert ((st.loss.double().cpu() - want).abs()[ok] <= (2 * tol + 4 * U * want)[ok]).all()
+    assert abs(float(st.share) * 76 - 1) <= 2 * U
+
+
 def test_threads_on_streams_of_their_own():
     """Two threads, a stream each, steps and scores at the same time: the results of one after the other."""
     import surfface_hip as S
