@@ -25,8 +25,8 @@
 // k_kn2_32 (rows times columns): each thread loads 24 values to registers, two
 // steps ahead, splits and writes them; a matrix with k in its rows is turned on
 // the way (a thread's 8 values are 8 k's of one column).  With D and the queries
-// as planes in memory, loaded directly and read transposed, it took 4% longer:
-// half as many bytes again come from L2.
+// as planes in memory, loaded directly and read transposed, it took as long (4%
+// longer to 2% less): half as many bytes again come from L2.
 //
 // 1024 x 100000 x 768: logits with the loss's sums 690 us (1.37 PFLOP/s of bf16
 // products, 228 TFLOP/s of f32 ones; the f32 matrix rate of a large library
@@ -309,8 +309,8 @@ __device__ __forceinline__ void kn32_tile(Planes &pl, const KnArgs &a, const EPI
     const int fr = lane & 15, fk = lane >> 4;
     const int s0 = z * a.steps, s1 = min(a.steps_all, s0 + a.steps), nstep = max(0, s1 - s0);
 
-    // pieces of i: as k_nt32, or column tid & 255, rows 8 (tid / 256) and 16
-    // more; of j: column tid % (32 NJ), rows 8 (tid / (32 NJ))
+    // pieces of i: rows tid / 4 and 128 more, 32 bytes at 32 (tid & 3), or column
+    // tid & 255, rows 8 (tid / 256) and 16 more; of j: column tid % (32 NJ), rows 8 (tid / (32 NJ))
     const int ri = A_T ? tid & 255 : tid >> 2, ki = A_T ? tid >> 8 : tid & 3;
     const int rj = tid % (32 * NJ), kj = tid / (32 * NJ);
     auto at = [](int r, int c) __attribute__((always_inline)) { return r * KBY + 16 * (c ^ quad_swizzle((r >> 2) & 3)); };

@@ -559,13 +559,21 @@ struct PartEpi {
     }
 };
 
+// dC of a piece, or partial sums of it (part not NULL)
 template <bool F32>
 struct GradEpi {
     void *out;
     int64_t m, n;
     const float *gs;
+    float *part;
+    int64_t ld;
     template <int NF>
-    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][NF], int64_t m0, int64_t n0, int lane, int) const {
+    __device__ __forceinline__ void operator()(mm::f32x4 (&acc)[4][NF], int64_t m0, int64_t n0, int lane, int z) const {
+        if (part) {
+            const PartEpi e = {part, m, ld, true};
+            e(acc, m0, n0, lane, z);
+            return;
+        }
         const float s = gs[0];
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
@@ -580,33 +588,46 @@ struct GradEpi {
     }
 };
 
-// dQ = factor (sum of the partials + resid c_target); a thread takes 4 columns
+// Joins partial sums: out = factor (their sum + resid c_target), a thread 4
+// columns; the second part only for dQ.
+struct Sums {
+    const float *part;       // [n][rows][ldp]
+    int n, blocks;
+    int64_t rows;
+    void *out;
+    const int64_t *targets;  // dQ: rows that have a part; NULL: dC
+};
 template <bool F32>
-__global__ __launch_bounds__(256) void k_reduce_dq(const float *__restrict__ part, int splits, int ldp, int64_t t, int d,
-                                                   const uint16_t *__restrict__ C, const Row *__restrict__ row,
-                                                   const int32_t *__restrict__ at,
-                                                   const int64_t *__restrict__ targets,
-                                                   const float *__restrict__ gs, void *__restrict__ dQ) {
+__device__ __forceinline__ void reduce(const Sums &p, int block, int ldp, int d, const uint16_t *C, const Row *row,
+                                       const int32_t *at, const float *gs) {
     const uint32_t n4 = ldp / 4;
-    const int64_t total = t * n4, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t total = p.rows * n4, e = (int64_t)block * 256 + threadIdx.x;
     if (e >= total) return;
     const int64_t i = total <= 0xffffffffll ? (int64_t)((uint32_t)e / n4) : e / n4;
     const int c = 4 * (int)(e - i * n4);
     mm::f32x4 x = (mm::f32x4)(0.f);
-    if (targets[i] >= 0) {
-        const mm::f32x4 *p = reinterpret_cast<const mm::f32x4 *>(part) + e;
+    if (!p.targets || p.targets[i] >= 0) {
+        const mm::f32x4 *src = reinterpret_cast<const mm::f32x4 *>(p.part) + e;
 #pragma unroll 8
-        for (int s = 0; s < splits; ++s) x += p[s * total];
-        if (!F32 && at[i] >= 0) {
+        for (int s = 0; s < p.n; ++s) x += src[s * total];
+        if (!F32 && p.targets && at[i] >= 0) {
             const float r = row[i].resid;
-            const uint16_t *src = C + (int64_t)at[i] * d + c;
+            const uint16_t *y = C + (int64_t)at[i] * d + c;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (c + q < d) x[q] += r * mm::bf16_value(src[q]);
+                if (c + q < d) x[q] += r * mm::bf16_value(y[q]);
         }
         x *= gs[0];
     }
-    mm::store4<F32>(dQ, i * d + c, min(4, d - c), x);
+    mm::store4<F32>(p.out, i * d + c, min(4, d - c), x);
+}
+template <bool F32>
+__global__ __launch_bounds__(256) void k_reduce(Sums dq, Sums dc, int ldp, int d, const uint16_t *__restrict__ C,
+                                                const Row *__restrict__ row, const int32_t *__restrict__ at,
+                                                const float *__restrict__ gs) {
+    const int b = (int)blockIdx.x;
+    if (b < dq.blocks) reduce<F32>(dq, b, ldp, d, C, row, at, gs);
+    else reduce<F32>(dc, b - dq.blocks, ldp, d, C, row, at, gs);
 }
 
 inline size_t up(size_t x) { return (x + 255) / 256 * 256; }
@@ -630,9 +651,10 @@ struct Plan {
     int64_t vc, vmax;   // items per piece (backward), of the longest piece, in whole tiles
     int nf;             // 32 nf columns a tile of dQ and dC
     int splits;         // of dQ's sum over a piece
+    int splits_c;       // of dC's sum over the queries
     int pieces, parts;  // of the table; partial sums of dQ in all
     bool apart;         // a piece's partial sums are its own
-    size_t q, planes, c, part, row, at, gs, D, dq, bytes;
+    size_t q, planes, c, part, row, at, gs, D, dq, dc, bytes;
 };
 
 inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
@@ -696,29 +718,35 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         if (all > piece && rest > 0 && piece + rest <= most) longest = piece + rest;
         p.vc = std::min(piece, all) * mm::TILE;
         p.vmax = longest * mm::TILE;
-        // dQ's runs of k: the cut with the least time for the blocks of both
-        // products on 256 processors, dQ's first, in steps: a block of dQ
-        // costs its run and 20 for its part of the sum (256 KB to memory), one
-        // of dC t / 32 and 10 (f32, whose steps take longer: 6 and 4).  Free
+        // The runs of k of both products: the cuts with the least time for
+        // their blocks on 256 processors, dQ's first, in steps: a block that
+        // writes partial sums costs its run and 20 (256 KB to memory), one that
+        // writes dC itself 10 (f32, whose steps take longer: 6 and 4).  Free
         // processors take the next block: dC's done by a time are counted from
-        // the two times at which dQ's blocks end.
+        // the two times at which dQ's blocks end.  dC's sum over the queries is
+        // only cut where its tiles do not fill the processors (3630 queries,
+        // 1384 x 64 items: 214 us without, 47 with in f32, 70 and 39 in bf16).
         p.nf = f32 ? (d > 64 ? 4 : 2) : d > 128 ? 8 : d > 64 ? 4 : 2;
-        const int64_t cols = (d + 32 * p.nf - 1) / (32 * p.nf), tiles = panels * cols;
-        const int64_t steps = p.vc / 32, nc = p.vc / mm::TILE * cols, b = t / 32 + (f32 ? 4 : 10);
+        const int64_t cols = (d + 32 * p.nf - 1) / (32 * p.nf), tiles = panels * cols, sum = f32 ? 6 : 20;
+        const int64_t steps = p.vc / 32, steps_c = (t + 31) / 32, nc1 = p.vc / mm::TILE * cols;
         int64_t best = INT64_MAX;
-        for (int64_t s = 1; s <= std::min<int64_t>(steps / 4 + 1, std::max<int64_t>(1, 512 / tiles)); ++s) {
-            const int64_t a = (steps + s - 1) / s + (f32 ? 6 : 20), nq = tiles * s, full = nq / 256 * a, more = nq % 256;
-            int64_t end = full + (more ? a : 0);
-            for (int64_t k = (nc + 255) / 256;; ++k) {
-                const int64_t e1 = full + k * b, e2 = std::max<int64_t>(0, e1 - full - a) / b;
-                if ((256 - more) * k + more * e2 >= nc) {
-                    end = std::max(end, e1);
-                    break;
+        for (int64_t sc = 1; sc == 1 || (sc * nc1 <= 256 && sc * 4 <= steps_c); sc *= 2) {
+            const int64_t nc = sc * nc1, b = (steps_c + sc - 1) / sc + (sc > 1 ? sum : f32 ? 4 : 10);
+            for (int64_t s = 1; s <= std::min<int64_t>(steps / 4 + 1, std::max<int64_t>(1, 512 / tiles)); ++s) {
+                const int64_t a = (steps + s - 1) / s + sum, nq = tiles * s, full = nq / 256 * a, more = nq % 256;
+                int64_t end = full + (more ? a : 0);
+                for (int64_t k = (nc + 255) / 256;; ++k) {
+                    const int64_t e1 = full + k * b, e2 = std::max<int64_t>(0, e1 - full - a) / b;
+                    if ((256 - more) * k + more * e2 >= nc) {
+                        end = std::max(end, e1);
+                        break;
+                    }
                 }
-            }
-            if (end < best) {
-                best = end;
-                p.splits = (int)s;
+                if (end < best) {
+                    best = end;
+                    p.splits = (int)s;
+                    p.splits_c = (int)sc;
+                }
             }
         }
         // every piece's partial sums apart (written once, read once) while
@@ -733,6 +761,7 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         p.ldd = p.vmax + 128 / p.size;  // an odd number of 128-byte lines: rows on different memory channels
         p.D = take((size_t)p.tp * p.ldd * p.size);
         p.dq = take((size_t)p.parts * t * p.ldp * 4);
+        p.dc = take(p.splits_c > 1 ? (size_t)p.splits_c * p.vmax * p.ldp * 4 : 0);
     }
     p.bytes = o;
     return p;
@@ -899,12 +928,14 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         gc.ldb = (int64_t)p.kp * p.size;
         gc.B = w + p.q;
         gc.k = t;
-        gc.steps_all = gc.steps = (int)((t + 31) / 32);
+        gc.steps_all = (int)((t + 31) / 32);
+        gc.steps = (gc.steps_all + p.splits_c - 1) / p.splits_c;
         const mm::KnGrid nq = {dQ ? col_tiles : 0, row_tiles, p.splits};
-        const mm::KnGrid nc = {dC ? col_tiles : 0, (int)((vn + mm::TILE - 1) / mm::TILE), 1};
+        const mm::KnGrid nc = {dC ? col_tiles : 0, (int)((vn + mm::TILE - 1) / mm::TILE), p.splits_c};
         const PartEpi pe = {(float *)(w + p.dq) + (p.apart ? (int64_t)piece * p.splits * t * p.ldp : 0), t, p.ldp,
                             p.apart || piece == 0};
-        const GradEpi<F32> ge = {(char *)dC + j0 * d * (F32 ? 4 : 2), vn, d, gs};
+        char *out = (char *)dC + j0 * d * (F32 ? 4 : 2);
+        const GradEpi<F32> ge = {out, vn, d, gs, p.splits_c > 1 ? (float *)(w + p.dc) : nullptr, p.ldp};
         auto go = [&](auto NF) {
             constexpr int n = decltype(NF)::value;
             const dim3 grid((unsigned)(nq.blocks() + nc.blocks()));
@@ -917,11 +948,17 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         else if (p.nf == 2) go(std::integral_constant<int, 2>());
         else if constexpr (!F32) go(std::integral_constant<int, 8>());
         MN_KCHECK(s, "k_kn2");
-    }
-    if (dQ) {
-        hipLaunchKernelGGL(k_reduce_dq<F32>, dim3((unsigned)((t * (p.ldp / 4) + 255) / 256)), dim3(256), 0, s,
-                           (const float *)(w + p.dq), p.parts, p.ldp, t, d, (const uint16_t *)C, row, at, targets, gs, dQ);
-        MN_KCHECK(s, "k_reduce_dq");
+        const bool last = j0 + vn >= v;
+        auto sums = [&](size_t part, int n, int64_t rows, void *to, const int64_t *tg) {
+            return Sums{(const float *)(w + part), n, (int)((rows * (p.ldp / 4) + 255) / 256), rows, to, tg};
+        };
+        const Sums sq = dQ && last ? sums(p.dq, p.parts, t, dQ, targets) : Sums{};
+        const Sums sd = dC && p.splits_c > 1 ? sums(p.dc, p.splits_c, vn, out, nullptr) : Sums{};
+        if (sq.blocks + sd.blocks > 0) {
+            hipLaunchKernelGGL(k_reduce<F32>, dim3((unsigned)(sq.blocks + sd.blocks)), dim3(256), 0, s, sq, sd, p.ldp, d,
+                               (const uint16_t *)C, row, at, gs);
+            MN_KCHECK(s, "k_reduce");
+        }
     }
     return MN_OK;
 }

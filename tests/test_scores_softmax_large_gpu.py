@@ -195,7 +195,7 @@ def test_items_masked_with_the_lowest_value(dtype, t):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("t,v,d", [(70001, 50, 16), (20000, 3, 9), (3, 70001, 1), (9, 2, 4100), (4100, 700, 8), (1, 300, 65536)])
+@pytest.mark.parametrize("t,v,d", [(70001, 50, 16), (20000, 3, 9), (3, 70001, 1), (9, 2, 4100), (4100, 700, 8), (1, 300, 65536), (262144, 1300, 20), (5003, 600, 200)])
 def test_lopsided_shapes(t, v, d, dtype):
     check(t, v, d, dtype, t + 3 * v + d, scale=3.0)
 
@@ -217,7 +217,7 @@ def untouched(*buffers):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("t,v,d", [(1, 1, 1), (5, 130, 7), (33, 700, 100), (70, 513, 65), (130, 1000, 260), (300, 40, 33)])
+@pytest.mark.parametrize("t,v,d", [(1, 1, 1), (5, 130, 7), (33, 700, 100), (70, 513, 65), (130, 1000, 260), (300, 40, 33), (2000, 40, 70)])
 def test_nothing_but_the_outputs_and_the_workspace_is_written(t, v, d, dtype):
     """The C entries with a workspace of exactly the size asked for, 16-byte aligned and no more."""
     import ctypes as C
