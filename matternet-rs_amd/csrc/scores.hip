@@ -42,6 +42,9 @@ __device__ __forceinline__ void load8(const T *row, int k, int d, bool vec, floa
     }
 }
 
+// threads a block, whole rows of L lanes
+constexpr int quantize_block(int L) { return L > 64 ? L : 256; }
+
 // L lanes take a row, 8 values a lane at a time; up to 16 values a lane stay in
 // registers between the two passes: such rows are read once, past the caches
 // (262144 x 768 f32 and back: 314 us, 5.8 TB/s; 339 with ordinary loads); longer
@@ -53,11 +56,11 @@ __device__ __forceinline__ void load8(const T *row, int k, int d, bool vec, floa
 // row of zeros has scale 0 and codes 0; a row that holds an infinity or a NaN
 // has scale NaN, which every score with it shows.
 template <typename T, int L>
-__global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64_t n, int d, bool vec,
+__global__ __launch_bounds__(quantize_block(L)) void k_quantize(const T *__restrict__ X, int64_t n, int d, bool vec,
                                                   int8_t *__restrict__ codes, int64_t ld,
                                                   float *__restrict__ scale) {
     const int l = threadIdx.x % L;
-    const int64_t i = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const int64_t i = (int64_t)blockIdx.x * (quantize_block(L) / L) + threadIdx.x / L;
     if (i >= n) return;  // whole groups of L lanes
     const T *row = X + i * d;
     float v[2][8];
@@ -80,7 +83,14 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ X, int64
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
     }
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    for (int o = std::min(L, 64) / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    if constexpr (L > 64) {  // a row a block
+        __shared__ uint32_t tops[L / 64];
+        if (l % 64 == 0) tops[l / 64] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < L / 64; ++w) top = max(top, tops[w]);
+    }
     const float a = __uint_as_float(top);
     const bool finite = top < 0x7f800000u;
     const float up = a < 0x1p-100f ? 0x1p64f : a > 0x1p100f ? 0x1p-64f : 1.f;
@@ -284,13 +294,15 @@ struct FewScoreEpi {
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-// lanes a row: the power of two that takes ld in one turn, 2 to 64
+// lanes a row: the power of two that takes ld in one turn, 2 to 64, and a block
+// of 128, 256 or 1024 for rows that do not fit a wave's registers (8 x 65536 f32:
+// 62 us with a wave a row, 8.5 so; 65536 x 1536 bf16: 55 and 57)
 template <typename T>
 void quantize(const T *X, int64_t n, int d, int8_t *codes, int64_t ld, float *scale, hipStream_t s) {
     const bool vec = (d * sizeof(T)) % 16 == 0 && aligned16(X);
     auto go = [&](auto L) {
-        constexpr int l = decltype(L)::value, per = 256 / l;
-        hipLaunchKernelGGL((k_quantize<T, l>), dim3((unsigned)((n + per - 1) / per)), dim3(256), 0, s, X, n, d, vec, codes,
+        constexpr int l = decltype(L)::value, block = quantize_block(l), per = block / l;
+        hipLaunchKernelGGL((k_quantize<T, l>), dim3((unsigned)((n + per - 1) / per)), dim3(block), 0, s, X, n, d, vec, codes,
                            ld, scale);
     };
     if (ld <= 16) go(std::integral_constant<int, 2>());
@@ -298,7 +310,10 @@ void quantize(const T *X, int64_t n, int d, int8_t *codes, int64_t ld, float *sc
     else if (ld <= 64) go(std::integral_constant<int, 8>());
     else if (ld <= 128) go(std::integral_constant<int, 16>());
     else if (ld <= 256) go(std::integral_constant<int, 32>());
-    else go(std::integral_constant<int, 64>());
+    else if (ld <= 1024) go(std::integral_constant<int, 64>());
+    else if (ld <= 2048) go(std::integral_constant<int, 128>());
+    else if (ld <= 4096) go(std::integral_constant<int, 256>());
+    else go(std::integral_constant<int, 1024>());
 }
 
 inline int padded(int d) { return (d + mm::KBY - 1) / mm::KBY * mm::KBY; }
@@ -321,8 +336,8 @@ extern "C" int mn_quantize_rows_i8(const void *X, int32_t x_type, int64_t n, int
                                    int8_t *codes, int64_t ld, float *scale, void *stream) {
     using namespace mn::i8;
     mn::clear_error();
-    MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX - 4096, MN_EINVAL,
-               "mn_quantize_rows_i8: n >= 0, d >= 1, ld >= d, a multiple of 16 and < 2^31 - 4096 needed");
+    MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX - 16384, MN_EINVAL,
+               "mn_quantize_rows_i8: n >= 0, d >= 1, ld >= d, a multiple of 16 and < 2^31 - 16384 needed");
     MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 256 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
                "mn_quantize_rows_i8: n < 2^31 - 1 rows and n d < 2^40 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_quantize_rows_i8: MN_F32 or MN_BF16");
@@ -340,8 +355,8 @@ extern "C" int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const floa
                                      int32_t d, void *X, int32_t x_type, void *stream) {
     using namespace mn::i8;
     mn::clear_error();
-    MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX - 4096, MN_EINVAL,
-               "mn_dequantize_rows_i8: n >= 0, d >= 1, ld >= d, a multiple of 16 and < 2^31 - 4096 needed");
+    MN_REQUIRE(n >= 0 && d >= 1 && ld >= d && ld % 16 == 0 && ld <= INT_MAX - 16384, MN_EINVAL,
+               "mn_dequantize_rows_i8: n >= 0, d >= 1, ld >= d, a multiple of 16 and < 2^31 - 16384 needed");
     MN_REQUIRE(n < INT_MAX && n * ((d + 3) / 4) / 256 < INT_MAX && d < INT_MAX - 4096, MN_ENOTSUP,
                "mn_dequantize_rows_i8: n < 2^31 - 1 rows and n d < 2^40 needed");
     MN_REQUIRE(x_type == MN_F32 || x_type == MN_BF16, MN_ENOTSUP, "mn_dequantize_rows_i8: MN_F32 or MN_BF16");

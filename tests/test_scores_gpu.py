@@ -32,7 +32,8 @@ def rows(n, d, seed, dtype=torch.float32):
     return x.to(dtype)
 
 
-@pytest.mark.parametrize("n,d", [(1, 1), (3, 15), (5, 16), (7, 17), (64, 64), (33, 96), (130, 768), (5, 1025), (2, 4099)])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 15), (5, 16), (7, 17), (64, 64), (33, 96), (130, 768), (5, 1025), (2, 4099), (3, 1536), (7, 2048),
+                                 (2, 2064), (3, 4112), (2, 16400), (1, 40001)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_quantize_is_the_formula_bit_for_bit(n, d, dtype):
     import surfface_hip as S
@@ -69,6 +70,21 @@ def test_quantize_rows_at_the_borders():
     np.testing.assert_array_equal(r.codes.cpu().numpy()[:, :20], codes)
     np.testing.assert_array_equal(r.scale.cpu().numpy(), scale)
     assert np.isnan(scale[6:8]).all() and codes[9, :4].tolist() == [0, 2, -2, 127]
+
+
+@pytest.mark.parametrize("d", [1100, 2100, 5000, 33000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_rows_that_are_not_finite(d, dtype):
+    """The largest value, an infinity and a NaN at either end of a row that several waves share."""
+    import surfface_hip as S
+    x = torch.randn(6, d, generator=torch.Generator().manual_seed(d)).to(dtype)
+    x[0, -1], x[1, 0], x[2, -1], x[3, 0] = 300.0, -300.0, float("nan"), float("-inf")
+    x[4] = 0
+    r = S.quantize_rows(x.cuda())
+    codes, scale = quantize_ref(x.float().numpy())
+    np.testing.assert_array_equal(r.codes.cpu().numpy()[:, :d], codes)
+    np.testing.assert_array_equal(r.scale.cpu().numpy(), scale)
+    assert np.isnan(scale[2:4]).all() and codes[0, -1] == 127 and codes[1, 0] == -127
 
 
 def check_scores(q, qs, c, cs, d, dtype, got):
