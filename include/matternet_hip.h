@@ -643,7 +643,7 @@ int mn_bf16_last_stats(mn_knn_stats *out);
  * among them; its contents mean nothing between calls.  Q, C, codes and the
  * workspace are 16-byte aligned (MN_EINVAL / MN_ECAP otherwise), X need not be.
  * Matrices are row-major and dense but for codes, whose rows are `ld` bytes
- * apart (a multiple of 16, >= d). */
+ * apart (a multiple of 16, >= d, below 2^31 - 16384). */
 
 /* Per row a = max |x|: scale = a / 127, code = rint(x (127 (1 / a))) (f32, ties to
  * even), codes d .. ld - 1 of a row 0.  X [n][d] MN_F32 or MN_BF16.  A row of

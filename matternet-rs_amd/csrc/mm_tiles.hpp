@@ -345,6 +345,17 @@ inline bool plan_few(FewArgs &a, bool split) {
     return true;
 }
 
+// Whether k_few takes less time than k_nt for more than 64 queries, by what both
+// take, in us (int8 and bf16): few problems have tiles enough to hide a tile's
+// start and end.  tile: that of a tile of k_nt beside its k-steps.  Scores of m x
+// n x d to f32: 128 x 16000 x 768 9.2 us by k_few, 20.1 by k_nt; 512 x 16000 x 768
+// 23.1, 22.1; 1000 x 4000 x 64 7.0, 17.2; 1000 x 64000 x 256 89, 70.
+inline bool few_faster(const FewArgs &a, const NtArgs &nt, double tile) {
+    const double few = 3 + 16.0 * a.mf * a.groups * a.n * (1.6e-7 * a.nk + 6e-7);
+    const int64_t rounds = ((int64_t)nt.panels * nt.slices + 255) / 256;
+    return a.groups <= 32 && few < 0.9 * (4 + (double)rounds * nt.run * (tile + 0.75 * nt.nk));
+}
+
 template <class OP, int MF, int LDSB, class EPI>
 __global__ __launch_bounds__(NT) void k_few(FewArgs a, EPI epi) {
     __shared__ alignas(16) char qs[LDSB];

@@ -318,15 +318,19 @@ void quantize(const T *X, int64_t n, int d, int8_t *codes, int64_t ld, float *sc
 
 inline int padded(int d) { return (d + mm::KBY - 1) / mm::KBY * mm::KBY; }
 
-// up to 64 queries of up to 144 KB go to k_few, which needs none
-inline bool few_args(mm::FewArgs &a, int64_t m, int d) {
-    a.m = (int)std::min<int64_t>(m, 65);
+// Up to 64 queries that fit LDS go to k_few, which needs no workspace; more where
+// it is the faster by the time of both (mm::few_faster).
+inline bool fits_few(mm::FewArgs &a, int64_t m, int d) {
+    a.m = (int)m;
     a.qbytes = d;
     return m <= 64 && mm::plan_few(a, false);
 }
+inline bool few_args(mm::FewArgs &a, const mm::NtArgs &nt, int64_t m, int d) {
+    return fits_few(a, m, d) || (mm::plan_few(a, true) && mm::few_faster(a, nt, 10));
+}
 inline size_t workspace(int64_t m, int d) {
     mm::FewArgs few = {};
-    return d % mm::KBY == 0 || few_args(few, m, d) ? 0 : (size_t)m * padded(d);
+    return d % mm::KBY == 0 || fits_few(few, m, d) ? 0 : (size_t)m * padded(d);
 }
 
 }  // namespace i8
@@ -406,15 +410,26 @@ extern "C" int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, 
     if (m == 0 || n == 0) return MN_OK;
     MN_REQUIRE(Q && q_scale && C && c_scale && Y, MN_EINVAL, "mn_scores_i8: NULL pointer");
     MN_REQUIRE(aligned16(Q) && aligned16(C), MN_EINVAL, "mn_scores_i8: codes not 16-byte aligned");
+    const size_t need = workspace(m, d);
+    MN_REQUIRE(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), MN_ECAP,
+               "mn_scores_i8: workspace of %zu bytes (16-byte aligned) needed", need);
     const int ldp = padded(d);
     hipStream_t s = (hipStream_t)stream;
+    mm::NtArgs a = {};
+    a.B = (const char *)C;
+    a.ldb = ldc;
+    a.m = m;
+    a.n = n;
+    a.nk = ldp / mm::KBY;
+    a.bmax = (d + 15) / 16 * 16 - 16;
+    mm::plan_runs(a);
     mm::FewArgs few = {};
     few.Q = (const char *)Q;
     few.B = (const char *)C;
     few.ldq = ldq;
     few.ldb = ldc;
     few.n = n;
-    if (few_args(few, m, d)) {
+    if (few_args(few, a, m, d)) {
         auto go = [&](auto out, auto MF) {
             typedef decltype(out) T;
             FewScoreEpi<T, decltype(MF)::value> epi = {};
@@ -435,28 +450,15 @@ extern "C" int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, 
         MN_KCHECK(s, "k_few");
         return MN_OK;
     }
-    const size_t need = workspace(m, d);
-    MN_REQUIRE(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), MN_ECAP,
-               "mn_scores_i8: workspace of %zu bytes (16-byte aligned) needed", need);
-    const int8_t *A = Q;
-    int64_t lda = ldq;
+    a.A = (const char *)Q;
+    a.lda = ldq;
     if (need) {
         const unsigned grid = (unsigned)std::min<int64_t>((m * ldp + 255) / 256, 8192);
         hipLaunchKernelGGL(k_pad_codes, dim3(grid), dim3(256), 0, s, Q, ldq, m, d, ldp, (int8_t *)ws);
         MN_KCHECK(s, "k_pad_codes");
-        A = (const int8_t *)ws;
-        lda = ldp;
+        a.A = (const char *)ws;
+        a.lda = ldp;
     }
-    mm::NtArgs a = {};
-    a.A = (const char *)A;
-    a.B = (const char *)C;
-    a.lda = lda;
-    a.ldb = ldc;
-    a.m = m;
-    a.n = n;
-    a.nk = ldp / mm::KBY;
-    a.bmax = (d + 15) / 16 * 16 - 16;
-    mm::plan_runs(a);
     const dim3 grid((unsigned)(a.panels * a.slices));
     if (y_type == MN_F32) {
         ScoreEpi<float> epi = {};

@@ -686,17 +686,19 @@ inline Plan make_plan(int64_t t, int64_t v, int d, bool f32, bool backward) {
         p.few.ldq = p.few.ldb = p.ldc;
         p.few.qbytes = (int)p.ldc;
         mm::plan_runs(p.nt, p.tile);
-        if (!mm::plan_few(p.few, f32)) {
+        if (!mm::plan_few(p.few, f32 || t > 64)) {
             p.few.slices = 0;
+        } else if (t > 64 && !f32) {
+            if (!mm::few_faster(p.few, p.nt, 7)) p.few.slices = 0;
         } else if (t > 64) {
-            // f32: also where there are too few tiles for the processors, by
-            // the rate of k_few's products (85 TFLOP/s) and the time of a step
-            // of k_nt32 (2.3 us, 256 blocks at a time), and 8 blocks a group
+            // where there are too few tiles for the processors, by the rate of
+            // k_few's products (85 TFLOP/s) and the time of a step of k_nt32
+            // (2.3 us, 256 blocks at a time), and 8 blocks a group
             // have a processor each: 192 queries on 3000 x 768 take 31 us so,
             // 58 by k_nt32, 1024 on 1500 x 2048 (64 groups) 155 and 138
             const double few_us = 16.0 * p.few.mf * p.few.groups * v * p.kp * 2 / 85e6;
             const double nt_us = 2.3 * p.nt.nk * p.nt.run * (((int64_t)p.nt.panels * p.nt.slices + 255) / 256);
-            if (!f32 || p.few.groups > 32 || few_us > 0.8 * nt_us) p.few.slices = 0;
+            if (p.few.groups > 32 || few_us > 0.8 * nt_us) p.few.slices = 0;
         }
         const bool few = p.few.slices > 0;
         p.q = take(few ? (p.few_q ? 0 : (size_t)t * p.kp * p.size) : f32 ? 0 : (size_t)t * p.kp * 2);

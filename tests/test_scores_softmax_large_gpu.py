@@ -112,6 +112,36 @@ def test_groups_of_queries_in_f32(t, v, d):
     check(t, v, d, torch.float32, t + v, scale=4.0)
 
 
+@pytest.mark.parametrize("t,v,d", [(2049, 10001, 33), (2000, 10003, 64), (701, 30011, 40), (1025, 20001, 129), (300, 60001, 768),
+                                   (4097, 6007, 16), (3000, 9001, 1), (2500, 8192, 1000), (70, 60001, 775)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tiles_with_odd_ends(t, v, d, dtype):
+    """Enough tiles that both passes go to the kernels of 256 x 256 (128) tiles; ends inside a tile and a k-step."""
+    check(t, v, d, dtype, t + v + d, scale=5.0)
+
+
+@pytest.mark.parametrize("m,n,d", [(2049, 16001, 33), (1999, 16003, 64), (4097, 8200, 768), (513, 64001, 100), (70, 90001, 769),
+                                   (3001, 20011, 1), (2050, 9003, 200), (256, 131072, 192), (65, 60001, 2000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_in_tiles_with_odd_ends(m, n, d, dtype):
+    import surfface_hip as S
+    g = torch.Generator(device="cuda").manual_seed(m + n + d)
+    q, c = S.quantize_rows(torch.randn(m, d, generator=g, device="cuda")), S.quantize_rows(torch.randn(n, d, generator=g, device="cuda"))
+    y = S.scores_i8(q, c, dtype)
+    for j in range(0, n, CHUNK):
+        exact = (q.codes[:, :d].double() @ c.codes[j:j + CHUNK, :d].double().T) * q.scale.double()[:, None] * \
+            c.scale[j:j + CHUNK].double()
+        tol = exact.abs() * (3.01 * U + (B if dtype == torch.bfloat16 else 0)) + 1e-44
+        assert worst(y[:, j:j + CHUNK], exact, tol) <= 1
+
+
+@pytest.mark.parametrize("m,n,d", [(65, 1500, 64), (700, 3001, 384), (1000, 1003, 1025), (130, 40001, 33), (2040, 50, 65),
+                                   (100, 200, 9000), (300, 77, 40000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_of_groups_of_queries(m, n, d, dtype):
+    test_scores_in_tiles_with_odd_ends(m, n, d, dtype)
+
+
 @pytest.mark.parametrize("m,d", [(1, 2560), (16, 2561), (16, 9216), (3, 9217), (17, 1280), (32, 1281), (32, 4608), (20, 4609),
                                  (33, 640), (64, 641), (64, 2304), (64, 2305)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
