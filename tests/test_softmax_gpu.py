@@ -375,6 +375,47 @@ def test_capture_of_the_loss():
             assert torch.equal(o, w)
 
 
+def test_autograd_rules():
+    """Gradients add up, a kept graph gives the same bits, what torch forbids is refused, a table that is its
+    own queries, views (strided, expanded)."""
+    import surfface_hip as S
+    q, c, at = (x.cuda() for x in data(100, 300, 40, torch.float32, 33))
+    q.requires_grad_(), c.requires_grad_()
+    S.softmax_loss(q, c, at).backward()
+    once = c.grad.clone()
+    S.softmax_loss(q, c, at).backward()
+    assert torch.equal(c.grad, 2 * once)
+    loss = S.softmax_loss(q, c, at)
+    a = torch.autograd.grad(loss, c, retain_graph=True)[0]
+    assert torch.equal(a, torch.autograd.grad(loss, c)[0])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, c)
+    first = torch.autograd.grad(S.softmax_loss(q, c, at), c, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), c)
+    loss = S.softmax_loss(q, c, at)
+    with torch.no_grad():
+        c.mul_(2)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+    g = torch.Generator().manual_seed(34)
+    x, t = torch.randn(200, 32, generator=g), torch.arange(200)
+    xg = x.cuda().requires_grad_()
+    got = torch.autograd.grad(S.softmax_loss(xg, xg, t.cuda(), 0.5), xg)[0]
+    _, w_dq, w_dc, s_dq, s_dc, delta = formula(x, x, t, 0.5)
+    close(got, w_dq + w_dc, (2 * delta + (6 * 200 + 64) * U) * (s_dq + s_dc) + 3 * U * (w_dq.abs() + w_dc.abs()), "own queries")
+
+    wide = torch.randn(200, 64, generator=g)
+    wg = wide.cuda().requires_grad_()
+    dq, = torch.autograd.grad(S.softmax_loss(wg[:, ::2], xg.detach(), t.cuda(), 0.5), wg)
+    _, w_dq, _, s_dq, _, delta = formula(wide[:, ::2].contiguous(), x, t, 0.5)
+    assert not dq[:, 1::2].any()
+    close(dq[:, ::2], w_dq, (2 * delta + (6 * 200 + 64) * U) * s_dq + U * w_dq.abs(), "strided")
+    e = torch.randn(5, 1, generator=g).cuda().expand(5, 32)
+    assert torch.equal(S.softmax_loss(e, xg.detach(), t[:5].cuda()), S.softmax_loss(e.contiguous(), xg.detach(), t[:5].cuda()))
+
+
 def test_empty_batch_and_refusals():
     import surfface_hip as S
     q, c, at = (x.cuda() for x in data(8, 30, 16, torch.float32, 1))
