@@ -682,6 +682,9 @@ int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, 
  * NULL (device).  It writes dC [v][d], this range's rows' gradient, and dQ
  * [t][d], this range's part of the queries' (add up the ranges'); either may be
  * NULL.  Types as Q and C.
+ * A grad that is not finite makes its row of dQ and all of dC NaN, and no other
+ * row of dQ.  Rows are taken relative to the largest finite |grad|: what is
+ * below 2^-126 of it may be lost.
  * bf16: the entries (p - [target]) of the logits' gradient are rounded to bf16
  * for the two products with C and Q (dQ gets the target's rounding back); sums
  * are f32.  f32: products of three-way split bf16 values, to f32 accuracy.

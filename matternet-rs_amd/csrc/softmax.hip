@@ -25,9 +25,10 @@ namespace sm {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
-// Per row for the gradients.  rel = g_i / max |g|, so that D = rel (p - [t])
-// is rounded to bf16 without the common factor; dt = rel times the target's
-// entry; resid = dt less its rounding (bf16 operands: added to dQ in f32).
+// Per row for the gradients.  rel = g_i / max |g| (of the finite g), so that D =
+// rel (p - [t]) is rounded to bf16 without the common factor; a g that is not
+// finite gives NaN and leaves the other rows' factor alone.  dt = rel times the
+// target's entry; resid = dt less its rounding (bf16 operands: added to dQ in f32).
 struct Row {
     float rel, lse2, dt, resid;
 };
@@ -157,6 +158,10 @@ struct FewStatsEpi {
     }
 };
 
+// |g|, 0 where it is not finite; the factor that the rows are relative to
+__device__ __forceinline__ float finite_abs(float g) { return fabsf(g) < __builtin_inff() ? fabsf(g) : 0.f; }
+__device__ __forceinline__ float grad_top(float most) { return most > 0.f ? most : 1.f; }
+
 __device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
 
 // What the rows need before the products: forward the targets' logits (a wave
@@ -172,7 +177,7 @@ struct Rows {
     const float *grad, *grad_scale;
     int64_t grad_n;
     float scale;
-    float *gs;             // [0] the factor of every gradient, [1] max |g| (grad_n > 1: of k_grad_max)
+    float *gs;             // [0] the factor of every gradient, [1] the largest finite |g| (grad_n > 1: of k_grad_max)
     Row *row;
     int32_t *at;
 };
@@ -203,7 +208,7 @@ __device__ __forceinline__ void rows(const Rows &p, int block) {
     }
     const int64_t i = (int64_t)block * 256 + threadIdx.x;
     if (i >= p.tp) return;
-    const float top = p.grad_n == 1 ? fabsf(p.grad[0]) : p.gs[1];
+    const float top = grad_top(p.grad_n == 1 ? finite_abs(p.grad[0]) : p.gs[1]);
     if (i == 0) p.gs[0] = (p.grad_scale ? top * p.grad_scale[0] : top) * p.scale;
     // no part (or only there to fill a tile, where the last query's logits of any
     // size are computed again): exp(z - inf) = 0
@@ -214,10 +219,10 @@ __device__ __forceinline__ void rows(const Rows &p, int block) {
         const float g = p.grad_n == 1 ? p.grad[0] : p.grad[i];
         const float inf = __builtin_inff();
         const float re = p.rest[i], z = p.zt[i];
-        r.rel = top == 0.f ? 0.f : g / top;
+        r.rel = fabsf(g) < inf ? g / top : __builtin_nanf("");
         const float lse = re == -inf ? z : z == -inf ? re : z + softplus(re - z);
         r.lse2 = lse * kLog2e;
-        r.dt = re == -inf ? 0.f : -r.rel / (1.f + expf(z - re));
+        r.dt = re == -inf ? 0.f * r.rel : -r.rel / (1.f + expf(z - re));
         if (tl >= 0 && tl < p.v) {
             a = (int32_t)tl;
             if (!F32) r.resid = r.dt - mm::bf16_value(mm::bf16_bits(r.dt));
@@ -451,12 +456,12 @@ __global__ __launch_bounds__(1024) void k_join_few(const float2 *__restrict__ pa
     }
 }
 
-// gs[1] = the largest |g| of the rows that take part
+// gs[1] = the largest finite |g| of the rows that take part
 __global__ __launch_bounds__(1024) void k_grad_max(const float *__restrict__ grad, int64_t t,
                                                    const int64_t *__restrict__ targets, float *__restrict__ gs) {
     __shared__ float sh[16];
     float top = 0.f;
-    for (int64_t i = threadIdx.x; i < t; i += 1024) top = fmaxf(top, targets[i] >= 0 ? fabsf(grad[i]) : 0.f);
+    for (int64_t i = threadIdx.x; i < t; i += 1024) top = fmaxf(top, targets[i] >= 0 ? finite_abs(grad[i]) : 0.f);
     top = block_fold(top, sh, [](float a, float b) { return fmaxf(a, b); });
     if (threadIdx.x == 0) gs[1] = top;
 }
