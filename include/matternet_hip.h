@@ -686,7 +686,7 @@ int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, 
  * row of dQ.  Rows are taken relative to the largest finite |grad|: what is
  * below 2^-126 of it may be lost.
  * bf16: the entries (p - [target]) of the logits' gradient are rounded to bf16
- * for the two products with C and Q (dQ gets the target's rounding back); sums
+ * for the two products with C and Q (both get the target's rounding back); sums
  * are f32.  f32: products of three-way split bf16 values, to f32 accuracy.
  * Results do not depend on the run: no atomics. */
 int mn_softmax_workspace(int64_t t, int64_t v, int32_t d, int32_t x_type, int32_t backward,

@@ -457,12 +457,119 @@ struct KnArgs {
     int steps_all;
 };
 
+// A fragment of [32 k][256] (16-column slot s), read transposed: row 8 fk + (fr >>
+// 2) and 4 below
+__device__ __forceinline__ u32x4 read_turned(const char *half, int s, int fr, int fk) {
+    const char *p = half + (8 * fk + (fr >> 2)) * 512 + 8 * (fr & 3) + 32 * (s ^ ((fr >> 2) | ((fk & 1) << 2)));
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * 512));
+    const uint2 a2 = __builtin_bit_cast(uint2, x), b2 = __builtin_bit_cast(uint2, y);
+    return (u32x4){a2.x, a2.y, b2.x, b2.y};
+}
+
+// One more entry for each k of A [k][m], x[k * stride] (as bf16) at column at[k] -
+// first where that is among the columns; at < 0: none.
+struct KnExtra {
+    const int32_t *at;
+    const float *x;
+    int stride;
+    int64_t first;
+};
+constexpr int EXTRA_SCAN = 8;   // entries of at that a thread looks at together
+constexpr int EXTRA_GROUPS = 3; // ring slots of 32 entries; the fourth holds the list
+
+// The extra entries of a tile, after its steps: the k's whose column is in the
+// tile are listed (in their order: the sums are the same every time), and 32 of
+// them are a step of their own, with gathered rows of B.  It costs a step of the
+// softmax loss of 4096 x 131072 x 768 1% (3.04 -> 3.08 ms), one of 70001 x 40 x 256,
+// where every k's column is in the tile, 10% (241 -> 266 us).
+template <int NF>
+__device__ __forceinline__ void add_extra(Ring &rg, int (&counts)[64], const KnArgs &a, const KnExtra &x, f32x4 (&acc)[4][NF],
+                                          int64_t m0, int64_t n0, int s0, int s1) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wi = w & 3, wj = w >> 2;
+    const int fr = lane & 15, fk = lane >> 4;
+    auto turned = [](int k) __attribute__((always_inline)) { return (k & 3) | (((k >> 3) & 1) << 2); };
+    uint2 *list = reinterpret_cast<uint2 *>(&rg.b[EXTRA_GROUPS][0][0]);  // k; column, value
+    const int64_t first = x.first + m0, k1 = min<int64_t>(a.k, 32 * (int64_t)s1);
+    const char *b = a.B + 2 * n0;
+    for (int64_t c0 = 32 * (int64_t)s0; c0 < k1; c0 += EXTRA_SCAN * NT) {
+        int at[EXTRA_SCAN];
+#pragma unroll
+        for (int u = 0; u < EXTRA_SCAN; ++u) {
+            const int64_t k = c0 + NT * u + tid;
+            at[u] = k < k1 ? x.at[k] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < EXTRA_SCAN; ++u) {
+            const int64_t m = at[u] - first;
+            at[u] = at[u] >= 0 && m >= 0 && m < TILE ? (int)m : -1;
+            const uint64_t in = __ballot(at[u] >= 0);
+            if (lane == 0) counts[8 * u + w] = __popcll(in);
+        }
+        __syncthreads();  // the steps' loads and reads have ended too
+        int sum = counts[lane];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(sum, o);
+            sum += lane >= o ? y : 0;
+        }
+        const int total = __builtin_amdgcn_readfirstlane(__shfl(sum, 63));
+#pragma unroll
+        for (int u = 0; u < EXTRA_SCAN; ++u) {
+            const uint64_t in = __ballot(at[u] >= 0);
+            const int end = __shfl(sum, 8 * u + w);
+            if (at[u] >= 0) {
+                const int64_t k = c0 + NT * u + tid;
+                const uint32_t v = __builtin_bit_cast(uint16_t, (__bf16)x.x[k * x.stride]);
+                list[end - __popcll(in >> lane)] = make_uint2((uint32_t)k, (uint32_t)at[u] | v << 16);
+            }
+        }
+        __syncthreads();
+        for (int e0 = 0; e0 < total; e0 += 32 * EXTRA_GROUPS) {
+            const int n = min(32 * EXTRA_GROUPS, total - e0), groups = (n + 31) / 32;
+            for (int h = 0; h < groups; ++h)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int k = 4 * w + 2 * p + (lane >> 5), e = e0 + 32 * h + k;
+                    const int c = 16 * ((((lane & 31) >> 1) ^ turned(k)) * 2 + (lane & 1));
+                    u32x4 y = (u32x4)(0u);
+                    if (e < total) y = *reinterpret_cast<const u32x4 *>(b + list[e].x * a.ldb + min<int64_t>(c, a.ldb - 16 - 2 * n0));
+                    const int to = 2048 * w + 1024 * p + 16 * lane;
+                    *reinterpret_cast<u32x4 *>(&rg.b[h][0][to]) = (u32x4)(0u);
+                    *reinterpret_cast<u32x4 *>(&rg.b[h][1][to]) = y;
+                }
+            __syncthreads();
+            if (tid < n) {
+                const int k = tid & 31, m = list[e0 + tid].y & 0xffff;
+                char *row = &rg.b[tid >> 5][0][512 * k];
+                *reinterpret_cast<uint16_t *>(row + 32 * ((m >> 4) ^ turned(k)) + 2 * (m & 15)) = (uint16_t)(list[e0 + tid].y >> 16);
+            }
+            __syncthreads();
+            for (int h = 0; h < groups; ++h) {
+                u32x4 fi[4], fj[NF];
+#pragma unroll
+                for (int f = 0; f < 4; ++f) fi[f] = read_turned(&rg.b[h][0][0], 4 * wi + f, fr, fk);
+#pragma unroll
+                for (int g = 0; g < NF; ++g) fj[g] = read_turned(&rg.b[h][1][0], NF * wj + g, fr, fk);
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+#pragma unroll
+                    for (int g = 0; g < NF; ++g) acc[f][g] = Bf16::mma(fj[g], fi[f], acc[f][g]);
+            }
+            __syncthreads();
+        }
+    }
+}
+
 // One tile of 256 rows and 32 NF columns (the rest of a step's 256 columns of B
 // is loaded and not used): accumulator r of (f, g) is row m = 16 f + (lane & 15)
 // of the wave's 64, column n = 16 g + 4 (lane >> 4) + r of its 16 NF; z: which
 // run of k-steps.  NF 8 wherever more than 128 columns are wanted, else 4 or 2.
 template <int NF, bool A_T, class EPI>
-__device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &epi, int64_t m0, int64_t n0, int z) {
+__device__ __forceinline__ void kn_tile(Ring &rg, int (&counts)[64], const KnArgs &a, const KnExtra &extra, const EPI &epi,
+                                        int64_t m0, int64_t n0, int z) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = w & 3, wj = w >> 2;
@@ -517,17 +624,7 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
 #pragma unroll
         for (int g = 0; g < NF; ++g) acc[f][g] = (f32x4)(0.f);
     u32x4 fi[4], fj[NF];
-    // transposed reads: row 8 fk + (fr >> 2) (and 4 below), 16-column slot s
-    const int fx = (fr >> 2) | ((fk & 1) << 2);
-    const int trow = (8 * fk + (fr >> 2)) * 512 + 8 * (fr & 3);
     const char *ri = &rg.b[0][0][(64 * wi + fr) * KBY + 16 * (fk ^ (((fr >> 3) & 1) << 1))];
-    auto tr = [&](const char *half, int s) __attribute__((always_inline)) {
-        const char *p = half + trow + 32 * (s ^ fx);
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * 512));
-        const uint2 a2 = __builtin_bit_cast(uint2, x), b2 = __builtin_bit_cast(uint2, y);
-        return (u32x4){a2.x, a2.y, b2.x, b2.y};
-    };
     if (nstep > 0) {
         issue();
         issue();
@@ -539,11 +636,11 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
             const int so = (n & (NSLOT - 1)) * 2 * HALF;
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
-                if constexpr (A_T) fi[f] = tr(&rg.b[0][0][0] + so, 4 * wi + f);
+                if constexpr (A_T) fi[f] = read_turned(&rg.b[0][0][0] + so, 4 * wi + f, fr, fk);
                 else fi[f] = *reinterpret_cast<const u32x4 *>(ri + so + 16 * f * KBY);
             }
 #pragma unroll
-            for (int g = 0; g < NF; ++g) fj[g] = tr(&rg.b[0][1][0] + so, NF * wj + g);
+            for (int g = 0; g < NF; ++g) fj[g] = read_turned(&rg.b[0][1][0] + so, NF * wj + g, fr, fk);
             read_window_end<4>();
 #pragma unroll
             for (int f = 0; f < 4; ++f)
@@ -561,6 +658,7 @@ __device__ __forceinline__ void kn_tile(Ring &rg, const KnArgs &a, const EPI &ep
         if (!wj) window_end();
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+    if constexpr (A_T) add_extra<NF>(rg, counts, a, extra, acc, m0, n0, s0, s1);
     epi(acc, m0 + 64 * wi, n0 + 16 * NF * wj, lane, z);
 }
 
@@ -578,15 +676,16 @@ struct KnGrid {
 // us; k_nt is the faster that way): 4096 x 32768 x 768 and its transpose 365 us,
 // 1.13 PFLOP/s.
 template <int NF, class E1, class E2>
-__global__ __launch_bounds__(NT, 2) void k_kn2(KnArgs a1, E1 e1, KnGrid g1, KnArgs a2, E2 e2, KnGrid g2) {
+__global__ __launch_bounds__(NT, 2) void k_kn2(KnArgs a1, E1 e1, KnGrid g1, KnArgs a2, E2 e2, KnGrid g2, KnExtra extra) {
     __shared__ Ring rg;
+    __shared__ int counts[64];
     const int b = (int)blockIdx.x, n1 = g1.blocks();
     if (b < n1) {
         const int v = xcd_range(b, n1), r = v / g1.cols;
-        kn_tile<NF, false>(rg, a1, e1, (int64_t)(r % g1.rows) * TILE, (int64_t)(v % g1.cols) * 32 * NF, r / g1.rows);
+        kn_tile<NF, false>(rg, counts, a1, extra, e1, (int64_t)(r % g1.rows) * TILE, (int64_t)(v % g1.cols) * 32 * NF, r / g1.rows);
     } else {
         const int v = xcd_range(b - n1, g2.blocks()), r = v / g2.cols;
-        kn_tile<NF, true>(rg, a2, e2, (int64_t)(r % g2.rows) * TILE, (int64_t)(v % g2.cols) * 32 * NF, r / g2.rows);
+        kn_tile<NF, true>(rg, counts, a2, extra, e2, (int64_t)(r % g2.rows) * TILE, (int64_t)(v % g2.cols) * 32 * NF, r / g2.rows);
     }
 }
 
