@@ -58,6 +58,8 @@ constexpr int NSLOT = 4;
 constexpr int HALF = TILE * KBY;       // one operand's step, 16 KB
 constexpr int NT = 512;
 constexpr int GP = 8;
+// Threads of one launch at most (HIP refuses 2^32); longer work is launched in parts.
+constexpr int64_t LAUNCH = (int64_t)1 << 30;
 
 struct Bf16 {
     typedef f32x4 acc_t;
@@ -168,10 +170,11 @@ inline void plan_runs(NtArgs &a, int cols = TILE) {  // cols: rows of B in a til
     a.panels = (int)((a.m + TILE - 1) / TILE);
     a.tiles = (int)((a.n + cols - 1) / cols);
     double best = 1e300;
+    a.run = a.tiles;  // panels alone are below the limit of blocks
     for (int run = 1; run <= a.tiles; run = run < 32 ? run + 1 : run + run / 16) {
         const int64_t s = (a.tiles + run - 1) / run, blocks = s * a.panels;
         const double cost = (double)((blocks + 255) / 256) * (run + 0.3);
-        if (blocks < (1 << 30) && cost < best * 0.999) {
+        if (blocks * NT < ((int64_t)1 << 32) && cost < best * 0.999) {
             best = cost;
             a.run = run;
         }

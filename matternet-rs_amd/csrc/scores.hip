@@ -302,8 +302,11 @@ void quantize(const T *X, int64_t n, int d, int8_t *codes, int64_t ld, float *sc
     const bool vec = (d * sizeof(T)) % 16 == 0 && aligned16(X);
     auto go = [&](auto L) {
         constexpr int l = decltype(L)::value, block = quantize_block(l), per = block / l;
-        hipLaunchKernelGGL((k_quantize<T, l>), dim3((unsigned)((n + per - 1) / per)), dim3(block), 0, s, X, n, d, vec, codes,
-                           ld, scale);
+        for (int64_t i = 0, m; i < n; i += m) {
+            m = std::min<int64_t>(n - i, mm::LAUNCH / l);
+            hipLaunchKernelGGL((k_quantize<T, l>), dim3((unsigned)((m + per - 1) / per)), dim3(block), 0, s, X + i * d, m, d,
+                               vec, codes + i * ld, ld, scale + i);
+        }
     };
     if (ld <= 16) go(std::integral_constant<int, 2>());
     else if (ld <= 32) go(std::integral_constant<int, 4>());
@@ -368,12 +371,15 @@ extern "C" int mn_dequantize_rows_i8(const int8_t *codes, int64_t ld, const floa
     MN_REQUIRE(X && codes && scale, MN_EINVAL, "mn_dequantize_rows_i8: NULL pointer");
     MN_REQUIRE(aligned16(codes), MN_EINVAL, "mn_dequantize_rows_i8: codes not 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const int64_t pieces = n * (x_type == MN_F32 ? (d + 3) / 4 : (d + 7) / 8);
+    const int64_t row = x_type == MN_F32 ? (d + 3) / 4 : (d + 7) / 8, pieces = n * row;
     auto go = [&](auto U, auto *x) {
         typedef std::remove_pointer_t<decltype(x)> T;
         constexpr int u = decltype(U)::value;
-        hipLaunchKernelGGL((k_dequantize<T, u>), dim3((unsigned)((pieces + 256 * u - 1) / (256 * u))), dim3(256), 0, s, codes,
-                           ld, scale, n, d, (d * sizeof(T)) % 16 == 0 && aligned16(X), x);
+        for (int64_t i = 0, m; i < n; i += m) {
+            m = std::min<int64_t>(n - i, std::max<int64_t>(1, mn::mm::LAUNCH * u / row));
+            hipLaunchKernelGGL((k_dequantize<T, u>), dim3((unsigned)((m * row + 256 * u - 1) / (256 * u))), dim3(256), 0, s,
+                               codes + i * ld, ld, scale + i, m, d, (d * sizeof(T)) % 16 == 0 && aligned16(X), x + i * d);
+        }
     };
     auto size = [&](auto *x) {
         if (pieces >= 1 << 21) go(std::integral_constant<int, 4>(), x);
