@@ -629,10 +629,10 @@ __device__ __forceinline__ void reduce(const Sums &p, int block, int ldp, int d,
     mm::store4<F32>(p.out, i * d + c, min(4, d - c), x);
 }
 template <bool F32>
-__global__ __launch_bounds__(256) void k_reduce(Sums dq, Sums dc, int ldp, int d, const uint16_t *__restrict__ C,
+__global__ __launch_bounds__(256) void k_reduce(Sums dq, Sums dc, int first, int ldp, int d, const uint16_t *__restrict__ C,
                                                 const Row *__restrict__ row, const int32_t *__restrict__ at,
                                                 const float *__restrict__ gs) {
-    const int b = (int)blockIdx.x;
+    const int b = first + (int)blockIdx.x;
     if (b < dq.blocks) reduce<F32>(dq, b, ldp, d, C, row, at, gs);
     else reduce<F32>(dc, b - dq.blocks, ldp, d, C, row, at, gs);
 }
@@ -965,9 +965,10 @@ int backward_impl(const void *Q, const void *C, int64_t t, int64_t v, int32_t d,
         };
         const Sums sq = dQ && last ? sums(p.dq, p.parts, t, dQ, targets) : Sums{};
         const Sums sd = dC && p.splits_c > 1 ? sums(p.dc, p.splits_c, vn, out, nullptr) : Sums{};
-        if (sq.blocks + sd.blocks > 0) {
-            hipLaunchKernelGGL(k_reduce<F32>, dim3((unsigned)(sq.blocks + sd.blocks)), dim3(256), 0, s, sq, sd, p.ldp, d,
-                               (const uint16_t *)C, row, at, gs);
+        for (int b = 0, n; b < sq.blocks + sd.blocks; b += n) {
+            n = (int)std::min<int64_t>(sq.blocks + sd.blocks - b, mm::LAUNCH / 256);
+            hipLaunchKernelGGL(k_reduce<F32>, dim3((unsigned)n), dim3(256), 0, s, sq, sd, b, p.ldp, d, (const uint16_t *)C, row,
+                               at, gs);
             MN_KCHECK(s, "k_reduce");
         }
     }
@@ -983,6 +984,10 @@ static int check_args(const char *who, int32_t x_type, int64_t t, int64_t v, int
                "%s: t <= 2^24, v < 2^31 - 1025, d <= 65536", who);
     MN_REQUIRE(v * ((d + 31) / 32) / 512 < (1 << 30), MN_ENOTSUP, "%s: v d too large for one call", who);
     MN_REQUIRE((t + 255) / 256 * ((v + 255) / 256) < (1 << 30), MN_ENOTSUP, "%s: t v too large for one call", who);
+    // what k_prep copies, 64 bytes a thread: 2^31 of them and a wave for each of t rows
+    const int64_t size = x_type == MN_F32 ? 4 : 2, copied = t + (d * size % 16 ? v : 0);
+    MN_REQUIRE(copied * ((d + 31) / 32 * 32) * size <= (int64_t)1 << 37, MN_ENOTSUP,
+               "%s: more than 128 GB of queries and of items whose rows start off 16-byte borders", who);
     return MN_OK;
 }
 
