@@ -31,23 +31,21 @@ def require_aligned(t: torch.Tensor, dtype, name: str, ndim: int, device=None) -
 
 
 def enqueues(fn):
-    """For calls that return before their work is done (first argument: a
-    tensor, or something with codes): on_device, and with `stream` given it is
-    the current stream inside, so that what is allocated belongs to it, and the
-    inputs' memory is kept until its work on them is done."""
+    """For calls that return before their work is done: on_device, and with
+    `stream` given it is the current stream inside, so that what is allocated
+    belongs to it, and the inputs' memory is kept until its work on them is done."""
     import functools
 
     @functools.wraps(fn)
     def wrapped(*args, stream=None, **kwargs):
-        t = args[0] if args else next(iter(kwargs.values()), None)
-        t = getattr(t, "codes", t)
+        dev = _first_cuda(args, kwargs)
         if stream is None:
-            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() == torch.cuda.current_device():
+            if dev is None or dev.index == torch.cuda.current_device():
                 return fn(*args, **kwargs)
-            with torch.cuda.device(t.device):
+            with torch.cuda.device(dev):
                 return fn(*args, **kwargs)
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.device != stream.device:
-            raise ValueError(f"stream is on {stream.device}, the call's tensors on {t.device}")
+        if dev is not None and dev != stream.device:
+            raise ValueError(f"stream is on {stream.device}, the call's tensors on {dev}")
         with torch.cuda.stream(stream):
             for a in (*args, *kwargs.values()):
                 for t in (a, getattr(a, "codes", None), getattr(a, "scale", None)):
@@ -78,11 +76,11 @@ def to_device(a, device="cuda") -> torch.Tensor:
 
 
 def _first_cuda(args, kwargs):
-    for a in list(args) + list(kwargs.values()):
-        if isinstance(a, torch.Tensor) and a.device.type == "cuda":
+    for a in (*args, *kwargs.values()):
+        if isinstance(a, torch.Tensor) and a.is_cuda:
             return a.device
         for v in (getattr(a, "indptr", None), getattr(a, "keys", None), getattr(a, "codes", None)):
-            if isinstance(v, torch.Tensor) and v.device.type == "cuda":
+            if isinstance(v, torch.Tensor) and v.is_cuda:
                 return v.device
     return None
 
