@@ -1,11 +1,14 @@
 // mm_f32.hpp — the products of mm_tiles.hpp for f32 operands, on the bf16
 // matrix cores.
 //
-// x = h + m + l, 8 + 8 + 8 significant bits cut off one after the other (exact
-// but for subnormal tails), and a product is six bf16 products, mm, lh, hl, mh,
-// hm, hh; what is left out (ml, lm, ll) is below 2^-23 |x||y| and mostly far
-// below: the size of an f32 product's rounding.  Six at the bf16 rate are 2.7
-// times the f32 matrix rate.
+// x = h + m + l, 8 significant bits each (exact but for subnormal tails), and a
+// product is six bf16 products, mm, lh, hl, mh, hm, hh.  h is cut off (rounded, the
+// largest values, which masks are made of, would become infinite), m rounded, so
+// that |m| <= 2^-7 |x| and |l| <= 2^-16 |x| with either sign: what is left out (ml,
+// lm, ll) is up to 2^-22 |x||y| but 0.4 2^-24 in the mean square, and has no sign of
+// its own that would add up over a sum (with m cut off too: up to 2^-21, in the
+// mean 0.7 2^-24 towards zero).  Six at the bf16 rate are 2.7 times the f32 matrix
+// rate.
 //
 // A block has a tile of 256 x 128 (or 64 columns), eight waves of 64 x 64 = 4 x
 // 4 tiles of 16 x 16.  A step is 32 k's.  LDS holds the three planes of two
@@ -54,7 +57,7 @@ struct alignas(1024) Planes {
 
 __device__ __forceinline__ int quad_swizzle(int a) { return ((a & 1) << 1) ^ ((a >> 1) & 1) * 3; }
 
-// 8 values to three times 8 bf16: the upper halves of x, x - h, x - h - m.  (The
+// 8 values to three times 8 bf16: the upper half of x, x - h rounded, x - h - m.  (The
 // differences as dot products of bf16 pairs with (-1, 0) and (0, -1) are exact
 // too and fewer instructions, but hold up the matrix pipe: 2.99 -> 3.28 ms for a
 // step of 1024 x 100000 x 768.)
@@ -68,9 +71,10 @@ __device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&s)[3]) {
             return u - __uint_as_float(__float_as_uint(u) & 0xffff0000u);
         };
         const float x = v[2 * p], y = v[2 * p + 1], x1 = rest(x), y1 = rest(y);
+        const uint32_t m = bf16_pair(x1, y1);
         s[0][p] = upper(x, y);
-        s[1][p] = upper(x1, y1);
-        s[2][p] = upper(rest(x1), rest(y1));
+        s[1][p] = m;
+        s[2][p] = upper(x1 - __uint_as_float(m << 16), y1 - __uint_as_float(m & 0xffff0000u));
     }
 }
 

@@ -45,10 +45,12 @@
 namespace mn {
 namespace mm {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -60,6 +62,12 @@ constexpr int NT = 512;
 constexpr int GP = 8;
 // Threads of one launch at most (HIP refuses 2^32); longer work is launched in parts.
 constexpr int64_t LAUNCH = (int64_t)1 << 30;
+
+__device__ __forceinline__ uint16_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+__device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {  // (one instruction so; two conversions took two and an or)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2));
+}
 
 struct Bf16 {
     typedef f32x4 acc_t;
@@ -690,12 +698,6 @@ __global__ __launch_bounds__(NT, 2) void k_kn2(KnArgs a1, E1 e1, KnGrid g1, KnAr
         const int v = xcd_range(b - n1, g2.blocks()), r = v / g2.cols;
         kn_tile<NF, true>(rg, counts, a2, extra, e2, (int64_t)(r % g2.rows) * TILE, (int64_t)(v % g2.cols) * 32 * NF, r / g2.rows);
     }
-}
-
-__device__ __forceinline__ uint16_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
-__device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
-    return (uint32_t)bf16_bits(x) | ((uint32_t)bf16_bits(y) << 16);
 }
 
 // the first n (<= 4) of x to element e of an f32 or bf16 array, any alignment
