@@ -6,9 +6,9 @@ no [t, v] matrix of logits is kept.  Has no counterpart in the reference.
 softmax_loss is the whole of it with autograd.  softmax_stats, softmax_merge
 and softmax_backward are its parts, for tables whose rows are spread over
 processes (c_offset, as in knn_l2sq_qc) and for steps captured into a graph.
-softmax_loss with gradients is refused in a capture: a backward pass of autograd
-that is captured while an eager graph of the same leaves lives ends the process,
-which no check here could see coming.
+softmax_loss with gradients is refused in a capture, and so is its backward pass
+on a stream that is being captured: a backward pass of autograd that is captured
+while an eager graph of the same leaves lives ends the process.
 
 The calls only enqueue on the stream (default: the current one).  With `stream`
 given the caller orders it after the work that made the inputs, as with
@@ -172,6 +172,8 @@ class _SoftmaxLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        if torch.cuda.is_current_stream_capturing():  # the loss was computed on this stream before
+            raise RuntimeError("softmax_loss's backward pass in a graph capture: capture softmax_stats and softmax_backward")
         tensors = ctx.saved_tensors
         sizes, rest, target, share, scale = ctx.of
         inputs = (*tensors, *sizes) if sizes else _inputs(*tensors)
