@@ -317,11 +317,12 @@ __global__ __launch_bounds__(NT, 2) void k_nt(NtArgs a, EPI epi) {
     epi.finish(sh, i0 + 64 * wi, slice * 2 + wj, lane);
 }
 
-// Up to 64 queries against many rows: that the bytes of B are in flight is all
-// that counts.  The queries lie in LDS ([k-step][query][64 bytes], pieces at c ^
-// 2 ((query >> 3) & 1): no bank conflicts), a wave takes 16 rows of B at a time
-// from memory to registers, a turn of k-steps ahead of their products (the next
-// 16 rows' first turn too), and the block's waves go through B side by side.
+// Few queries against many rows (up to 64, or more in groups of 16 to 64 where
+// that is the faster): that the bytes of B are in flight is all that counts.  The
+// queries lie in LDS ([k-step][query][64 bytes], pieces at c ^ 2 ((query >> 3) & 1):
+// no bank conflicts), a wave takes 16 rows of B at a time from memory to
+// registers, a turn of k-steps ahead of their products (the next 16 rows' first
+// turn too), and the block's waves go through B side by side.
 // One query on 1M rows of 768 codes (768 MB): 132 us, 5.8 TB/s; 512 blocks (768:
 // 134, 1024: 145, 256: 181), turns of two k-steps (one: 162, three: 138, four:
 // 137), through the caches (past them: 150).  f32, whose products take longer
@@ -408,7 +409,7 @@ __global__ __launch_bounds__(NT) void k_few(FewArgs a, EPI epi) {
     };
     const char *row = nullptr;
     int kc = 0;
-    // four k-steps: those after them on their way first, of the next rows too
+    // a turn of U k-steps: those after them on their way first, of the next rows too
     auto turn = [&](u32x4 (&x)[U], u32x4 (&next)[U]) __attribute__((always_inline)) {
         const bool last = kc + U >= a.nk;
         const int64_t gn = last ? g + stride : g;

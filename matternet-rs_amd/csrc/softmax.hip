@@ -639,9 +639,6 @@ __global__ __launch_bounds__(256) void k_reduce(Sums dq, Sums dc, int first, int
 
 inline size_t up(size_t x) { return (x + 255) / 256 * 256; }
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
-inline unsigned grid1(int64_t n, int per, int64_t most = 1 << 20) {
-    return (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + per - 1) / per, most));
-}
 
 // Sizes of one call and where its workspace holds what.
 struct Plan {
