@@ -31,9 +31,9 @@
 // as planes in memory, loaded directly and read transposed, it took as long (4%
 // longer to 2% less): half as many bytes again come from L2.
 //
-// 1024 x 100000 x 768: logits with the loss's sums 690 us (1.37 PFLOP/s of bf16
-// products, 228 TFLOP/s of f32 ones; the f32 matrix rate of a large library
-// product is 154), the gradients' two products 790 us for 65536 rows.  A step
+// 1024 x 100000 x 768: logits with the loss's sums 672 us (1.40 PFLOP/s of bf16
+// products, 234 TFLOP/s of f32 ones; the f32 matrix rate of a large library
+// product is 154), the gradients' two products 985 us for 65536 rows.  A step
 // takes 4.4 thousand cycles on a few blocks, 5 to 5.4 on all, for 3.1 of matrix
 // instructions (490 us if there were nothing else): the reading half's window is
 // the longer one, and what comes from L2 slows it when all blocks run (590 us

@@ -22,13 +22,13 @@
 // loads repeat it into the slot that nobody reads any more: the count stays.
 //
 // What bounds it: the chip's power, then LDS.  4096 x 131072 x 768 in bf16
-// without the epilogue takes 618 us, 1.33 PFLOP/s: 65% of the matrix pipe at the
-// 1.95 GHz that the chip then holds.  A large library product (8192^3, 1.33 to
-// 1.40) fills 87% of the pipe and gets 1.5 GHz for it.  A step's 32 matrix
-// instructions a wave take a SIMD 512 cycles for each of its two waves; its
-// fragments (96 KB a block) and the loads that land (32 KB) take LDS the same
-// 1024 at 128 bytes a cycle.  An epilogue is not hidden: the other wave of the
-// SIMD has one window to give.
+// without the epilogue takes 618 us, 1.33 PFLOP/s; with the softmax loss's 667, 62%
+// of the matrix pipe at the 1.90 GHz that the chip then holds.  A large library
+// product (8192^3, 1.33 to 1.40) fills 87% of the pipe and gets 1.60 GHz for it.
+// A step's 32 matrix instructions a wave take a SIMD 512 cycles for each of its
+// two waves; its fragments (96 KB a block) and the loads that land (32 KB) take LDS
+// the same 1024 at 128 bytes a cycle.  An epilogue is not hidden: the other wave of
+// the SIMD has one window to give.
 //
 // LDS layouts, free of bank conflicts.  Rows of k: a row's k-step is 64 bytes,
 // piece c (16 bytes) of row r at c ^ 2 ((r >> s) & 1), s = 3 where a fragment's
@@ -685,8 +685,8 @@ struct KnGrid {
 // processors that the last round of the first leaves idle: A [m][k] first, then
 // A [k][m].  Bound as k_nt, with twice the read instructions for a transposed
 // fragment; the loads are issued among the products (in the reading window: 379
-// us; k_nt is the faster that way): 4096 x 32768 x 768 and its transpose 365 us,
-// 1.13 PFLOP/s.
+// us; k_nt is the faster that way): 4096 x 32768 x 768 and its transpose 351 to 373
+// us, 1.1 PFLOP/s, with the extra entries of the second.
 template <int NF, class E1, class E2>
 __global__ __launch_bounds__(NT, 2) void k_kn2(KnArgs a1, E1 e1, KnGrid g1, KnArgs a2, E2 e2, KnGrid g2, KnExtra extra) {
     __shared__ Ring rg;

@@ -205,10 +205,11 @@ struct ScoreEpi {
     }
     // 16 rows by 256 bytes at a time through LDS (272 bytes a row), so that a
     // store of the wave is 256 bytes of each of four rows; rows of Y on 16-byte
-    // borders or not (a store may start anywhere).  4096 x 131072 x 768 to bf16:
-    // 560 us so, 605 with 128 bytes of each of 8 rows, 830 with 64 of each of 16
-    // (D of the softmax loss, whose row stride is ours, takes the same time with
-    // all three); without any store 475, without this whole step 337.
+    // borders or not (a store may start anywhere).  4096 x 131072 x 768 takes 566 us
+    // to bf16, 798 to f32.  On a card where it took 560: 605 with 128 bytes of each
+    // of 8 rows, 830 with 64 of each of 16 (D of the softmax loss, whose row stride
+    // is ours, takes the same time with all three); without any store 475, without
+    // this whole step 337.
     __device__ __forceinline__ void tile(Shared &sh, char *stage, mm::i32x4 (&acc)[4][8], int64_t j0, int lane, int par) {
         constexpr int E = 16 / sizeof(T), PASS = sizeof(T) / 2;  // values of a piece; passes of 128 / PASS columns
         const int jl = 8 * (lane >> 4);

@@ -247,8 +247,8 @@ __global__ __launch_bounds__(256) void k_prep(Pack q, Pack c, Rows r) {
 // Per lane and row the largest logit so far (m2, base 2, rounded: the number
 // that every exponent is taken from) and the sum of exp of the rest, the
 // target's left out; joined over the lanes and written per run of tiles and
-// half of the columns.  An element costs a max, an fma, an exp and an add: 701 us
-// for 4096 x 131072 x 768 in bf16, 618 without.
+// half of the columns.  An element costs a max, an fma, an exp and an add: 667 to
+// 694 us for 4096 x 131072 x 768 in bf16, 618 without.
 struct StatsEpi {
     struct Shared {};
     static constexpr bool FETCH = false;

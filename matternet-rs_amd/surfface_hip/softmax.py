@@ -191,8 +191,8 @@ def softmax_loss(queries: torch.Tensor, items: torch.Tensor, targets: torch.Tens
     gradient 0).  reduction: "mean" over the queries that take part (0 when
     there is none), "sum" or "none".  In a graph capture only without gradients
     (else RuntimeError): capture softmax_stats and softmax_backward.  A step of
-    few rows is bound by the host: 123 us, 67 inside
-    torch.autograd.set_multithreading_enabled(False), 47 with those two."""
+    few rows is bound by the host: 130 us, 68 inside
+    torch.autograd.set_multithreading_enabled(False), 49 with those two."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("reduction must be 'mean', 'sum' or 'none'")
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad and x.is_cuda
