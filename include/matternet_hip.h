@@ -648,7 +648,7 @@ int mn_bf16_last_stats(mn_knn_stats *out);
 /* Per row a = max |x|: scale = a / 127, code = rint(x (127 (1 / a))) (f32, ties to
  * even), codes d .. ld - 1 of a row 0.  X [n][d] MN_F32 or MN_BF16.  A row of
  * zeros: scale 0, codes 0.  A row with an infinity or a NaN: scale NaN (so
- * every score with it is NaN), codes 0. */
+ * every score with it is NaN), codes 0.  n < 2^31 - 1, n d < 2^40 (MN_ENOTSUP). */
 int mn_quantize_rows_i8(const void *X, int32_t x_type, int64_t n, int32_t d, int8_t *codes,
                         int64_t ld, float *scale, void *stream);
 /* X [n][d] = code * scale, MN_F32, or rounded to MN_BF16. */
@@ -669,7 +669,8 @@ int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, 
  * negative target has no part: loss 0, gradient 0, and what it holds (a NaN)
  * reaches no other row.  All other values have to be finite: an infinity or a
  * NaN makes the results that it meets NaN.  The type's lowest value in an item
- * (a mask) is finite; a logit below -2^127 counts as -infinity.
+ * (a mask) is finite; a logit below -2^127 counts as -infinity, one above 2^127
+ * makes its row NaN.
  * mn_softmax_stats writes per row rest = log sum exp z over the items but the
  * target, zt = the target's logit (-inf where it is not among the rows here),
  * loss = log(1 + exp(rest - zt)) (+inf where zt is -inf), and where mean is not
@@ -688,7 +689,9 @@ int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, 
  * bf16: the entries (p - [target]) of the logits' gradient are rounded to bf16
  * for the two products with C and Q (both get the target's rounding back); sums
  * are f32.  f32: products of three-way split bf16 values, to f32 accuracy.
- * Results do not depend on the run: no atomics. */
+ * Results do not depend on the run: no atomics.
+ * t <= 2^24, v < 2^31 - 1025, d <= 65536, and at most 128 GB of queries and of
+ * items whose rows start off 16-byte borders, which are copied (MN_ENOTSUP). */
 int mn_softmax_workspace(int64_t t, int64_t v, int32_t d, int32_t x_type, int32_t backward,
                          size_t *bytes);
 int mn_softmax_stats(const void *Q, const void *C, int32_t x_type, int64_t t, int64_t v, int32_t d,
