@@ -669,8 +669,8 @@ int mn_scores_i8(const int8_t *Q, int64_t ldq, const float *q_scale, int64_t m, 
  * negative target has no part: loss 0, gradient 0, and what it holds (a NaN)
  * reaches no other row.  All other values have to be finite: an infinity or a
  * NaN makes the results that it meets NaN.  The type's lowest value in an item
- * (a mask) is finite; a logit below -2^127 counts as -infinity, one above 2^127
- * makes its row NaN.
+ * (a mask) is finite; a logit below -2^127 may count as -infinity, one above 2^127
+ * may make its row NaN.
  * mn_softmax_stats writes per row rest = log sum exp z over the items but the
  * target, zt = the target's logit (-inf where it is not among the rows here),
  * loss = log(1 + exp(rest - zt)) (+inf where zt is -inf), and where mean is not
